@@ -658,6 +658,263 @@ std::vector<at::Tensor> polynomial_sincos_f32(at::Tensor angles, std::vector<dou
 }
 
 // ---------------------------------------------------------------------------
+// query / key heads ahead of the attention: norm and rotation by positions
+// ---------------------------------------------------------------------------
+
+// The operand as the kernels take it: rows of a contiguous head dimension,
+// pointer and strides whole multiples of four elements, or a copy of it.
+at::Tensor head_rows(const at::Tensor& t) {
+    bool ok = (t.size(3) <= 1 || t.stride(3) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 4 == 0);
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Element strides (batch, sequence, head) of a tensor whose dimensions b, s
+// and h those are; a dimension of one element has none.
+void row_strides(int64_t (&out)[3], const at::Tensor& t, int b, int s, int h) {
+    const int dim[3] = {b, s, h};
+    for (int i = 0; i < 3; ++i) out[i] = t.size(dim[i]) > 1 ? t.stride(dim[i]) : 0;
+}
+
+void check_heads(const at::Tensor& t, const char* name, const char* shape) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, name,
+                " must be float16 or bfloat16");
+    TORCH_CHECK(t.dim() == 4, name, " must have shape ", shape);
+}
+
+void check_head_pair(const at::Tensor& q, const at::Tensor& k, const char* qn, const char* kn, int seq_dim,
+                     const char* shape) {
+    check_heads(q, qn, shape);
+    check_heads(k, kn, shape);
+    const int head_dim = 3 - seq_dim;
+    TORCH_CHECK(q.scalar_type() == k.scalar_type(), qn, " and ", kn, " must have the same dtype");
+    TORCH_CHECK(q.get_device() == k.get_device(), qn, " and ", kn, " must be on the same CUDA device");
+    TORCH_CHECK(q.size(0) == k.size(0), qn, " and ", kn, " batch sizes must match");
+    TORCH_CHECK(q.size(seq_dim) == k.size(seq_dim), qn, " and ", kn, " sequence lengths must match");
+    TORCH_CHECK(q.size(3) == k.size(3), qn, " and ", kn, " head dimensions must match");
+    TORCH_CHECK(q.size(head_dim) > 0 && k.size(head_dim) > 0, qn, " and ", kn, " must contain at least one head");
+    TORCH_CHECK(q.size(head_dim) <= 65536 && k.size(head_dim) <= 65536, "at most 65536 heads are supported");
+    TORCH_CHECK(q.size(3) > 0 && q.size(3) % 8 == 0 && q.size(3) <= 256,
+                "head_dim must be a positive multiple of eight up to 256");
+    TORCH_CHECK(q.size(0) == 0 || q.size(seq_dim) <= std::numeric_limits<int32_t>::max() / q.size(0),
+                "at most 2^31 - 1 tokens are supported");
+}
+
+// The frequencies and positions of a call; the tensors it returns are held
+// until the launch.
+struct Angles {
+    at::Tensor increments, positions, axes;
+};
+
+Angles fill_angles(spline_hip_qk_rope& a, const at::Tensor& like, int64_t b, int64_t s, int64_t d,
+                   const at::Tensor& increments, const c10::optional<at::Tensor>& positions,
+                   const c10::optional<at::Tensor>& frequency_axes, bool interleaved) {
+    Angles held;
+    auto check = [&](const at::Tensor& t, const char* name) {
+        TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+        TORCH_CHECK(t.get_device() == like.get_device(), name, " must be on the same CUDA device as q and k");
+    };
+    check(increments, "phase_increments");
+    TORCH_CHECK(increments.scalar_type() == at::kInt, "phase_increments must be int32");
+    TORCH_CHECK(increments.dim() == 1, "phase_increments must be one-dimensional");
+    const int64_t f = increments.numel();
+    TORCH_CHECK(f % 4 == 0 && 2 * f <= d,
+                "phase_increments must hold a multiple of four frequencies, at most head_dim / 2, got ", f);
+    held.increments = increments.contiguous();
+    a.phase_increments = held.increments.data_ptr();
+    a.rotary_dim = 2 * f;
+    a.interleaved = interleaved ? 1 : 0;
+    a.position_bytes = 4;
+    a.axes = 1;
+    if (frequency_axes.has_value() && frequency_axes->defined()) {
+        TORCH_CHECK(positions.has_value() && positions->defined(), "frequency_axes needs positions");
+        const at::Tensor& x = *frequency_axes;
+        check(x, "frequency_axes");
+        TORCH_CHECK(x.scalar_type() == at::kInt, "frequency_axes must be int32");
+        TORCH_CHECK(x.dim() == 1 && x.numel() == f, "frequency_axes must hold one axis for each frequency");
+        held.axes = x.contiguous();
+        a.frequency_axes = held.axes.data_ptr<int32_t>();
+    }
+    if (positions.has_value() && positions->defined()) {
+        const at::Tensor& p = *positions;
+        check(p, "positions");
+        TORCH_CHECK(p.scalar_type() == at::kInt || p.scalar_type() == at::kLong, "positions must be int32 or int64");
+        const bool many = held.axes.defined();
+        const int64_t n = p.dim();
+        TORCH_CHECK(many ? n == 3 : n == 1 || n == 2, many ? "positions must have shape [axes, batch, sequence]"
+                                                           : "positions must have shape [sequence] or [batch, sequence]");
+        TORCH_CHECK(p.size(n - 1) == s && (n == 1 || p.size(n - 2) == b),
+                    "positions must agree with q and k in batch and sequence length");
+        TORCH_CHECK(!many || p.size(0) > 0, "positions must have at least one axis");
+        held.positions = p;
+        a.positions = p.data_ptr();
+        a.position_bytes = p.scalar_type() == at::kLong ? 8 : 4;
+        a.position_strides[2] = p.stride(n - 1);
+        if (n > 1) a.position_strides[1] = p.stride(n - 2);
+        if (many) {
+            a.position_strides[0] = p.stride(0);
+            a.axes = p.size(0);
+        }
+    }
+    return held;
+}
+
+at::Tensor fill_weight(spline_hip_qk_rope& a, const void* spline_hip_qk_rope::*field, const at::Tensor& q,
+                       const c10::optional<at::Tensor>& w, const char* name) {
+    if (!w.has_value() || !w->defined()) return at::Tensor();
+    TORCH_CHECK(w->is_cuda() && w->get_device() == q.get_device(), name, " must be on the same CUDA device as q and k");
+    TORCH_CHECK(w->scalar_type() == q.scalar_type() || w->scalar_type() == at::kFloat, name,
+                " must be float32 or of q's dtype");
+    TORCH_CHECK(w->dim() == 1 && w->numel() == q.size(3), name, " must have shape [head_dim]");
+    at::Tensor held = w->contiguous();
+    a.*field = held.data_ptr();
+    a.weight_f32 = w->scalar_type() == at::kFloat ? 1 : 0;
+    return held;
+}
+
+void check_weight_pair(const at::Tensor& qw, const at::Tensor& kw) {
+    TORCH_CHECK(!qw.defined() || !kw.defined() || qw.scalar_type() == kw.scalar_type(),
+                "q_weight and k_weight must have the same dtype");
+}
+
+void fill_sizes(spline_hip_qk_rope& a, int64_t b, int64_t s, int64_t hq, int64_t hk, int64_t d) {
+    a.batch = b;
+    a.sequence_length = s;
+    a.q_heads = hq;
+    a.k_heads = hk;
+    a.head_dim = d;
+}
+
+const char* const kTokensFirst = "[batch, sequence, heads, head_dim]";
+const char* const kHeadsFirst = "[batch, heads, sequence, head_dim]";
+
+// Norm (or not) and rotation of q [B, S, Hq, D], k [B, S, Hk, D] -> [B, H, S, D].
+std::vector<at::Tensor> heads_forward(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& qw,
+                                      const c10::optional<at::Tensor>& kw, const at::Tensor& increments,
+                                      const c10::optional<at::Tensor>& positions,
+                                      const c10::optional<at::Tensor>& frequency_axes, double eps, bool interleaved,
+                                      bool norm) {
+    check_head_pair(q, k, "q", "k", 1, kTokensFirst);
+    c10::OptionalDeviceGuard guard(q.device());
+    const int64_t b = q.size(0), s = q.size(1), hq = q.size(2), hk = k.size(2), d = q.size(3);
+    spline_hip_qk_rope a{};
+    fill_sizes(a, b, s, hq, hk, d);
+    const Angles angles = fill_angles(a, q, b, s, d, increments, positions, frequency_axes, interleaved);
+    const at::Tensor hw = fill_weight(a, &spline_hip_qk_rope::q_weight, q, qw, "q_weight");
+    const at::Tensor hw2 = fill_weight(a, &spline_hip_qk_rope::k_weight, q, kw, "k_weight");
+    check_weight_pair(hw, hw2);
+    const at::Tensor qr = head_rows(q), kr = head_rows(k);
+    at::Tensor q_out = at::empty({b, hq, s, d}, q.options()), k_out = at::empty({b, hk, s, d}, k.options());
+    a.q = qr.data_ptr();
+    a.k = kr.data_ptr();
+    a.q_out = q_out.data_ptr();
+    a.k_out = k_out.data_ptr();
+    a.eps = (float)eps;
+    row_strides(a.q_strides, qr, 0, 1, 2);
+    row_strides(a.k_strides, kr, 0, 1, 2);
+    row_strides(a.q_out_strides, q_out, 0, 2, 1);
+    row_strides(a.k_out_strides, k_out, 0, 2, 1);
+    void* st = current_stream(q);
+    const bool bf = q.scalar_type() == at::kBFloat16;
+    check_launch(norm ? (bf ? launch_qk_norm_rope_bf16 : launch_qk_norm_rope_fp16)(&a, st)
+                      : (bf ? launch_rope_axes_bf16 : launch_rope_axes_fp16)(&a, 0, st),
+                 st);
+    return {q_out, k_out};
+}
+
+std::vector<at::Tensor> qk_norm_rope_fwd(at::Tensor q, at::Tensor k, c10::optional<at::Tensor> q_weight,
+                                         c10::optional<at::Tensor> k_weight, at::Tensor phase_increments,
+                                         c10::optional<at::Tensor> positions,
+                                         c10::optional<at::Tensor> frequency_axes, double eps, bool interleaved) {
+    return heads_forward(q, k, q_weight, k_weight, phase_increments, positions, frequency_axes, eps, interleaved, true);
+}
+
+std::vector<at::Tensor> rope_axes_fwd(at::Tensor q, at::Tensor k, at::Tensor phase_increments, at::Tensor positions,
+                                      at::Tensor frequency_axes, bool interleaved) {
+    return heads_forward(q, k, c10::nullopt, c10::nullopt, phase_increments, positions, frequency_axes, 0.0,
+                         interleaved, false);
+}
+
+// Gradients [B, H, S, D] at rope_axes_fwd's outputs -> those at q and k [B, S, H, D]:
+// the rotation by the negative angles.
+std::vector<at::Tensor> rope_axes_bwd(at::Tensor dq_out, at::Tensor dk_out, at::Tensor phase_increments,
+                                      at::Tensor positions, at::Tensor frequency_axes, bool interleaved) {
+    check_head_pair(dq_out, dk_out, "dq_out", "dk_out", 2, kHeadsFirst);
+    c10::OptionalDeviceGuard guard(dq_out.device());
+    const int64_t b = dq_out.size(0), s = dq_out.size(2), hq = dq_out.size(1), hk = dk_out.size(1), d = dq_out.size(3);
+    spline_hip_qk_rope a{};
+    fill_sizes(a, b, s, hq, hk, d);
+    const Angles angles = fill_angles(a, dq_out, b, s, d, phase_increments, positions, frequency_axes, interleaved);
+    const at::Tensor qr = head_rows(dq_out), kr = head_rows(dk_out);
+    at::Tensor dq = at::empty({b, s, hq, d}, dq_out.options()), dk = at::empty({b, s, hk, d}, dk_out.options());
+    a.q = qr.data_ptr();
+    a.k = kr.data_ptr();
+    a.q_out = dq.data_ptr();
+    a.k_out = dk.data_ptr();
+    row_strides(a.q_strides, qr, 0, 2, 1);
+    row_strides(a.k_strides, kr, 0, 2, 1);
+    row_strides(a.q_out_strides, dq, 0, 1, 2);
+    row_strides(a.k_out_strides, dk, 0, 1, 2);
+    void* st = current_stream(dq_out);
+    check_launch((dq_out.scalar_type() == at::kBFloat16 ? launch_rope_axes_bf16 : launch_rope_axes_fp16)(&a, 1, st), st);
+    return {dq, dk};
+}
+
+// [dq, dk, dq_weight, dk_weight], the last two undefined without their weight.
+std::vector<c10::optional<at::Tensor>> qk_norm_rope_bwd(
+    at::Tensor q, at::Tensor k, c10::optional<at::Tensor> q_weight, c10::optional<at::Tensor> k_weight,
+    at::Tensor phase_increments, c10::optional<at::Tensor> positions, c10::optional<at::Tensor> frequency_axes,
+    at::Tensor dq_out, at::Tensor dk_out, double eps, bool interleaved) {
+    check_head_pair(q, k, "q", "k", 1, kTokensFirst);
+    check_head_pair(dq_out, dk_out, "dq_out", "dk_out", 2, kHeadsFirst);
+    const int64_t b = q.size(0), s = q.size(1), hq = q.size(2), hk = k.size(2), d = q.size(3);
+    TORCH_CHECK(dq_out.scalar_type() == q.scalar_type() && dq_out.get_device() == q.get_device() &&
+                    dq_out.size(0) == b && dq_out.size(1) == hq && dq_out.size(2) == s && dq_out.size(3) == d &&
+                    dk_out.size(1) == hk,
+                "dq_out and dk_out must match q and k");
+    c10::OptionalDeviceGuard guard(q.device());
+    spline_hip_qk_rope a{};
+    fill_sizes(a, b, s, hq, hk, d);
+    const Angles angles = fill_angles(a, q, b, s, d, phase_increments, positions, frequency_axes, interleaved);
+    const at::Tensor qw = fill_weight(a, &spline_hip_qk_rope::q_weight, q, q_weight, "q_weight");
+    const at::Tensor kw = fill_weight(a, &spline_hip_qk_rope::k_weight, q, k_weight, "k_weight");
+    check_weight_pair(qw, kw);
+    const at::Tensor qr = head_rows(q), kr = head_rows(k), dqr = head_rows(dq_out), dkr = head_rows(dk_out);
+    at::Tensor dq = at::empty({b, s, hq, d}, q.options()), dk = at::empty({b, s, hk, d}, k.options());
+    const bool empty = b == 0 || s == 0;  // a sum over no rows
+    auto weight_grad = [&](const at::Tensor& w) -> c10::optional<at::Tensor> {
+        if (!w.defined()) return c10::nullopt;
+        return empty ? at::zeros({d}, w.options()) : at::empty({d}, w.options());
+    };
+    const c10::optional<at::Tensor> dqw = weight_grad(qw), dkw = weight_grad(kw);
+    at::Tensor ws;
+    if (dqw || dkw) {
+        ws = at::empty({spline_hip_qk_norm_rope_bwd_bytes(d) / 4}, q.options().dtype(at::kFloat));
+        a.dw_workspace = ws.data_ptr<float>();
+        if (dqw) a.dq_weight = dqw->data_ptr();
+        if (dkw) a.dk_weight = dkw->data_ptr();
+    }
+    a.q = qr.data_ptr();
+    a.k = kr.data_ptr();
+    a.dq_out = dqr.data_ptr();
+    a.dk_out = dkr.data_ptr();
+    a.q_out = dq.data_ptr();
+    a.k_out = dk.data_ptr();
+    a.eps = (float)eps;
+    row_strides(a.q_strides, qr, 0, 1, 2);
+    row_strides(a.k_strides, kr, 0, 1, 2);
+    row_strides(a.dq_out_strides, dqr, 0, 2, 1);
+    row_strides(a.dk_out_strides, dkr, 0, 2, 1);
+    row_strides(a.q_out_strides, dq, 0, 1, 2);
+    row_strides(a.k_out_strides, dk, 0, 1, 2);
+    void* st = current_stream(q);
+    check_launch((q.scalar_type() == at::kBFloat16 ? launch_qk_norm_rope_bwd_bf16 : launch_qk_norm_rope_bwd_fp16)(&a, st),
+                 st);
+    return {dq, dk, dqw, dkw};
+}
+
+// ---------------------------------------------------------------------------
 // fused attention (the runtime behind sfu_repro.fa4; FA4's flash_attn_fwd,
 // src/sfu_repro/fa4.py:356-428): q [B, S, Hq, 128], k and v [B, S, Hkv, 128]
 // BF16 with a contiguous head dimension -> out [B, S, Hq, 128], lse [B, Hq, S]
@@ -1426,6 +1683,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                 launch_rope_apply_native_bf16);
           },
           "Fused native BF16 Q/K rotary embedding and transpose");
+
+    // query / key heads ahead of the attention
+    m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, py::arg("q"), py::arg("k"), py::arg("q_weight"),
+          py::arg("k_weight"), py::arg("phase_increments"), py::arg("positions") = c10::nullopt,
+          py::arg("frequency_axes") = c10::nullopt, py::arg("eps") = 1e-6, py::arg("interleaved") = true,
+          "RMS norm of each query / key head and its rotation; q [B,S,Hq,D], k [B,S,Hk,D] -> "
+          "[q [B,Hq,S,D], k [B,Hk,S,D]]");
+    m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, py::arg("q"), py::arg("k"), py::arg("q_weight"),
+          py::arg("k_weight"), py::arg("phase_increments"), py::arg("positions"), py::arg("frequency_axes"),
+          py::arg("dq_out"), py::arg("dk_out"), py::arg("eps") = 1e-6, py::arg("interleaved") = true,
+          "Gradients of qk_norm_rope_fwd -> [dq, dk, dq_weight, dk_weight] (None without a weight)");
+    m.def("rope_axes_fwd", &rope_axes_fwd, py::arg("q"), py::arg("k"), py::arg("phase_increments"),
+          py::arg("positions"), py::arg("frequency_axes"), py::arg("interleaved") = true,
+          "Rotary embedding by positions [axes,B,S]; q [B,S,Hq,D], k [B,S,Hk,D] -> [q [B,Hq,S,D], k [B,Hk,S,D]]");
+    m.def("rope_axes_bwd", &rope_axes_bwd, py::arg("dq_out"), py::arg("dk_out"), py::arg("phase_increments"),
+          py::arg("positions"), py::arg("frequency_axes"), py::arg("interleaved") = true,
+          "Gradients of rope_axes_fwd: the inverse rotation, [B,H,S,D] -> [B,S,H,D]");
 
     // fused attention
     m.def("flash_attn_fwd_bf16", &flash_attn_fwd_bf16, py::arg("q"), py::arg("k"), py::arg("v"),

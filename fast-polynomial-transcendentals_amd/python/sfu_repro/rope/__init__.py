@@ -3,3 +3,7 @@
 
 Importing this package performs no model or runtime monkey-patching.
 """
+
+from .heads import axis_sections, phase_increments, qk_norm_rope, rope_axes
+
+__all__ = ["axis_sections", "phase_increments", "qk_norm_rope", "rope_axes"]

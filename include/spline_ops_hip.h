@@ -508,6 +508,64 @@ int launch_rope_sincos_fixed_lut_fp16_compute(void* out, const void* phase_incre
              int64_t q_heads, int64_t k_heads, int64_t head_dim, void* stream);
 SPLINE_HIP_ROPE_APPLY_LAUNCHERS(SPLINE_HIP_DECLARE_ROPE_APPLY)
 
+/* ---- query / key heads ahead of the attention ------------------------------
+ * No counterpart in the reference, whose fused RoPE rotates interleaved pairs
+ * by positions 0..S-1 and leaves the norm to the model
+ * (src/sfu_repro/fa4.py:500-549).
+ *
+ * q [B, S, Hq, D] and k [B, S, Hk, D] -> q_out [B, Hq, S, D], k_out
+ * [B, Hk, S, D], 16-bit:
+ *   n = x / sqrt(mean(x^2) + eps), u = n w       (qk_norm_rope only)
+ *   (y_a, y_b) = (u_a cos t - u_b sin t, u_a sin t + u_b cos t)
+ * over the rotary_dim / 2 pairs of a head: elements (2i, 2i + 1) if
+ * interleaved, else (i, i + rotary_dim / 2); elements from rotary_dim on are
+ * not rotated.  t = 2 pi 2^-32 (position * phase_increments[i] mod 2^32), so a
+ * position may be any integer.  All arithmetic is FP32 with one rounding of
+ * each result.
+ *
+ * head_dim a multiple of 8, at most 256; rotary_dim a multiple of 8 up to
+ * head_dim; at most 65536 heads and 2^31 - 1 tokens.  Strides are in elements;
+ * the head dimension is contiguous; every operand's pointer and strides are
+ * multiples of 4 elements (8 bytes), and of 8 (16 bytes) for the widest
+ * accesses.
+ *
+ * launch_qk_norm_rope_bwd_*: q_out and k_out receive the gradients at q and k
+ * (strides q_out_strides, k_out_strides), dq_out and dk_out hold those at the
+ * forward's outputs, dq_weight and dk_weight receive those at the weights that
+ * are not null (of the weights' type; summed in FP32 in a fixed order).
+ * dw_workspace: spline_hip_qk_norm_rope_bwd_bytes(head_dim) bytes, with
+ * weights only.  Calls that may overlap need workspaces of their own.
+ *
+ * launch_rope_axes_*: the rotation alone (weights and eps are not read); with
+ * inverse the rotation by -t, which carries gradients back. */
+typedef struct spline_hip_qk_rope {
+    void *q_out, *k_out;
+    const void *q, *k;
+    const void *q_weight, *k_weight;  /* [D], or null for ones */
+    const void* phase_increments;     /* int32 [rotary_dim / 2] */
+    const void* positions;            /* integers of position_bytes (4 or 8), or null for 0..S-1 */
+    const int32_t* frequency_axes;    /* [rotary_dim / 2]: the axis whose position turns the pair,
+                                         held to 0..axes-1; null with one axis */
+    int64_t axes;
+    int64_t batch, sequence_length, q_heads, k_heads, head_dim, rotary_dim;
+    int64_t q_strides[3], k_strides[3];          /* batch, sequence, head */
+    int64_t q_out_strides[3], k_out_strides[3];
+    int64_t position_strides[3];                 /* axis, batch, sequence, in positions */
+    int32_t position_bytes, weight_f32, interleaved;
+    float eps;
+    const void *dq_out, *dk_out;                 /* backward */
+    int64_t dq_out_strides[3], dk_out_strides[3];
+    void *dq_weight, *dk_weight;
+    float* dw_workspace;
+} spline_hip_qk_rope;
+int launch_qk_norm_rope_fp16(const spline_hip_qk_rope* args, void* stream);
+int launch_qk_norm_rope_bf16(const spline_hip_qk_rope* args, void* stream);
+int64_t spline_hip_qk_norm_rope_bwd_bytes(int64_t head_dim);
+int launch_qk_norm_rope_bwd_fp16(const spline_hip_qk_rope* args, void* stream);
+int launch_qk_norm_rope_bwd_bf16(const spline_hip_qk_rope* args, void* stream);
+int launch_rope_axes_fp16(const spline_hip_qk_rope* args, int inverse, void* stream);
+int launch_rope_axes_bf16(const spline_hip_qk_rope* args, int inverse, void* stream);
+
 /* ---- RoPE reference evaluator (src/sfu_repro/rope/polynomial_sincos.py:85-165)
  * FP32 or FP64 angles (angles_f64 = 1) -> FP32 cos and sin planes.  accurate = 1
  * reduces to a quarter turn in FP64 (q = rint(a * 2/pi), r = a - q * pi/2), 0 in
