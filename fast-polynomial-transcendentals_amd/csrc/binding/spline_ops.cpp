@@ -1003,6 +1003,87 @@ std::vector<at::Tensor> flash_attn_fwd_heads_first_bf16(at::Tensor q, at::Tensor
     return {first};
 }
 
+// Attention of a batch over one shared prefix and each sequence's own cache:
+// q [B, T, Hq, D], prefix_k / prefix_v [P, Hkv, D], suffix_k / suffix_v
+// [B, L, Hkv, D], suffix_lens [B] -> [out [B, T, Hq, D], lse [B, Hq, T]].
+std::vector<at::Tensor> shared_prefix_attn_fwd(at::Tensor q, at::Tensor prefix_k, at::Tensor prefix_v,
+                                               at::Tensor suffix_k, at::Tensor suffix_v, at::Tensor suffix_lens,
+                                               int64_t mode, double softmax_scale, double softcap) {
+    const at::ScalarType dtype = q.scalar_type();
+    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "q must be float16 or bfloat16");
+    TORCH_CHECK(q.dim() == 4, "q must have shape [batch, tokens, heads, head_dim]");
+    const int64_t d = q.size(3);
+    TORCH_CHECK(d == 64 || d == 128, "head_dim must be 64 or 128, got ", d);
+    auto check = [&](const at::Tensor& t, const char* name, int64_t dims, const char* shape) {
+        TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+        TORCH_CHECK(t.get_device() == q.get_device(), name, " must be on the same CUDA device as q");
+        TORCH_CHECK(t.scalar_type() == dtype, name, " must have q's dtype");
+        TORCH_CHECK(t.dim() == dims && t.size(dims - 1) == d, name, " must have shape ", shape);
+    };
+    check(prefix_k, "prefix_k", 3, "[prefix, kv_heads, head_dim]");
+    check(prefix_v, "prefix_v", 3, "[prefix, kv_heads, head_dim]");
+    check(suffix_k, "suffix_k", 4, "[batch, suffix, kv_heads, head_dim]");
+    check(suffix_v, "suffix_v", 4, "[batch, suffix, kv_heads, head_dim]");
+    TORCH_CHECK(prefix_k.sizes() == prefix_v.sizes(), "prefix_k and prefix_v must have the same shape");
+    TORCH_CHECK(suffix_k.sizes() == suffix_v.sizes(), "suffix_k and suffix_v must have the same shape");
+    const int64_t b = q.size(0), tokens = q.size(1), hq = q.size(2), hkv = prefix_k.size(1);
+    TORCH_CHECK(suffix_k.size(0) == b, "the suffix must hold q's batch");
+    TORCH_CHECK(suffix_k.size(2) == hkv, "prefix and suffix must have the same kv heads");
+    TORCH_CHECK(hkv > 0 && hq > 0 && hq % hkv == 0, "q heads (", hq, ") must be a positive multiple of kv heads (", hkv, ")");
+    TORCH_CHECK(suffix_lens.is_cuda() && suffix_lens.get_device() == q.get_device() &&
+                    suffix_lens.scalar_type() == at::kInt && suffix_lens.dim() == 1 && suffix_lens.numel() == b,
+                "suffix_lens must be an int32 tensor [batch] on the same CUDA device as q");
+    TORCH_CHECK(softmax_scale > 0 && softmax_scale <= std::numeric_limits<float>::max(),
+                "softmax_scale must be positive and finite");
+    // rows are read 16 bytes at a time and never copied: the caches are the caller's
+    auto rows = [](int64_t* strides, const at::Tensor& t, const char* name) {
+        const int64_t n = t.dim() - 1;
+        bool ok = t.numel() == 0 || (t.stride(n) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+        for (int64_t i = 0; i < n; ++i) {
+            strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+            ok = ok && strides[i] % 8 == 0;
+        }
+        TORCH_CHECK(ok, name, " must have a contiguous head dimension, strides of whole multiples of 8 elements and "
+                              "16-byte alignment");
+    };
+    c10::OptionalDeviceGuard guard(q.device());
+    spline_hip_shared_prefix a{};
+    rows(a.q_strides, q, "q");
+    rows(a.prefix_k_strides, prefix_k, "prefix_k");
+    rows(a.prefix_v_strides, prefix_v, "prefix_v");
+    rows(a.suffix_k_strides, suffix_k, "suffix_k");
+    rows(a.suffix_v_strides, suffix_v, "suffix_v");
+    const at::Tensor lens = suffix_lens.contiguous();
+    at::Tensor out = at::empty({b, tokens, hq, d}, q.options());
+    at::Tensor lse = at::empty({b, hq, tokens}, q.options().dtype(at::kFloat));
+    a.out = out.data_ptr();
+    a.lse = lse.data_ptr<float>();
+    a.q = q.data_ptr();
+    a.prefix_k = prefix_k.data_ptr();
+    a.prefix_v = prefix_v.data_ptr();
+    a.suffix_k = suffix_k.data_ptr();
+    a.suffix_v = suffix_v.data_ptr();
+    a.suffix_lens = lens.data_ptr<int32_t>();
+    a.batch = b;
+    a.tokens = tokens;
+    a.q_heads = hq;
+    a.kv_heads = hkv;
+    a.prefix = prefix_k.size(0);
+    a.suffix = suffix_k.size(1);
+    a.head_dim = d;
+    a.mode = (int32_t)mode;
+    a.scale = (float)softmax_scale;
+    a.cap = (float)softcap;
+    const int64_t bytes = spline_hip_shared_prefix_workspace_bytes(&a);
+    TORCH_CHECK(bytes >= 0, "too many rows, keys or heads for the shared-prefix attention");
+    at::Tensor ws = at::empty({bytes / 4}, q.options().dtype(at::kFloat));
+    a.workspace = bytes > 0 ? ws.data_ptr() : nullptr;
+    void* s = current_stream(q);
+    check_launch((dtype == at::kBFloat16 ? launch_shared_prefix_attention_bf16 : launch_shared_prefix_attention_fp16)(&a, s), s);
+    return {out, lse};
+}
+
 // Largest dS workspace the attention backward allocates: the environment's
 // SPLINE_ATTN_DS_MAX_BYTES (bytes, 0 turns the dS-keeping backward off),
 // 8 GiB by default.
@@ -1720,6 +1801,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("exp2_route") = 0, py::arg("causal") = true, py::arg("softmax_scale"),
           py::arg("softcap") = 0.0, py::arg("sigmoid_bias") = 0.0,
           "Fused attention backward -> [dq [B,S,Hq,D], dk, dv [B,S,Hkv,D]] BF16");
+
+    m.def("shared_prefix_attn_fwd", &shared_prefix_attn_fwd, py::arg("q"), py::arg("prefix_k"), py::arg("prefix_v"),
+          py::arg("suffix_k"), py::arg("suffix_v"), py::arg("suffix_lens"), py::arg("mode"),
+          py::arg("softmax_scale"), py::arg("softcap") = 0.0,
+          "Attention of new tokens [B,T,Hq,D] over a prefix [P,Hkv,D] that the batch shares and each sequence's "
+          "own cache [B,L,Hkv,D] -> [out [B,T,Hq,D], lse [B,Hq,T] FP32]; mode 0 softmax, 3 softcap");
 
     // RoPE reference evaluator (sfu_repro.rope.polynomial_sincos on the device)
     m.def("polynomial_sincos_f32", &polynomial_sincos_f32, py::arg("angles"),

@@ -1,0 +1,555 @@
+// shared_prefix.hip -- attention of a batch whose sequences share one prefix,
+// for gfx950: the new tokens of every sequence attend to the prefix's keys,
+// held once for all, and to the keys of their own suffix cache.
+//
+//   out[b, t] = softmax(s) V over prefix keys 0 .. P - 1 and suffix keys
+//   0 .. lens[b] - T + t of sequence b (the last T of which are the new tokens'
+//   own), s = q.k scale, or cap tanh(q.k scale / cap)
+//
+// For one KV head the rows that meet the prefix are all B T g rows of the batch
+// (g query heads to a KV head), so the prefix is one product over many rows,
+// read once per row tile; each sequence's suffix has T g rows of its own.  Both
+// are cut along the keys into enough parts to fill the chip, each part leaves its
+// rows' O, maximum and sum in FP32 in a workspace, and a second launch joins the
+// parts of a row: O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+//
+// A part is a block of four waves, two blocks to a CU:
+//  * up to 32 rows ("narrow"): every wave has all rows and a quarter of the
+//    keys, in tiles of 8 KiB of K and of V that it alone moves to its LDS; K of
+//    the next tile flies while the scores are turned into probabilities, V of the
+//    next while the next scores are made, and no wave waits for another;
+//  * more ("wide"): each wave has 32 of 128 rows and all waves share 64-key tiles,
+//    one staged ahead.
+// Products are S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16, so a lane
+// keeps one row (query) and a row's reductions stay in two lanes
+// (flash_attn.hpp).
+//
+// What bounds it: up to about 128 rows a KV head the bytes of K and V, beyond
+// that the matrix cores and the exponentials beside them.
+#include <hip/hip_runtime.h>
+
+#include "flash_attn.hpp"
+#include "spline_ops_hip.h"
+
+namespace pt {
+namespace {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kWideRows = 128, kNarrowRows = 32;
+constexpr float kEmptyMax = -1e30f;  // log2 units: below any score, and no infinity
+
+struct PrefixParams {
+    const uint16_t* q;
+    const uint16_t *pk, *pv, *sk, *sv;
+    const int32_t* lens;
+    float* part_o;  // [parts][rows][HD]
+    float2* part_ml;  // [parts][rows]
+    void* out;
+    float* lse;
+    AttnStrides qs, pks, pvs, sks, svs;  // prefix: b unused
+    int64_t rows;     // B T Hq
+    int64_t mrows;    // B T g: rows of a KV head
+    int hq, hkv, group, tokens, batch;
+    int prefix, suffix;
+    int parts_p, parts_s;      // along the keys
+    int chunk;                 // prefix keys per part, a multiple of 64
+    int tiles_p, tiles_s;      // row tiles of a KV head; of a sequence and KV head
+    int groups_p;              // hkv * parts_p
+    int64_t blocks_p;
+    int narrow_p, narrow_s, wide_strides;
+    float sl, cap, unit;  // log2 e scale; softcap: cap, scale / cap
+};
+
+template <bool BF>
+__device__ __forceinline__ f32x16_t mfma(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+}
+
+// The rows that a lane's query has seen so far.
+template <int HD>
+struct RowState {
+    f32x16_t o[HD / 32];  // O^T: o[dt][r] = element dt*32 + 8(r/4) + 4h + r%4 of row c32
+    float m, l;           // log2 units; l of this lane's half of the keys
+
+    __device__ __forceinline__ RowState() : m(kEmptyMax), l(0.0f) {
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) o[dt] = (f32x16_t){};
+    }
+};
+
+// One tile of NT 32-key accumulators of scores: s becomes probabilities, O and
+// l are rescaled if the tile raises the maximum by more than 8 (log2), which
+// keeps the exponents at 8 and below.  MASKED: keys k0 + 32 kt + 8(r/4) + 4h + r%4
+// past klast count nothing; diag = k0 + 4h - klast.
+template <int MODE, int HD, int NT, bool MASKED>
+__device__ __forceinline__ void score_tile(f32x16_t (&s)[NT], RowState<HD>& st, const PrefixParams& p, int diag) {
+    const float sl = MODE == kAttnSoftcapNative ? kLog2e : p.sl;
+    if constexpr (MODE == kAttnSoftcapNative) {
+        const float cap = p.cap, unit = p.unit;
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kt][r] = cap * native_lane<kTanh, kFwd>(s[kt][r] * unit);
+    }
+    float mx[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (MASKED && diag + kt * 32 + 8 * (r >> 2) + (r & 3) > 0) s[kt][r] = -__builtin_inff();
+            mx[r & 3] = __builtin_fmaxf(mx[r & 3], s[kt][r]);
+        }
+    const float mt = half_max(__builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]))) * sl;
+    const bool move = mt > st.m + 8.0f;  // both lanes of a row decide alike
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(move)) {
+        const float m = move ? mt : st.m;
+        const float alpha = __builtin_amdgcn_exp2f(st.m - m);
+        st.m = m;
+        st.l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) st.o[dt] *= alpha;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], sl, -st.m));
+            ls[r & 3] += s[kt][r];
+        }
+    st.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+}
+
+// Probabilities 8 cc .. 8 cc + 7 of an accumulator as the B operand of P V,
+// rounded to the operands' 16-bit type for the matrix cores (l adds them
+// unrounded; the roundings average out over the keys).
+template <bool BF>
+__device__ __forceinline__ bf16x8_t prob_frag(const f32x16_t& s, int cc) {
+    if constexpr (BF) {
+        bf16x8_t f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (__bf16)s[8 * cc + e];
+        return f;
+    } else {
+        f16x8_t f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (_Float16)s[8 * cc + e];
+        return __builtin_bit_cast(bf16x8_t, f);
+    }
+}
+
+template <int HD>
+struct PrefixShape {
+    static constexpr int kNarrowKeys = 4096 / HD;  // 8 KiB tiles
+    static constexpr int kNarrowTileB = lds_row<HD>(kNarrowKeys);
+    static constexpr int kWideTileB = lds_row<HD>(kAttnBlockK);
+    static constexpr int kWideRing = 2;
+    static constexpr int kRegionB = 32 * HD * 4;  // 32 FP32 rows of O
+    static constexpr int kNarrowB = 2 * kNarrowTileB > kRegionB ? 2 * kNarrowTileB : kRegionB;  // per wave
+    static constexpr int kWideB = 2 * kWideRing * kWideTileB;
+    static constexpr int kLds = 4 * kNarrowB > kWideB ? 4 * kNarrowB : kWideB;
+    static_assert(4 * kRegionB <= kLds, "O leaves through LDS");
+};
+
+// FP32 rows of O in LDS, 16-byte chunks swizzled by the row.
+template <int HD>
+__device__ __forceinline__ uint32_t o_chunk(int row, int chunk) {
+    return (uint32_t)(row * HD * 4 + ((chunk ^ row) & (HD / 4 - 1)) * 16);
+}
+template <int HD>
+__device__ __forceinline__ void spill_rows(unsigned char* region, const RowState<HD>& st, int h, int c32) {
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4_t*>(region + o_chunk<HD>(c32, dt * 8 + 2 * g + h)) =
+                (f32x4_t){st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
+}
+
+template <int MODE, int HD, bool BF>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) shared_prefix_kernel(PrefixParams p) {
+    using F = PrefixShape<HD>;
+    constexpr int kC = HD / 16, kD = HD / 32;
+    __shared__ __align__(1024) unsigned char smem[F::kLds];
+    __shared__ float2 sml[4][32];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int h = lane >> 5, c32 = lane & 31;
+
+    // ---- which rows and keys
+    int kvh, part, nrows;           // nrows: of this block
+    int64_t m0;                     // the block's first row among its KV head's
+    const uint16_t *kp, *vp;
+    int64_t kstride, vstride;
+    int k0, kend;                   // keys of the block
+    int seen = 0;                   // suffix keys that the sequence's token 0 sees (token t: t more)
+    const bool own = (int64_t)blockIdx.x >= p.blocks_p;
+    if (!own) {
+        // neighbours in a row of eight blocks go to eight XCDs: the row tiles of
+        // one part and KV head follow each other on one XCD, whose L2 holds its keys
+        const uint32_t idx = blockIdx.x, xcd = idx & 7, slot = idx >> 3;
+        const uint32_t g = slot / (uint32_t)p.tiles_p * 8 + xcd, tile = slot % (uint32_t)p.tiles_p;
+        if (g >= (uint32_t)p.groups_p) return;
+        part = (int)(g / (uint32_t)p.hkv);
+        kvh = (int)(g % (uint32_t)p.hkv);
+        m0 = (int64_t)tile * kWideRows;
+        const int64_t left = p.mrows - m0;
+        nrows = left < kWideRows ? (int)left : kWideRows;
+        kp = p.pk + kvh * p.pks.h;
+        vp = p.pv + kvh * p.pvs.h;
+        kstride = p.pks.s;
+        vstride = p.pvs.s;
+        k0 = part * p.chunk;
+        kend = k0 + p.chunk < p.prefix ? k0 + p.chunk : p.prefix;
+    } else {
+        uint32_t rest = (uint32_t)((int64_t)blockIdx.x - p.blocks_p);
+        const uint32_t tile = rest % (uint32_t)p.tiles_s;
+        rest /= (uint32_t)p.tiles_s;
+        kvh = (int)(rest % (uint32_t)p.hkv);
+        rest /= (uint32_t)p.hkv;
+        const int s = (int)(rest % (uint32_t)p.parts_s), b = (int)(rest / (uint32_t)p.parts_s);
+        part = p.parts_p + s;
+        const int per = p.tokens * p.group, r0 = (int)tile * kWideRows;
+        m0 = (int64_t)b * per + r0;
+        nrows = per - r0 < kWideRows ? per - r0 : kWideRows;
+        kp = p.sk + b * p.sks.b + kvh * p.sks.h;
+        vp = p.sv + b * p.svs.b + kvh * p.svs.h;
+        kstride = p.sks.s;
+        vstride = p.svs.s;
+        int len = p.lens[b];
+        len = len < 0 ? 0 : len < p.suffix ? len : p.suffix;  // held to the cache
+        seen = len - p.tokens + 1;
+        const int last_token = (r0 + nrows - 1) / p.group;
+        const int visible = seen + last_token > 0 ? seen + last_token : 0;  // keys that any row sees
+        const int each = ((visible + p.parts_s - 1) / p.parts_s + 63) & ~63;
+        k0 = s * each;
+        kend = k0 + each < visible ? k0 + each : visible;
+    }
+    const bool narrow = own ? p.narrow_s : p.narrow_p;
+    const int rbase = narrow ? 0 : wave * 32;        // the wave's rows in the block
+    const bool rin = rbase + c32 < nrows;            // this lane has a row
+    const int64_t mrow = m0 + (rin ? rbase + c32 : 0);
+    // row m of a KV head is (b, t, head in the group)
+    const int64_t bt = mrow / p.group;
+    const int b = (int)(bt / p.tokens), t = (int)(bt - (int64_t)b * p.tokens);
+    const uint16_t* qrow =
+        p.q + b * p.qs.b + t * p.qs.s + (kvh * p.group + (int)(mrow - bt * p.group)) * p.qs.h;
+    // the last key that the lane's row sees (a lane without a row computes one
+    // that is not stored, and asks for no mask)
+    int klast = own && rin ? seen + t - 1 : kend - 1;
+    klast = klast < kend - 1 ? klast : kend - 1;
+
+    RowState<HD> st;
+    bf16x8_t qf[kC];  // Q^T fragments: columns 16c + 8h .. of row c32
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+        qf[c] = (bf16x8_t){};
+        if (rin) qf[c] = *reinterpret_cast<const bf16x8_t*>(qrow + 16 * c + 8 * h);
+    }
+    const RowLoader<HD> loader(lane, p.wide_strides);
+    const TileReader<HD> reader(lane);
+    constexpr int kLoadRows = RowLoader<HD>::kLoadRows;
+
+    if (narrow) {
+        constexpr int NK = F::kNarrowKeys, NT = NK / 32, kL = NK / kLoadRows;
+        const int all = kend - k0, tiles = all > 0 ? (all + NK - 1) / NK : 0;
+        // wave w takes tiles w, w + 4, ..
+        const uint32_t ldsk = lds0 + (uint32_t)(wave * F::kNarrowB), ldsv = ldsk + F::kNarrowTileB;
+        const unsigned char* kt0 = smem + wave * F::kNarrowB;
+        const unsigned char* vt0 = kt0 + F::kNarrowTileB;
+        auto load = [&](uint32_t lds, const uint16_t* base, int64_t stride, int tile) {
+#pragma unroll
+            for (int j = 0; j < kL; ++j)
+                loader.load(lds + lds_row<HD>(kLoadRows * j), kLoadRows * j & 7, base, stride,
+                            k0 + tile * NK + kLoadRows * j, kend - 1);
+        };
+        if (wave < tiles) {
+            load(ldsk, kp, kstride, wave);
+            load(ldsv, vp, vstride, wave);
+        }
+        for (int i = wave; i < tiles; i += 4) {
+            wait_loads<kL>();  // K(i) has landed; V(i) may fly
+            f32x16_t s[NT];
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt)
+                    s[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], s[kt]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(i) is read: its place is free
+            const bool more = i + 4 < tiles;
+            if (more) load(ldsk, kp, kstride, i + 4);
+            const int base = k0 + i * NK;
+            if (__any(klast < base + NK - 1)) score_tile<MODE, HD, NT, true>(s, st, p, base + 4 * h - klast);
+            else score_tile<MODE, HD, NT, false>(s, st, p, 0);
+            if (more) wait_loads<kL>();  // V(i) has landed; K(i + 4) may fly
+            else wait_loads<0>();
+#pragma unroll
+            for (int g = 0; g < 2 * NT; ++g) {
+                const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
+#pragma unroll
+                for (int dt = 0; dt < kD; ++dt)
+                    st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) load(ldsv, vp, vstride, i + 4);
+        }
+    } else {
+        constexpr int NK = kAttnBlockK, NT = NK / 32, kL = NK / kLoadRows / 4, kRing = F::kWideRing;
+        const int all = kend - k0, tiles = all > 0 ? (all + NK - 1) / NK : 0;
+        constexpr uint32_t kV = kRing * F::kWideTileB;
+        auto load = [&](uint32_t lds, const uint16_t* base, int64_t stride, int tile) {
+#pragma unroll
+            for (int j = 0; j < kL; ++j) {
+                const int r = kLoadRows * (j * 4 + wave);
+                loader.load(lds + lds_row<HD>(r), kLoadRows * wave & 7, base, stride, k0 + tile * NK + r, kend - 1);
+            }
+        };
+        auto stage = [&](int i) {
+            load(lds0 + (uint32_t)(i % kRing * F::kWideTileB), kp, kstride, i);
+            load(lds0 + kV + (uint32_t)(i % kRing * F::kWideTileB), vp, vstride, i);
+        };
+        const bool active = rbase < nrows;
+        if (tiles > 0) stage(0);
+        for (int i = 0; i < tiles; ++i) {
+            wait_loads<0>();
+            block_barrier();  // tile i is whole, and every wave is done with tile i - 1
+            if (i + 1 < tiles) stage(i + 1);
+            if (!active) continue;
+            const unsigned char* kt0 = smem + i % kRing * F::kWideTileB;
+            const unsigned char* vt0 = kt0 + kV;
+            f32x16_t s[NT];
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt)
+                    s[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], s[kt]);
+            const int base = k0 + i * NK;
+            if (__any(klast < base + NK - 1)) score_tile<MODE, HD, NT, true>(s, st, p, base + 4 * h - klast);
+            else score_tile<MODE, HD, NT, false>(s, st, p, 0);
+#pragma unroll
+            for (int g = 0; g < 2 * NT; ++g) {
+                const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
+#pragma unroll
+                for (int dt = 0; dt < kD; ++dt)
+                    st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
+            }
+        }
+        block_barrier();  // the tiles are read: their place is free
+    }
+
+    // ---- the rows to the workspace, whole rows through LDS
+    unsigned char* region = smem + wave * (narrow ? F::kNarrowB : F::kRegionB);
+    spill_rows<HD>(region, st, h, c32);
+    const float l = half_sum(st.l);
+    if (h == 0) sml[wave][c32] = make_float2(st.m, l);
+    __syncthreads();
+    const int64_t prow = (int64_t)part * p.rows + (int64_t)kvh * p.mrows + m0;
+    float* po = p.part_o + prow * HD;
+    constexpr int kChunks = HD / 4;
+    for (int i = tid; i < nrows * kChunks; i += 256) {
+        const int row = i / kChunks, chunk = i % kChunks;
+        f32x4_t o;
+        float2 ml;
+        if (narrow) {
+            float m = sml[0][row].x;
+#pragma unroll
+            for (int w = 1; w < 4; ++w) m = __builtin_fmaxf(m, sml[w][row].x);
+            o = (f32x4_t){};
+            ml = make_float2(m, 0.0f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float2 x = sml[w][row];
+                const float a = __builtin_amdgcn_exp2f(x.x - m);
+                o += *reinterpret_cast<const f32x4_t*>(smem + w * F::kNarrowB + o_chunk<HD>(row, chunk)) * a;
+                ml.y = __builtin_fmaf(x.y, a, ml.y);
+            }
+        } else {
+            o = *reinterpret_cast<const f32x4_t*>(smem + (row >> 5) * F::kRegionB + o_chunk<HD>(row & 31, chunk));
+            ml = sml[row >> 5][row & 31];
+        }
+        *reinterpret_cast<f32x4_t*>(po + (int64_t)row * HD + chunk * 4) = o;
+        if (chunk == 0) p.part_ml[prow + row] = ml;
+    }
+}
+
+// Joins the parts of each row: HD / 4 lanes a row.
+template <int HD, bool BF>
+__global__ void __launch_bounds__(256) shared_prefix_join_kernel(PrefixParams p) {
+    constexpr int kChunks = HD / 4;
+    const int chunk = threadIdx.x % kChunks;
+    const int64_t row = (int64_t)blockIdx.x * (256 / kChunks) + threadIdx.x / kChunks;
+    if (row >= p.rows) return;
+    const int parts = p.parts_p + p.parts_s;
+    float m = kEmptyMax;
+    for (int i = 0; i < parts; ++i) m = __builtin_fmaxf(m, p.part_ml[(int64_t)i * p.rows + row].x);
+    float l = 0.0f;
+    f32x4_t o = (f32x4_t){};
+    for (int i = 0; i < parts; ++i) {
+        const int64_t at = (int64_t)i * p.rows + row;
+        const float2 ml = p.part_ml[at];
+        const float a = __builtin_amdgcn_exp2f(ml.x - m);
+        l = __builtin_fmaf(ml.y, a, l);
+        o += *reinterpret_cast<const f32x4_t*>(p.part_o + at * HD + chunk * 4) * a;
+    }
+    // a row that sees no key is zero, its partition function too
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t kvh = row / p.mrows, mrow = row - kvh * p.mrows, bt = mrow / p.group;
+    const int64_t head = kvh * p.group + (mrow - bt * p.group);
+    uint2 w;
+    if constexpr (BF) {
+        w = make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
+    } else {
+        w = make_uint2(as_u32((h2_t){(_Float16)(o[0] * inv), (_Float16)(o[1] * inv)}),
+                       as_u32((h2_t){(_Float16)(o[2] * inv), (_Float16)(o[3] * inv)}));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (bt * p.hq + head) * HD + chunk * 4) = w;
+    if (chunk == 0 && p.lse != nullptr) {
+        const int64_t b = bt / p.tokens, t = bt - b * p.tokens;
+        p.lse[(b * p.hq + head) * p.tokens + t] =
+            l == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
+    }
+}
+
+// ---- host side -----------------------------------------------------------------
+
+constexpr int64_t kMaxBlocks = 0xffffffffll / 256;  // a grid counts its threads in 32 bits
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How the work is cut: sets the parts, tiles and blocks.  False: too large.
+bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
+    const int64_t group = a->q_heads / a->kv_heads, per = a->tokens * group;
+    if (a->batch > 0x7fffffff / per || a->batch * per > 0x7fffffff / a->kv_heads) return false;
+    p.batch = (int)a->batch;
+    p.tokens = (int)a->tokens;
+    p.hq = (int)a->q_heads;
+    p.hkv = (int)a->kv_heads;
+    p.group = (int)group;
+    p.prefix = (int)a->prefix;
+    p.suffix = (int)a->suffix;
+    p.mrows = a->batch * per;
+    p.rows = p.mrows * p.hkv;
+    // blocks that run at once: two to a CU
+    const int64_t slots = 2 * (int64_t)device_shape().cus;
+    auto parts_for = [&](int64_t streams, int64_t keys) {
+        const int64_t most = ceil_div(keys, 256), want = ceil_div(slots, streams);
+        return want < most ? want : most;
+    };
+    p.narrow_p = p.mrows <= kNarrowRows;
+    p.narrow_s = per <= kNarrowRows;
+    p.tiles_p = (int)ceil_div(p.mrows, kWideRows);
+    p.tiles_s = (int)ceil_div(per, kWideRows);
+    p.parts_p = p.parts_s = 0;
+    p.chunk = 64;
+    if (p.prefix > 0) {
+        const int64_t parts = parts_for((int64_t)p.hkv * p.tiles_p, p.prefix);
+        p.chunk = (int)(ceil_div(ceil_div(p.prefix, parts), 64) * 64);
+        p.parts_p = (int)ceil_div(p.prefix, p.chunk);
+    }
+    if (p.suffix > 0) p.parts_s = (int)parts_for(a->batch * p.hkv * p.tiles_s, p.suffix);
+    p.groups_p = p.hkv * p.parts_p;
+    p.blocks_p = ceil_div(p.groups_p, 8) * 8 * p.tiles_p;
+    const int64_t blocks_s = a->batch * p.parts_s * p.hkv * p.tiles_s;
+    blocks = p.blocks_p + blocks_s;
+    return blocks <= kMaxBlocks && ceil_div(p.rows, 4) <= kMaxBlocks;
+}
+
+bool sizes_ok(const spline_hip_shared_prefix* a) {
+    const int64_t limit = 0x7fffffff - 4096;  // keys and tokens, with what a tile adds to them
+    return a && a->batch >= 0 && a->tokens >= 0 && a->q_heads > 0 && a->kv_heads > 0 && a->q_heads % a->kv_heads == 0 &&
+           a->q_heads <= 65536 && (a->head_dim == 64 || a->head_dim == 128) && a->prefix >= 0 && a->prefix <= limit &&
+           a->suffix >= 0 && a->suffix <= limit && a->tokens <= limit / 65536;
+}
+
+template <int MODE, int HD, bool BF>
+void go(const PrefixParams& p, int64_t blocks, hipStream_t st) {
+    if (blocks > 0)
+        hipLaunchKernelGGL((shared_prefix_kernel<MODE, HD, BF>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((shared_prefix_join_kernel<HD, BF>), dim3((unsigned)ceil_div(p.rows, 1024 / HD)), dim3(256), 0,
+                       st, p);
+}
+
+template <bool BF>
+int run(const spline_hip_shared_prefix* a, void* stream) {
+    if (!sizes_ok(a) || !(a->scale > 0.0f && a->scale <= __FLT_MAX__)) return hipErrorInvalidValue;
+    if (a->mode != kAttnSoftmaxNative && a->mode != kAttnSoftcapNative) return hipErrorInvalidValue;
+    if (a->mode == kAttnSoftcapNative && !(a->cap > 0.0f && a->cap <= __FLT_MAX__)) return hipErrorInvalidValue;
+    if (a->batch == 0 || a->tokens == 0) return hipSuccess;
+    PrefixParams p{};
+    int64_t blocks = 0;
+    if (!plan(a, p, blocks)) return hipErrorInvalidValue;
+    auto rows_ok = [](const void* x, const int64_t* s, int n) {
+        bool ok = x != nullptr && aligned16(x);
+        for (int i = 0; i < n; ++i) ok = ok && s[i] >= 0 && s[i] % 8 == 0;
+        return ok;
+    };
+    if (!rows_ok(a->q, a->q_strides, 3) || !a->out || !aligned16(a->out) || ((uintptr_t)a->lse & 3) != 0)
+        return hipErrorInvalidValue;
+    if (a->prefix > 0 && (!rows_ok(a->prefix_k, a->prefix_k_strides, 2) || !rows_ok(a->prefix_v, a->prefix_v_strides, 2)))
+        return hipErrorInvalidValue;
+    if (a->suffix > 0 && (!rows_ok(a->suffix_k, a->suffix_k_strides, 3) || !rows_ok(a->suffix_v, a->suffix_v_strides, 3) ||
+                          !a->suffix_lens || ((uintptr_t)a->suffix_lens & 3) != 0))
+        return hipErrorInvalidValue;
+    const int64_t parts = p.parts_p + p.parts_s;
+    if (parts > 0 && (!a->workspace || !aligned16(a->workspace))) return hipErrorInvalidValue;
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.pk = static_cast<const uint16_t*>(a->prefix_k);
+    p.pv = static_cast<const uint16_t*>(a->prefix_v);
+    p.sk = static_cast<const uint16_t*>(a->suffix_k);
+    p.sv = static_cast<const uint16_t*>(a->suffix_v);
+    p.lens = a->suffix_lens;
+    p.part_o = static_cast<float*>(a->workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * p.rows * a->head_dim);
+    p.out = a->out;
+    p.lse = a->lse;
+    p.qs = {a->q_strides[0], a->q_strides[2], a->q_strides[1]};
+    p.pks = {0, a->prefix_k_strides[1], a->prefix_k_strides[0]};
+    p.pvs = {0, a->prefix_v_strides[1], a->prefix_v_strides[0]};
+    p.sks = {a->suffix_k_strides[0], a->suffix_k_strides[2], a->suffix_k_strides[1]};
+    p.svs = {a->suffix_v_strides[0], a->suffix_v_strides[2], a->suffix_v_strides[1]};
+    // staging adds up to 7 rows to a wave's address as a 32-bit byte offset
+    for (const AttnStrides* s : {&p.pks, &p.pvs, &p.sks, &p.svs}) p.wide_strides |= s->s > (int64_t(1) << 27);
+    p.sl = a->scale * kLog2e;
+    p.cap = a->cap;
+    p.unit = a->scale / a->cap;
+    const hipStream_t st = hs(stream);
+    if (a->head_dim == 128) {
+        if (a->mode == kAttnSoftmaxNative) go<kAttnSoftmaxNative, 128, BF>(p, blocks, st);
+        else go<kAttnSoftcapNative, 128, BF>(p, blocks, st);
+    } else {
+        if (a->mode == kAttnSoftmaxNative) go<kAttnSoftmaxNative, 64, BF>(p, blocks, st);
+        else go<kAttnSoftcapNative, 64, BF>(p, blocks, st);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace pt
+
+using namespace pt;
+
+extern "C" int64_t spline_hip_shared_prefix_workspace_bytes(const spline_hip_shared_prefix* a) {
+    if (!sizes_ok(a)) return -1;
+    if (a->batch == 0 || a->tokens == 0) return 0;
+    PrefixParams p{};
+    int64_t blocks = 0;
+    if (!plan(a, p, blocks)) return -1;
+    return (int64_t)(p.parts_p + p.parts_s) * p.rows * (a->head_dim + 2) * 4;
+}
+extern "C" int launch_shared_prefix_attention_bf16(const spline_hip_shared_prefix* args, void* stream) {
+    return run<true>(args, stream);
+}
+extern "C" int launch_shared_prefix_attention_fp16(const spline_hip_shared_prefix* args, void* stream) {
+    return run<false>(args, stream);
+}

@@ -391,6 +391,38 @@ def flash_attn_bwd(q, k, v, out, dout, lse, softmax_scale=None, causal=False, so
                                             scale, cap, bias))
 
 
+def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, softmax_scale=None,
+                             softcap=0.0, **program):
+    """Attention of a batch whose sequences share a prefix, for serving: returns
+    (out [B, T, Hq, D], lse [B, Hq, T]).
+
+    ``q [B, T, Hq, D]`` holds the T new tokens of each sequence (1 when
+    decoding), ``prefix_k`` and ``prefix_v [P, Hkv, D]`` the keys and values that
+    every sequence shares, read once for all of them, ``suffix_k`` and
+    ``suffix_v [B, L, Hkv, D]`` each sequence's own cache, whose first
+    ``suffix_lens[b]`` (int32, on the device, held to 0..L) rows are valid, the
+    new tokens' own last.  Token t sees the prefix and suffix rows 0 ..
+    ``suffix_lens[b] - T + t``; rows past them may hold anything.  A token that
+    sees no key gets zeros and an lse of -inf.
+
+    Any strides over a contiguous head dimension in whole multiples of 8
+    elements (nothing is copied); float16 or bfloat16; head_dim 64 or 128.  The
+    score program is that of :func:`flash_attn_fwd`'s arguments; hardware softmax
+    and hardware softcap are built.  There is no backward: the operands'
+    gradients are refused.
+    """
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, prefix_k, prefix_v, suffix_k, suffix_v)):
+        raise RuntimeError("flash_attn_shared_prefix has no backward; call it under torch.no_grad()")
+    scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
+    if program:
+        mode, _, cap, _ = select_forward(seqlen=max(1, prefix_k.shape[0]), softcap=softcap, **program)
+        if mode not in (MODE_SOFTMAX_NATIVE, MODE_SOFTCAP_NATIVE):
+            raise NotImplementedError("the shared-prefix attention is built with the hardware softmax and softcap")
+    else:
+        mode, cap = (MODE_SOFTCAP_NATIVE, float(softcap)) if softcap and softcap > 0 else (MODE_SOFTMAX_NATIVE, 1.0)
+    return tuple(_ops().shared_prefix_attn_fwd(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, mode, scale, cap))
+
+
 def runtime() -> dict:
     """The mapping ``sfu_repro.fa4`` resolves configurations against."""
     return {

@@ -736,6 +736,40 @@ int launch_flash_attention_bwd_strided_bf16_noalloc(void* dq, void* dk, void* dv
                                                     int grad, int exp2_route, int causal, float scale,
                                                     float cap, float sigmoid_bias, void* stream);
 
+/* ---- attention of a batch over one shared prefix ---------------------------
+ * No counterpart in the reference, whose attention is FA4's for sequences of
+ * their own (src/sfu_repro/fa4.py:356-428).  For serving: the T new tokens of
+ * each sequence, q [B, T, Hq, D], attend to the P keys of a prefix that all
+ * sequences share, prefix_k and prefix_v [P, Hkv, D], and to the keys of their
+ * own caches, suffix_k and suffix_v [B, L, Hkv, D], whose lens[b] first rows are
+ * valid, the last T of them the new tokens': token t sees suffix keys
+ * 0 .. lens[b] - T + t.  lens are held to 0 .. L; rows from lens[b] on may
+ * hold anything.  out [B, T, Hq, D] contiguous, and lse, float [B, Hq, T] or
+ * null: ln of the row's sum of exp(s').  A row that sees no key is zero with
+ * lse -inf.  D 64 or 128, Hq a multiple of Hkv, 16-bit (P is rounded to the
+ * operands' type ahead of P V; sums are FP32).  mode: 0 softmax of q.k scale,
+ * 3 of cap tanh(q.k scale / cap), as in launch_flash_attention_fwd_bf16.
+ * Pointers 16-byte aligned, strides (elements) multiples of 8, head dimension
+ * contiguous.  workspace: spline_hip_shared_prefix_workspace_bytes of the same
+ * sizes on the same device (-1: sizes that are refused), 16-byte aligned; calls
+ * that may overlap need workspaces of their own. */
+typedef struct spline_hip_shared_prefix {
+    void* out;
+    float* lse;
+    const void *q, *prefix_k, *prefix_v, *suffix_k, *suffix_v;
+    const int32_t* suffix_lens;
+    void* workspace;
+    int64_t batch, tokens, q_heads, kv_heads, prefix, suffix, head_dim;
+    int64_t q_strides[3];                             /* batch, token, head */
+    int64_t prefix_k_strides[2], prefix_v_strides[2]; /* key, head */
+    int64_t suffix_k_strides[3], suffix_v_strides[3]; /* batch, key, head */
+    int32_t mode;
+    float scale, cap;
+} spline_hip_shared_prefix;
+int64_t spline_hip_shared_prefix_workspace_bytes(const spline_hip_shared_prefix* args);
+int launch_shared_prefix_attention_fp16(const spline_hip_shared_prefix* args, void* stream);
+int launch_shared_prefix_attention_bf16(const spline_hip_shared_prefix* args, void* stream);
+
 /* ---- device/launch introspection --------------------------------------- */
 /* Number of compute units of the current device and the grid the
  * elementwise launchers use for `size` 16-bit elements and `streams` tensors
