@@ -228,12 +228,16 @@ struct RowLoader {
     // Rows row0 .. row0 + kLoadRows - 1 of base to LDS address lds (their
     // lds_row in some tile, tile_row = row0's row there modulo 8).  Rows past
     // `last` are zeros: a copy of a real row that holds an infinity would meet
-    // the zero probability of a masked one, and 0 * Inf is NaN.
+    // the zero probability of a masked one, and 0 * Inf is NaN.  ONCE: memory
+    // that nobody reads again.
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(uint32_t lds, int tile_row, const uint16_t* base, int64_t stride, int row0,
                                          int last) const {
         const uint32_t col = (uint32_t)((lc ^ row_swizzle<HD>(tile_row + lr)) * 16);
         if (row0 + kLoadRows - 1 <= last && !wide) {  // wave-uniform
-            load_to_lds(lds, base + row0 * stride, (uint32_t)lr * (uint32_t)(int)stride * 2 + col);
+            const uint32_t offset = (uint32_t)lr * (uint32_t)(int)stride * 2 + col;
+            if constexpr (ONCE) load_to_lds_once(lds, base + row0 * stride, offset);
+            else load_to_lds(lds, base + row0 * stride, offset);
         } else {
             const unsigned char* src = reinterpret_cast<const unsigned char*>(base + (row0 + lr) * stride) + col;
             load_to_lds_each(lds, row0 + lr <= last ? src : reinterpret_cast<const unsigned char*>(kZeroChunk));

@@ -13,13 +13,14 @@
 // rows' O, maximum and sum in FP32 in a workspace, and a second launch joins the
 // parts of a row: O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 //
-// A part is a block of four waves, two blocks to a CU:
+// A part is a block of four waves, two blocks to a CU (three at head_dim 64):
 //  * up to 32 rows ("narrow"): every wave has all rows and a quarter of the
-//    keys, in tiles of 8 KiB of K and of V that it alone moves to its LDS; K of
+//    keys, in tiles of 32 keys that it alone moves to its LDS; K of
 //    the next tile flies while the scores are turned into probabilities, V of the
 //    next while the next scores are made, and no wave waits for another;
 //  * more ("wide"): each wave has 32 of 128 rows and all waves share 64-key tiles,
-//    one staged ahead.
+//    one staged ahead (two at head_dim 64); with up to 64 rows two waves share a
+//    row and halve each tile's keys.
 // Products are S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16, so a lane
 // keeps one row (query) and a row's reductions stay in two lanes
 // (flash_attn.hpp).
@@ -27,6 +28,8 @@
 // What bounds it: up to about 128 rows a KV head the bytes of K and V, beyond
 // that the matrix cores and the exponentials beside them.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "flash_attn.hpp"
 #include "spline_ops_hip.h"
@@ -37,6 +40,7 @@ namespace {
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kWideRows = 128, kNarrowRows = 32;
+constexpr int kLeastKeys = 128;  // of a part: a tile for each wave of a narrow block
 constexpr float kEmptyMax = -1e30f;  // log2 units: below any score, and no infinity
 
 struct PrefixParams {
@@ -58,6 +62,7 @@ struct PrefixParams {
     int groups_p;              // hkv * parts_p
     int64_t blocks_p;
     int narrow_p, narrow_s, wide_strides;
+    int once;                  // K and V do not stay in the caches
     float sl, cap, unit;  // log2 e scale; softcap: cap, scale / cap
 };
 
@@ -146,10 +151,10 @@ __device__ __forceinline__ bf16x8_t prob_frag(const f32x16_t& s, int cc) {
 
 template <int HD>
 struct PrefixShape {
-    static constexpr int kNarrowKeys = 4096 / HD;  // 8 KiB tiles
+    static constexpr int kNarrowKeys = 32;  // one accumulator
     static constexpr int kNarrowTileB = lds_row<HD>(kNarrowKeys);
     static constexpr int kWideTileB = lds_row<HD>(kAttnBlockK);
-    static constexpr int kWideRing = 2;
+    static constexpr int kWideRing = HD == 64 ? 3 : 2;
     static constexpr int kRegionB = 32 * HD * 4;  // 32 FP32 rows of O
     static constexpr int kNarrowB = 2 * kNarrowTileB > kRegionB ? 2 * kNarrowTileB : kRegionB;  // per wave
     static constexpr int kWideB = 2 * kWideRing * kWideTileB;
@@ -173,7 +178,7 @@ __device__ __forceinline__ void spill_rows(unsigned char* region, const RowState
 }
 
 template <int MODE, int HD, bool BF>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) shared_prefix_kernel(PrefixParams p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2))) shared_prefix_kernel(PrefixParams p) {
     using F = PrefixShape<HD>;
     constexpr int kC = HD / 16, kD = HD / 32;
     __shared__ __align__(1024) unsigned char smem[F::kLds];
@@ -232,15 +237,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
         k0 = s * each;
         kend = k0 + each < visible ? k0 + each : visible;
     }
-    const bool narrow = own ? p.narrow_s : p.narrow_p;
-    const int rbase = narrow ? 0 : wave * 32;        // the wave's rows in the block
-    const bool rin = rbase + c32 < nrows;            // this lane has a row
-    const int64_t mrow = m0 + (rin ? rbase + c32 : 0);
-    // row m of a KV head is (b, t, head in the group)
-    const int64_t bt = mrow / p.group;
-    const int b = (int)(bt / p.tokens), t = (int)(bt - (int64_t)b * p.tokens);
+    // the waves that share a row's keys among them: narrow four, half two, else one
+    const bool narrow = own ? p.narrow_s : p.narrow_p, half = !narrow && nrows <= 64;
+    const int rbase = narrow ? 0 : half ? (wave & 1) * 32 : wave * 32;  // the wave's rows in the block
+    const bool rin = rbase + c32 < nrows;                                // this lane has a row
+    // row m of a KV head is (b, t, head in the group); fewer than 2^31 of them
+    const uint32_t mrow = (uint32_t)m0 + (uint32_t)(rin ? rbase + c32 : 0);
+    const uint32_t bt = mrow / (uint32_t)p.group;
+    const uint32_t b = bt / (uint32_t)p.tokens;
+    const int t = (int)(bt - b * (uint32_t)p.tokens);
     const uint16_t* qrow =
-        p.q + b * p.qs.b + t * p.qs.s + (kvh * p.group + (int)(mrow - bt * p.group)) * p.qs.h;
+        p.q + b * p.qs.b + t * p.qs.s + (kvh * p.group + (int)(mrow - bt * (uint32_t)p.group)) * p.qs.h;
     // the last key that the lane's row sees (a lane without a row computes one
     // that is not stored, and asks for no mask)
     int klast = own && rin ? seen + t - 1 : kend - 1;
@@ -257,6 +264,59 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     const TileReader<HD> reader(lane);
     constexpr int kLoadRows = RowLoader<HD>::kLoadRows;
 
+    // S^T of the NT 32-key accumulators at kt0, fragments read six ahead
+    auto scores = [&](auto& s, const unsigned char* kt0) {
+        constexpr int NT = sizeof(s) / sizeof(f32x16_t), kN = NT * kC;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt)
+                s[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], s[kt]);
+        constexpr int kAhead = kN < 6 ? kN : 6;
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int g = 0; g < kN - kAhead; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // O^T += V^T P^T, three fragments (two reads each) ahead
+    auto accumulate = [&](const auto& s, const unsigned char* vt0) {
+        constexpr int NT = sizeof(s) / sizeof(f32x16_t), kN = 2 * NT * kD;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < 2 * NT; ++g) {
+            const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
+#pragma unroll
+            for (int dt = 0; dt < kD; ++dt)
+                st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int g = 0; g < kN - 3; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // the first and the last key that bound what the wave's rows see: tiles that
+    // end ahead of the first need no mask, tiles behind the last no arithmetic
+    int kfull = klast, kmost = klast;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) {
+        const int x = __shfl_xor(kfull, step), y = __shfl_xor(kmost, step);
+        kfull = x < kfull ? x : kfull;
+        kmost = y > kmost ? y : kmost;
+    }
+    kfull = __builtin_amdgcn_readfirstlane(kfull);
+    kmost = __builtin_amdgcn_readfirstlane(kmost);
+
     if (narrow) {
         constexpr int NK = F::kNarrowKeys, NT = NK / 32, kL = NK / kLoadRows;
         const int all = kend - k0, tiles = all > 0 ? (all + NK - 1) / NK : 0;
@@ -265,45 +325,39 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
         const unsigned char* kt0 = smem + wave * F::kNarrowB;
         const unsigned char* vt0 = kt0 + F::kNarrowTileB;
         auto load = [&](uint32_t lds, const uint16_t* base, int64_t stride, int tile) {
+            auto rows = [&](auto once) {
 #pragma unroll
-            for (int j = 0; j < kL; ++j)
-                loader.load(lds + lds_row<HD>(kLoadRows * j), kLoadRows * j & 7, base, stride,
-                            k0 + tile * NK + kLoadRows * j, kend - 1);
+                for (int j = 0; j < kL; ++j)
+                    loader.template load<decltype(once)::value>(lds + lds_row<HD>(kLoadRows * j), kLoadRows * j & 7, base,
+                                                                stride, k0 + tile * NK + kLoadRows * j, kend - 1);
+            };
+            if (p.once) rows(std::integral_constant<bool, true>{});
+            else rows(std::integral_constant<bool, false>{});
         };
         if (wave < tiles) {
             load(ldsk, kp, kstride, wave);
             load(ldsv, vp, vstride, wave);
         }
-        for (int i = wave; i < tiles; i += 4) {
+        f32x16_t s[NT];
+        auto tile = [&](auto masked, int i) {
             wait_loads<kL>();  // K(i) has landed; V(i) may fly
-            f32x16_t s[NT];
-#pragma unroll
-            for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
-#pragma unroll
-            for (int c = 0; c < kC; ++c)
-#pragma unroll
-                for (int kt = 0; kt < NT; ++kt)
-                    s[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], s[kt]);
+            scores(s, kt0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(i) is read: its place is free
             const bool more = i + 4 < tiles;
             if (more) load(ldsk, kp, kstride, i + 4);
-            const int base = k0 + i * NK;
-            if (__any(klast < base + NK - 1)) score_tile<MODE, HD, NT, true>(s, st, p, base + 4 * h - klast);
-            else score_tile<MODE, HD, NT, false>(s, st, p, 0);
+            score_tile<MODE, HD, NT, decltype(masked)::value>(s, st, p, k0 + i * NK + 4 * h - klast);
             if (more) wait_loads<kL>();  // V(i) has landed; K(i + 4) may fly
             else wait_loads<0>();
-#pragma unroll
-            for (int g = 0; g < 2 * NT; ++g) {
-                const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
-#pragma unroll
-                for (int dt = 0; dt < kD; ++dt)
-                    st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
-            }
+            accumulate(s, vt0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (more) load(ldsv, vp, vstride, i + 4);
-        }
+        };
+        const int full = (kfull + 1 - k0) / NK;  // tiles without a masked key (negative: none)
+        int i = wave;
+        for (; i < tiles && i < full; i += 4) tile(std::integral_constant<bool, false>{}, i);
+        for (; i < tiles; i += 4) tile(std::integral_constant<bool, true>{}, i);
     } else {
-        constexpr int NK = kAttnBlockK, NT = NK / 32, kL = NK / kLoadRows / 4, kRing = F::kWideRing;
+        constexpr int NK = kAttnBlockK, kL = NK / kLoadRows / 4, kRing = F::kWideRing;
         const int all = kend - k0, tiles = all > 0 ? (all + NK - 1) / NK : 0;
         constexpr uint32_t kV = kRing * F::kWideTileB;
         auto load = [&](uint32_t lds, const uint16_t* base, int64_t stride, int tile) {
@@ -317,39 +371,51 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
             load(lds0 + (uint32_t)(i % kRing * F::kWideTileB), kp, kstride, i);
             load(lds0 + kV + (uint32_t)(i % kRing * F::kWideTileB), vp, vstride, i);
         };
-        const bool active = rbase < nrows;
-        if (tiles > 0) stage(0);
-        for (int i = 0; i < tiles; ++i) {
-            wait_loads<0>();
+#pragma unroll
+        for (int t = 0; t < kRing - 1; ++t)
+            if (t < tiles) stage(t);
+        auto sync = [&](int i) {
+            // the loads of the kRing - 2 tiles behind tile i may still fly
+            if (kRing > 2 && i + kRing - 2 < tiles) wait_loads<2 * kL * (kRing - 2)>();
+            else wait_loads<0>();
             block_barrier();  // tile i is whole, and every wave is done with tile i - 1
-            if (i + 1 < tiles) stage(i + 1);
-            if (!active) continue;
-            const unsigned char* kt0 = smem + i % kRing * F::kWideTileB;
-            const unsigned char* vt0 = kt0 + kV;
+            if (i + kRing - 1 < tiles) stage(i + kRing - 1);
+        };
+        // the wave's keys of a tile: all 64, or with half of the rows 32 of them
+        auto run = [&](auto nt_c, int off) {
+            constexpr int NT = decltype(nt_c)::value;
             f32x16_t s[NT];
-#pragma unroll
-            for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
-#pragma unroll
-            for (int c = 0; c < kC; ++c)
-#pragma unroll
-                for (int kt = 0; kt < NT; ++kt)
-                    s[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], s[kt]);
-            const int base = k0 + i * NK;
-            if (__any(klast < base + NK - 1)) score_tile<MODE, HD, NT, true>(s, st, p, base + 4 * h - klast);
-            else score_tile<MODE, HD, NT, false>(s, st, p, 0);
-#pragma unroll
-            for (int g = 0; g < 2 * NT; ++g) {
-                const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
-#pragma unroll
-                for (int dt = 0; dt < kD; ++dt)
-                    st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
+            auto tile = [&](auto masked, int i) {
+                const unsigned char* kt0 = smem + i % kRing * F::kWideTileB + lds_row<HD>(off);
+                __builtin_amdgcn_s_setprio(1);  // the other block keeps the VALU busy meanwhile
+                scores(s, kt0);
+                __builtin_amdgcn_s_setprio(0);
+                score_tile<MODE, HD, NT, decltype(masked)::value>(s, st, p, k0 + i * NK + off + 4 * h - klast);
+                accumulate(s, kt0 + kV);
+            };
+            // tiles without a masked key, and with one that a row sees; a wave
+            // without rows only stages
+            const int x = kfull + 1 - k0 - off - 32 * NT, y = kmost - k0 - off;
+            const int whole = x < 0 ? 0 : x / NK + 1, most = y < 0 || rbase >= nrows ? 0 : y / NK + 1;
+            const int last = most < tiles ? most : tiles;
+            int i = 0;
+            for (; i < last && i < whole; ++i) {
+                sync(i);
+                tile(std::integral_constant<bool, false>{}, i);
             }
-        }
-        block_barrier();  // the tiles are read: their place is free
+            for (; i < last; ++i) {
+                sync(i);
+                tile(std::integral_constant<bool, true>{}, i);
+            }
+            for (; i < tiles; ++i) sync(i);
+        };
+        if (half) run(std::integral_constant<int, 1>{}, (wave >> 1) * 32);
+        else run(std::integral_constant<int, 2>{}, 0);
     }
 
     // ---- the rows to the workspace, whole rows through LDS
-    unsigned char* region = smem + wave * (narrow ? F::kNarrowB : F::kRegionB);
+    __syncthreads();  // every wave has read its tiles
+    unsigned char* region = smem + wave * F::kRegionB;
     spill_rows<HD>(region, st, h, c32);
     const float l = half_sum(st.l);
     if (h == 0) sml[wave][c32] = make_float2(st.m, l);
@@ -359,50 +425,77 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     constexpr int kChunks = HD / 4;
     for (int i = tid; i < nrows * kChunks; i += 256) {
         const int row = i / kChunks, chunk = i % kChunks;
-        f32x4_t o;
-        float2 ml;
-        if (narrow) {
-            float m = sml[0][row].x;
-#pragma unroll
-            for (int w = 1; w < 4; ++w) m = __builtin_fmaxf(m, sml[w][row].x);
-            o = (f32x4_t){};
-            ml = make_float2(m, 0.0f);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float2 x = sml[w][row];
-                const float a = __builtin_amdgcn_exp2f(x.x - m);
-                o += *reinterpret_cast<const f32x4_t*>(smem + w * F::kNarrowB + o_chunk<HD>(row, chunk)) * a;
-                ml.y = __builtin_fmaf(x.y, a, ml.y);
+        // the row's share of each wave that has it
+        const int first = narrow ? 0 : row >> 5, step = narrow ? 1 : 2, shares = narrow ? 4 : half ? 2 : 1, r = row & 31;
+        float2 ml = sml[first][r];
+        f32x4_t o = *reinterpret_cast<const f32x4_t*>(smem + first * F::kRegionB + o_chunk<HD>(r, chunk));
+        if (shares > 1) {
+            const float own_max = ml.x;
+            for (int w = 1; w < shares; ++w) ml.x = __builtin_fmaxf(ml.x, sml[first + w * step][r].x);
+            const float a = __builtin_amdgcn_exp2f(own_max - ml.x);
+            o *= a;
+            ml.y *= a;
+            for (int w = 1; w < shares; ++w) {
+                const float2 x = sml[first + w * step][r];
+                const float a2 = __builtin_amdgcn_exp2f(x.x - ml.x);
+                o += *reinterpret_cast<const f32x4_t*>(smem + (first + w * step) * F::kRegionB + o_chunk<HD>(r, chunk)) * a2;
+                ml.y = __builtin_fmaf(x.y, a2, ml.y);
             }
-        } else {
-            o = *reinterpret_cast<const f32x4_t*>(smem + (row >> 5) * F::kRegionB + o_chunk<HD>(row & 31, chunk));
-            ml = sml[row >> 5][row & 31];
         }
         *reinterpret_cast<f32x4_t*>(po + (int64_t)row * HD + chunk * 4) = o;
         if (chunk == 0) p.part_ml[prow + row] = ml;
     }
 }
 
-// Joins the parts of each row: HD / 4 lanes a row.
-template <int HD, bool BF>
+// Joins the parts of each row.  HD / 4 lanes hold a row, and G groups of them
+// take the parts in turn, four loads in flight each, so that few rows with many
+// parts do not wait for one load after the other.
+template <int HD, bool BF, int G>
 __global__ void __launch_bounds__(256) shared_prefix_join_kernel(PrefixParams p) {
-    constexpr int kChunks = HD / 4;
-    const int chunk = threadIdx.x % kChunks;
-    const int64_t row = (int64_t)blockIdx.x * (256 / kChunks) + threadIdx.x / kChunks;
-    if (row >= p.rows) return;
+    constexpr int kChunks = HD / 4, kRows = 256 / (kChunks * G);
+    const int chunk = threadIdx.x % kChunks, g = threadIdx.x / kChunks % G, r = threadIdx.x / (kChunks * G);
+    const int64_t row = (int64_t)blockIdx.x * kRows + r;
     const int parts = p.parts_p + p.parts_s;
-    float m = kEmptyMax;
-    for (int i = 0; i < parts; ++i) m = __builtin_fmaxf(m, p.part_ml[(int64_t)i * p.rows + row].x);
-    float l = 0.0f;
+    float m = kEmptyMax, l = 0.0f;
     f32x4_t o = (f32x4_t){};
-    for (int i = 0; i < parts; ++i) {
-        const int64_t at = (int64_t)i * p.rows + row;
-        const float2 ml = p.part_ml[at];
-        const float a = __builtin_amdgcn_exp2f(ml.x - m);
-        l = __builtin_fmaf(ml.y, a, l);
-        o += *reinterpret_cast<const f32x4_t*>(p.part_o + at * HD + chunk * 4) * a;
+    auto add = [&](float m2, float l2, f32x4_t o2) {
+        const float top = __builtin_fmaxf(m, m2);
+        const float a = __builtin_amdgcn_exp2f(m - top), a2 = __builtin_amdgcn_exp2f(m2 - top);
+        l = __builtin_fmaf(l, a, l2 * a2);
+        o = o * a + o2 * a2;
+        m = top;
+    };
+    if (row < p.rows) {
+        for (int i = g; i < parts; i += 4 * G) {
+            float2 ml[4];
+            f32x4_t part[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool in = i + u * G < parts;
+                const int64_t at = (int64_t)(in ? i + u * G : i) * p.rows + row;
+                ml[u] = p.part_ml[at];
+                part[u] = *reinterpret_cast<const f32x4_t*>(p.part_o + at * HD + chunk * 4);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * G < parts) add(ml[u].x, ml[u].y, part[u]);
+        }
     }
-    // a row that sees no key is zero, its partition function too
+    if constexpr (G > 1) {
+        __shared__ f32x4_t so[256];
+        __shared__ float2 sml[256 / kChunks];
+        so[threadIdx.x] = o;
+        if (chunk == 0) sml[threadIdx.x / kChunks] = make_float2(m, l);
+        __syncthreads();
+        if (g != 0) return;
+#pragma unroll
+        for (int u = 1; u < G; ++u) {
+            const float2 ml = sml[r * G + u];
+            add(ml.x, ml.y, so[threadIdx.x + u * kChunks]);
+        }
+    }
+    if (row >= p.rows) return;
+    // a row that sees no key is zero
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t kvh = row / p.mrows, mrow = row - kvh * p.mrows, bt = mrow / p.group;
     const int64_t head = kvh * p.group + (mrow - bt * p.group);
@@ -440,29 +533,29 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
     p.suffix = (int)a->suffix;
     p.mrows = a->batch * per;
     p.rows = p.mrows * p.hkv;
-    // blocks that run at once: two to a CU
-    const int64_t slots = 2 * (int64_t)device_shape().cus;
-    auto parts_for = [&](int64_t streams, int64_t keys) {
-        const int64_t most = ceil_div(keys, 256), want = ceil_div(slots, streams);
-        return want < most ? want : most;
-    };
     p.narrow_p = p.mrows <= kNarrowRows;
     p.narrow_s = per <= kNarrowRows;
     p.tiles_p = (int)ceil_div(p.mrows, kWideRows);
     p.tiles_s = (int)ceil_div(per, kWideRows);
+    // one round of blocks, two to a CU, if the caches are half full
+    const int64_t slots = 2 * (int64_t)device_shape().cus;
+    const int64_t keys = p.hkv * (p.tiles_p * a->prefix + (a->batch * p.tiles_s * a->suffix + 1) / 2);
+    int64_t each = ceil_div(keys, slots);
+    each = each < kLeastKeys ? kLeastKeys : each;
+    auto parts_of = [&](int64_t n) { return n <= each ? 1 : n / each; };
     p.parts_p = p.parts_s = 0;
     p.chunk = 64;
     if (p.prefix > 0) {
-        const int64_t parts = parts_for((int64_t)p.hkv * p.tiles_p, p.prefix);
-        p.chunk = (int)(ceil_div(ceil_div(p.prefix, parts), 64) * 64);
+        p.chunk = (int)(ceil_div(ceil_div(p.prefix, parts_of(p.prefix)), 64) * 64);
         p.parts_p = (int)ceil_div(p.prefix, p.chunk);
     }
-    if (p.suffix > 0) p.parts_s = (int)parts_for(a->batch * p.hkv * p.tiles_s, p.suffix);
+    if (p.suffix > 0) p.parts_s = (int)parts_of(p.suffix);
+    p.once = 4 * a->head_dim * p.hkv * (a->prefix + a->batch * a->suffix) >= kMallBytes;
     p.groups_p = p.hkv * p.parts_p;
     p.blocks_p = ceil_div(p.groups_p, 8) * 8 * p.tiles_p;
     const int64_t blocks_s = a->batch * p.parts_s * p.hkv * p.tiles_s;
     blocks = p.blocks_p + blocks_s;
-    return blocks <= kMaxBlocks && ceil_div(p.rows, 4) <= kMaxBlocks;
+    return blocks <= kMaxBlocks && p.rows <= kMaxBlocks;
 }
 
 bool sizes_ok(const spline_hip_shared_prefix* a) {
@@ -476,8 +569,12 @@ template <int MODE, int HD, bool BF>
 void go(const PrefixParams& p, int64_t blocks, hipStream_t st) {
     if (blocks > 0)
         hipLaunchKernelGGL((shared_prefix_kernel<MODE, HD, BF>), dim3((unsigned)blocks), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((shared_prefix_join_kernel<HD, BF>), dim3((unsigned)ceil_div(p.rows, 1024 / HD)), dim3(256), 0,
-                       st, p);
+    if (p.parts_p + p.parts_s > 4)
+        hipLaunchKernelGGL((shared_prefix_join_kernel<HD, BF, 8>), dim3((unsigned)ceil_div(p.rows, 128 / HD)), dim3(256),
+                           0, st, p);
+    else
+        hipLaunchKernelGGL((shared_prefix_join_kernel<HD, BF, 1>), dim3((unsigned)ceil_div(p.rows, 1024 / HD)), dim3(256),
+                           0, st, p);
 }
 
 template <bool BF>
