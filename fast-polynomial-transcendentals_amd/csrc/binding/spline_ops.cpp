@@ -7,6 +7,7 @@
 // AutogradCUDA / CUDA split (on ROCm the HIP device uses the CUDA dispatch
 // keys).  All compute goes through the C ABI of libspline_hip.so
 // (include/spline_ops_hip.h); nothing here computes on the host.
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 #include <torch/library.h>
 
@@ -1336,6 +1337,93 @@ struct GeluVariantFwd : public torch::autograd::Function<GeluVariantFwd> {
     }
 };
 
+// Gradients whose own gradients are not built: a graph through them, to what
+// they were made from or only through them, raises.
+variable_list once_differentiable(variable_list grads, const variable_list& from, const char* what) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list inputs;
+    std::vector<size_t> defined;
+    for (size_t i = 0; i < grads.size(); ++i)
+        if (grads[i].defined()) {
+            defined.push_back(i);
+            inputs.push_back(grads[i].detach().requires_grad_(true));
+        }
+    for (const at::Tensor& t : from)
+        if (t.defined() && t.requires_grad()) inputs.push_back(t);
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative",
+                                                                 (int64_t)inputs.size());
+    const auto raised = (*error)(std::move(inputs));
+    for (size_t i = 0; i < defined.size(); ++i) grads[defined[i]] = raised[i];
+    return grads;
+}
+
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
+c10::optional<at::Tensor> or_none(const at::Tensor& t) {
+    return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt;
+}
+
+struct QkNormRope : public torch::autograd::Function<QkNormRope> {
+    using Optional = c10::optional<at::Tensor>;
+    static variable_list forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, Optional q_weight, Optional k_weight,
+                                 at::Tensor increments, Optional positions, Optional frequency_axes, double eps,
+                                 bool interleaved) {
+        ctx->save_for_backward({q, k, or_undefined(q_weight), or_undefined(k_weight), increments,
+                                or_undefined(positions), or_undefined(frequency_axes)});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["interleaved"] = interleaved;
+        return qk_norm_rope_fwd(q, k, q_weight, k_weight, increments, positions, frequency_axes, eps, interleaved);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto g = qk_norm_rope_bwd(v[0], v[1], or_none(v[2]), or_none(v[3]), v[4], or_none(v[5]), or_none(v[6]),
+                                  grads[0], grads[1], ctx->saved_data["eps"].toDouble(),
+                                  ctx->saved_data["interleaved"].toBool());
+        variable_list out(9);
+        for (int i = 0; i < 4; ++i) out[i] = or_undefined(g[i]);
+        return once_differentiable(std::move(out), {v[0], v[1], v[2], v[3], grads[0], grads[1]}, "qk_norm_rope");
+    }
+};
+
+struct RopeAxes : public torch::autograd::Function<RopeAxes> {
+    static variable_list forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor increments,
+                                 at::Tensor positions, at::Tensor frequency_axes, bool interleaved) {
+        ctx->save_for_backward({increments, positions, frequency_axes});
+        ctx->saved_data["interleaved"] = interleaved;
+        return rope_axes_fwd(q, k, increments, positions, frequency_axes, interleaved);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto g = rope_axes_bwd(grads[0], grads[1], v[0], v[1], v[2], ctx->saved_data["interleaved"].toBool());
+        return once_differentiable({g[0], g[1], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()},
+                                   {grads[0], grads[1]}, "rope_axes");
+    }
+};
+
+// Whether autograd records a call with these operands (a node costs a decoding
+// step 1.4 us of 9).
+bool records(std::initializer_list<const at::Tensor*> operands) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor* t : operands)
+        if (t != nullptr && t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+std::vector<at::Tensor> qk_norm_rope_autograd(at::Tensor q, at::Tensor k, c10::optional<at::Tensor> q_weight,
+                                              c10::optional<at::Tensor> k_weight, at::Tensor phase_increments,
+                                              c10::optional<at::Tensor> positions,
+                                              c10::optional<at::Tensor> frequency_axes, double eps, bool interleaved) {
+    if (!records({&q, &k, q_weight ? &*q_weight : nullptr, k_weight ? &*k_weight : nullptr}))
+        return qk_norm_rope_fwd(q, k, q_weight, k_weight, phase_increments, positions, frequency_axes, eps, interleaved);
+    return QkNormRope::apply(q, k, q_weight, k_weight, phase_increments, positions, frequency_axes, eps, interleaved);
+}
+std::vector<at::Tensor> rope_axes_autograd(at::Tensor q, at::Tensor k, at::Tensor phase_increments,
+                                           at::Tensor positions, at::Tensor frequency_axes, bool interleaved) {
+    if (!records({&q, &k})) return rope_axes_fwd(q, k, phase_increments, positions, frequency_axes, interleaved);
+    return RopeAxes::apply(q, k, phase_increments, positions, frequency_axes, interleaved);
+}
+
 at::Tensor gelu_fwd_variant_autograd(at::Tensor x, int64_t degree, int64_t coeff_source_id) {
     return GeluVariantFwd::apply(x, degree, coeff_source_id);
 }
@@ -1775,6 +1863,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("k_weight"), py::arg("phase_increments"), py::arg("positions"), py::arg("frequency_axes"),
           py::arg("dq_out"), py::arg("dk_out"), py::arg("eps") = 1e-6, py::arg("interleaved") = true,
           "Gradients of qk_norm_rope_fwd -> [dq, dk, dq_weight, dk_weight] (None without a weight)");
+    m.def("qk_norm_rope_ag", &qk_norm_rope_autograd, py::arg("q"), py::arg("k"), py::arg("q_weight"),
+          py::arg("k_weight"), py::arg("phase_increments"), py::arg("positions") = c10::nullopt,
+          py::arg("frequency_axes") = c10::nullopt, py::arg("eps") = 1e-6, py::arg("interleaved") = true,
+          "qk_norm_rope_fwd with C++ autograd");
+    m.def("rope_axes_ag", &rope_axes_autograd, py::arg("q"), py::arg("k"), py::arg("phase_increments"),
+          py::arg("positions"), py::arg("frequency_axes"), py::arg("interleaved") = true,
+          "rope_axes_fwd with C++ autograd");
     m.def("rope_axes_fwd", &rope_axes_fwd, py::arg("q"), py::arg("k"), py::arg("phase_increments"),
           py::arg("positions"), py::arg("frequency_axes"), py::arg("interleaved") = true,
           "Rotary embedding by positions [axes,B,S]; q [B,S,Hq,D], k [B,S,Hk,D] -> [q [B,Hq,S,D], k [B,Hk,S,D]]");

@@ -25,6 +25,8 @@
 // What bounds it: memory, 4 bytes an element forward and 6 backward.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "ops.hpp"
 #include "spline_ops_hip.h"
 
@@ -91,6 +93,8 @@ __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
     else return as_u32((h2_t){(_Float16)lo, (_Float16)hi});
 }
 
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
 // V elements, V / 2 words.
 template <int V>
 struct Words {
@@ -108,14 +112,16 @@ __device__ __forceinline__ Words<V> load_words(const uint16_t* p) {
     }
     return o;
 }
-template <int V>
-__device__ __forceinline__ void store_words(uint16_t* p, const Words<V>& o, bool nt) {
+template <int V, bool NT>
+__device__ __forceinline__ void store_words(uint16_t* p, const Words<V>& o) {
     if constexpr (V == 8) {
         const u32x4_t v = {o.w[0], o.w[1], o.w[2], o.w[3]};
-        if (nt) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(p));
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(p));
         else *reinterpret_cast<u32x4_t*>(p) = v;
     } else {
-        *reinterpret_cast<uint2*>(p) = make_uint2(o.w[0], o.w[1]);
+        const u32x2_t v = {o.w[0], o.w[1]};
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x2_t*>(p));
+        else *reinterpret_cast<u32x2_t*>(p) = v;
     }
 }
 
@@ -131,7 +137,7 @@ struct QkSide {
     const void* w;       // [D], or null
     float* dw;           // backward: [blocks, D] partial sums, or null
     Strides xs, ys, dys;
-    int heads, groups;   // groups of HPT heads
+    int heads, splits;   // parts that the heads are cut into
     int blocks;          // backward: blocks of this side
 };
 
@@ -222,14 +228,14 @@ __device__ __forceinline__ void widen_row(const Words<V> (&raw)[2], float (&f)[2
         widen<BF>(raw[1].w[i / 2], f[V + i], f[V + i + 1]);
     }
 }
-template <bool BF, int V>
-__device__ __forceinline__ void store_row(uint16_t* row, const int (&e)[2], const float (&f)[2 * V], bool nt) {
+template <bool BF, int V, bool NT>
+__device__ __forceinline__ void store_row(uint16_t* row, const int (&e)[2], const float (&f)[2 * V]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         Words<V> o;
 #pragma unroll
         for (int i = 0; i < V; i += 2) o.w[i / 2] = narrow<BF>(f[c * V + i], f[c * V + i + 1]);
-        store_words<V>(row + e[c], o, nt);
+        store_words<V, NT>(row + e[c], o);
     }
 }
 
@@ -241,65 +247,93 @@ __device__ __forceinline__ float sum_squares(const float (&f)[2 * V]) {
     return (t[0] + t[1]) + (t[2] + t[3]);
 }
 
-// Grid (tokens / rows per block, groups of heads: the queries', then the keys').
-template <bool BF, int V, bool INTER, bool NORM, int HPT>
-__global__ void __launch_bounds__(kBlock) qk_rope_kernel(QkParams p) {
+// The heads of the queries and of the keys are cut into splits, and a block takes
+// one split of a chunk of tokens (blockIdx.x runs over the splits first), so the
+// blocks that run together share whole rows of memory, and a thread evaluates its
+// angles once for all heads of its split.  Loads of the next HPT heads are in
+// flight behind the arithmetic of these.  With the norm, w is folded into the
+// rotation, y_a = r (x_a (w_a cos) - x_b (w_b sin)), which leaves r for the end.
+template <bool BF, int V, bool INTER, bool NORM, bool NT, int HPT>
+__global__ void __launch_bounds__(kBlock, 4) qk_rope_kernel(QkParams p) {
     using Part = LanePart<V, INTER>;
-    const bool is_k = (int)blockIdx.y >= p.q.groups;
-    const uint16_t* x = is_k ? p.k.x : p.q.x;
-    uint16_t* y = is_k ? p.k.y : p.q.y;
-    const Strides xs = is_k ? p.k.xs : p.q.xs, ys = is_k ? p.k.ys : p.q.ys;
-    const int heads = is_k ? p.k.heads : p.q.heads;
-    const int h0 = ((int)blockIdx.y - (is_k ? p.q.groups : 0)) * HPT;
     const int l = threadIdx.x & ((1 << p.log_lanes) - 1);
     const bool own = l < p.lanes;
     const Part part(p, l);
-    float w[2 * V] = {};
-    if (NORM && own) part.template weights<BF>(p, is_k ? p.k.w : p.q.w, w);
-
-    const int64_t stride = (int64_t)gridDim.x * (kBlock >> p.log_lanes);
-    for (int64_t t0 = (int64_t)blockIdx.x * (kBlock >> p.log_lanes); t0 < p.tokens; t0 += stride) {
+    const uint32_t splits = p.q.splits + p.k.splits;
+    const uint32_t chunk0 = blockIdx.x / splits;
+    int split = (int)(blockIdx.x - chunk0 * splits);
+    const bool is_k = split >= p.q.splits;
+    split -= is_k ? p.q.splits : 0;
+    const int heads = is_k ? p.k.heads : p.q.heads, parts = is_k ? p.k.splits : p.q.splits;
+    const int h_begin = heads * split / parts, h_end = heads * (split + 1) / parts;
+    const Strides xs = is_k ? p.k.xs : p.q.xs, ys = is_k ? p.k.ys : p.q.ys;
+    const int64_t rows = kBlock >> p.log_lanes, stride = gridDim.x / splits * rows;
+    for (int64_t t0 = chunk0 * rows; t0 < p.tokens; t0 += stride) {
         const int64_t token = t0 + (threadIdx.x >> p.log_lanes);
         const bool in = own && token < p.tokens;
         const uint32_t b = (uint32_t)token / p.seq, s = (uint32_t)token - b * p.seq;
-        const uint16_t* xrow = x + b * xs.b + s * xs.s + h0 * xs.h;
-        Words<V> raw[HPT][2];
+        const uint16_t* x = (is_k ? p.k.x : p.q.x) + b * xs.b + s * xs.s;
+        uint16_t* y = (is_k ? p.k.y : p.q.y) + b * ys.b + s * ys.s;
+        auto load = [&](int h, Words<V> (&raw)[HPT][2]) {
 #pragma unroll
-        for (int u = 0; u < HPT; ++u)
+            for (int u = 0; u < HPT; ++u)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                raw[u][c] = Words<V>{};
-                if (in && h0 + u < heads) raw[u][c] = load_words<V>(xrow + u * xs.h + part.e[c]);
-            }
-        float cs[V] = {}, sn[V] = {};
-        if (in) part.angles(p, b, s, cs, sn);
-        uint16_t* yrow = y + b * ys.b + s * ys.s + h0 * ys.h;
-#pragma unroll
-        for (int u = 0; u < HPT; ++u) {
-            if (h0 + u >= heads) break;  // the same for every thread of the block
-            float f[2 * V];
-            widen_row<BF, V>(raw[u], f);
-            if constexpr (NORM) {
-                const float r = __builtin_amdgcn_rsqf(
-                    __builtin_fmaf(group_sum(sum_squares<V>(f), p.log_lanes), p.inv_d, p.eps));
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) f[i] = f[i] * r * w[i];
-            }
+                for (int c = 0; c < 2; ++c) {
+                    raw[u][c] = Words<V>{};
+                    if (in && h + u < h_end) raw[u][c] = load_words<V>(x + (h + u) * xs.h + part.e[c]);
+                }
+        };
+        Words<V> raw[2][HPT][2];
+        load(h_begin, raw[0]);
+        // y_a = ca x_a - sb x_b, y_b = sa x_a + cb x_b
+        float ca[V] = {}, sa[V] = {}, cb[V], sb[V];
+        if (in) part.angles(p, b, s, ca, sa);
+        if constexpr (NORM) {
+            float w[2 * V] = {};
+            if (own) part.template weights<BF>(p, is_k ? p.k.w : p.q.w, w);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float a = f[Part::first(j)], d = f[Part::second(j)];
-                f[Part::first(j)] = __builtin_fmaf(a, cs[j], -(d * sn[j]));
-                f[Part::second(j)] = __builtin_fmaf(a, sn[j], d * cs[j]);
+                cb[j] = ca[j] * w[Part::second(j)];
+                sb[j] = sa[j] * w[Part::second(j)];
+                ca[j] *= w[Part::first(j)];
+                sa[j] *= w[Part::first(j)];
             }
-            if (in) store_row<BF, V>(yrow + u * ys.h, part.e, f, p.nt);
+        }
+        auto turn = [&](int h, const Words<V> (&now)[HPT][2]) {
+#pragma unroll
+            for (int u = 0; u < HPT; ++u) {
+                if (h + u >= h_end) break;  // the same for every thread of the block
+                float f[2 * V];
+                widen_row<BF, V>(now[u], f);
+                float r = 1.0f;
+                if constexpr (NORM)
+                    r = __builtin_amdgcn_rsqf(
+                        __builtin_fmaf(group_sum(sum_squares<V>(f), p.log_lanes), p.inv_d, p.eps));
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float a = f[Part::first(j)], d = f[Part::second(j)];
+                    const float ya = __builtin_fmaf(a, ca[j], -(d * (NORM ? sb[j] : sa[j])));
+                    const float yb = __builtin_fmaf(a, sa[j], d * (NORM ? cb[j] : ca[j]));
+                    f[Part::first(j)] = NORM ? ya * r : ya;
+                    f[Part::second(j)] = NORM ? yb * r : yb;
+                }
+                if (in) store_row<BF, V, NT>(y + (h + u) * ys.h, part.e, f);
+            }
+        };
+        for (int h = h_begin; h < h_end; h += 2 * HPT) {
+            if (h + HPT < h_end) load(h + HPT, raw[1]);
+            turn(h, raw[0]);
+            if (h + HPT >= h_end) break;
+            if (h + 2 * HPT < h_end) load(h + 2 * HPT, raw[0]);
+            turn(h + HPT, raw[1]);
         }
     }
 }
 
-// Grid q.blocks + k.blocks; a block takes items (a group of heads of a chunk
-// of tokens) blocks apart.
-template <bool BF, int V, bool INTER, int HPT>
-__global__ void __launch_bounds__(kBlock) qk_rope_bwd_kernel(QkParams p) {
+// Grid q.blocks + k.blocks; a block takes items (a split of the side's heads of a
+// chunk of tokens) blocks apart, and a thread evaluates its angles once an item.
+template <bool BF, int V, bool INTER, bool NT, int HPT>
+__global__ void __launch_bounds__(kBlock, 3) qk_rope_bwd_kernel(QkParams p) {
     using Part = LanePart<V, INTER>;
     const bool is_k = (int)blockIdx.x >= p.q.blocks;
     const uint16_t* x = is_k ? p.k.x : p.q.x;
@@ -307,9 +341,9 @@ __global__ void __launch_bounds__(kBlock) qk_rope_bwd_kernel(QkParams p) {
     uint16_t* dx = is_k ? p.k.y : p.q.y;
     float* dw = is_k ? p.k.dw : p.q.dw;
     const Strides xs = is_k ? p.k.xs : p.q.xs, ys = is_k ? p.k.ys : p.q.ys, dys = is_k ? p.k.dys : p.q.dys;
-    const int heads = is_k ? p.k.heads : p.q.heads, groups = is_k ? p.k.groups : p.q.groups;
-    const int blocks = is_k ? p.k.blocks : p.q.blocks;
-    const int block = (int)blockIdx.x - (is_k ? p.q.blocks : 0);
+    const int heads = is_k ? p.k.heads : p.q.heads;
+    const uint32_t blocks = is_k ? p.k.blocks : p.q.blocks, splits = is_k ? p.k.splits : p.q.splits;
+    const uint32_t block = (uint32_t)((int)blockIdx.x - (is_k ? p.q.blocks : 0));
     const int l = threadIdx.x & ((1 << p.log_lanes) - 1), row = threadIdx.x >> p.log_lanes;
     const int rows = kBlock >> p.log_lanes;
     const bool own = l < p.lanes;
@@ -317,59 +351,66 @@ __global__ void __launch_bounds__(kBlock) qk_rope_bwd_kernel(QkParams p) {
     float w[2 * V] = {}, acc[2 * V] = {};
     if (own) part.template weights<BF>(p, is_k ? p.k.w : p.q.w, w);
 
-    // item = chunk * groups + group, stepped without a division
+    // item = chunk * splits + split, stepped without a division
     const int64_t chunks = ((int64_t)p.tokens + rows - 1) / rows;
-    int64_t chunk = (uint32_t)block / (uint32_t)groups;
-    int group = block - (int)chunk * groups;
-    const int chunk_step = (int)((uint32_t)blocks / (uint32_t)groups), group_step = blocks - chunk_step * groups;
-    for (; chunk < chunks; chunk += chunk_step + (group + group_step >= groups),
-                           group += group_step - (group + group_step >= groups ? groups : 0)) {
-        const int h0 = group * HPT;
+    const uint32_t chunk_step = blocks / splits, split_step = blocks - chunk_step * splits;
+    int64_t chunk = block / splits;
+    uint32_t split = block - (uint32_t)chunk * splits;
+    while (chunk < chunks) {
         const int64_t token = chunk * rows + row;
         const bool in = own && token < p.tokens;
         const uint32_t b = (uint32_t)token / p.seq, s = (uint32_t)token - b * p.seq;
-        const uint16_t* xrow = x + b * xs.b + s * xs.s + h0 * xs.h;
-        const uint16_t* dyrow = dy + b * dys.b + s * dys.s + h0 * dys.h;
-        uint16_t* dxrow = dx + b * ys.b + s * ys.s + h0 * ys.h;
-        Words<V> rx[HPT][2], rdy[HPT][2];
-#pragma unroll
-        for (int u = 0; u < HPT; ++u)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                rx[u][c] = rdy[u][c] = Words<V>{};
-                if (in && h0 + u < heads) {
-                    rx[u][c] = load_words<V>(xrow + u * xs.h + part.e[c]);
-                    rdy[u][c] = load_words<V>(dyrow + u * dys.h + part.e[c]);
-                }
-            }
+        const int h_begin = heads * (int)split / (int)splits, h1 = heads * ((int)split + 1) / (int)splits;
+        const uint16_t* xtoken = x + b * xs.b + s * xs.s;
+        const uint16_t* dytoken = dy + b * dys.b + s * dys.s;
+        uint16_t* dxtoken = dx + b * ys.b + s * ys.s;
         float cs[V] = {}, sn[V] = {};
-        if (in) part.angles(p, b, s, cs, sn);
+        for (int h0 = h_begin; h0 < h1; h0 += HPT) {
+            Words<V> rx[HPT][2], rdy[HPT][2];
 #pragma unroll
-        for (int u = 0; u < HPT; ++u) {
-            if (h0 + u >= heads) break;  // the same for every thread of the block
-            float n[2 * V], g[2 * V];
-            widen_row<BF, V>(rx[u], n);
-            widen_row<BF, V>(rdy[u], g);
-            const float r = __builtin_amdgcn_rsqf(
-                __builtin_fmaf(group_sum(sum_squares<V>(n), p.log_lanes), p.inv_d, p.eps));
+            for (int u = 0; u < HPT; ++u)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float a = g[Part::first(j)], d = g[Part::second(j)];
-                g[Part::first(j)] = __builtin_fmaf(a, cs[j], d * sn[j]);
-                g[Part::second(j)] = __builtin_fmaf(d, cs[j], -(a * sn[j]));
+                for (int c = 0; c < 2; ++c) {
+                    rx[u][c] = rdy[u][c] = Words<V>{};
+                    if (in && h0 + u < h1) {
+                        rx[u][c] = load_words<V>(xtoken + (h0 + u) * xs.h + part.e[c]);
+                        rdy[u][c] = load_words<V>(dytoken + (h0 + u) * dys.h + part.e[c]);
+                    }
+                }
+            if (in && h0 == h_begin) part.angles(p, b, s, cs, sn);
+#pragma unroll
+            for (int u = 0; u < HPT; ++u) {
+                if (h0 + u >= h1) break;  // the same for every thread of the block
+                float n[2 * V], g[2 * V];
+                widen_row<BF, V>(rx[u], n);
+                widen_row<BF, V>(rdy[u], g);
+                const float r = __builtin_amdgcn_rsqf(
+                    __builtin_fmaf(group_sum(sum_squares<V>(n), p.log_lanes), p.inv_d, p.eps));
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float a = g[Part::first(j)], d = g[Part::second(j)];
+                    g[Part::first(j)] = __builtin_fmaf(a, cs[j], d * sn[j]);
+                    g[Part::second(j)] = __builtin_fmaf(d, cs[j], -(a * sn[j]));
+                }
+                float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) {
+                    n[i] *= r;
+                    if (in) acc[i] = __builtin_fmaf(g[i], n[i], acc[i]);
+                    g[i] *= w[i];
+                    t[i & 3] = __builtin_fmaf(g[i], n[i], t[i & 3]);
+                }
+                const float mean = group_sum((t[0] + t[1]) + (t[2] + t[3]), p.log_lanes) * p.inv_d;
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) g[i] = r * __builtin_fmaf(n[i], -mean, g[i]);
+                if (in) store_row<BF, V, NT>(dxtoken + (h0 + u) * ys.h, part.e, g);
             }
-            float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) {
-                n[i] *= r;
-                if (in) acc[i] = __builtin_fmaf(g[i], n[i], acc[i]);
-                g[i] *= w[i];
-                t[i & 3] = __builtin_fmaf(g[i], n[i], t[i & 3]);
-            }
-            const float mean = group_sum((t[0] + t[1]) + (t[2] + t[3]), p.log_lanes) * p.inv_d;
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) g[i] = r * __builtin_fmaf(n[i], -mean, g[i]);
-            if (in) store_row<BF, V>(dxrow + u * ys.h, part.e, g, p.nt);
+        }
+        chunk += chunk_step;
+        split += split_step;
+        if (split >= splits) {
+            split -= splits;
+            ++chunk;
         }
     }
     if (dw == nullptr) return;  // the same for every thread of the block
@@ -396,21 +437,24 @@ struct DwSide {
     int rows;
 };
 
-// Adds the partial rows: 32 columns a block, 32 rows at a time.
+// Adds the partial rows: 16 columns a block, 64 rows at a time.
 template <bool BF>
 __global__ void __launch_bounds__(1024) qk_dw_kernel(DwSide q, DwSide k, int head_dim, bool w32) {
     const DwSide s = blockIdx.y ? k : q;
     if (s.part == nullptr) return;
-    const int c = threadIdx.x & 31, r0 = threadIdx.x >> 5, e = blockIdx.x * 32 + c;
+    const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
     float t = 0.0f;
-    if (e < head_dim)
-        for (int r = r0; r < s.rows; r += 32) t += s.part[(int64_t)r * head_dim + e];
-    __shared__ float sums[32][33];
+    if (e < head_dim) {
+#pragma unroll 8
+        for (int r = r0; r < s.rows; r += 64) t += s.part[(int64_t)r * head_dim + e];
+    }
+    __shared__ float sums[64][17];
     sums[r0][c] = t;
     __syncthreads();
     if (r0 != 0 || e >= head_dim) return;
     float total = 0.0f;
-    for (int r = 0; r < 32; ++r) total += sums[r][c];
+#pragma unroll 16
+    for (int r = 0; r < 64; ++r) total += sums[r][c];
     if (w32) static_cast<float*>(s.out)[e] = total;
     else static_cast<uint16_t*>(s.out)[e] = (uint16_t)narrow<BF>(total, 0.0f);
 }
@@ -489,48 +533,61 @@ int make_params(const spline_hip_qk_rope* a, bool norm, bool backward, QkParams&
     p.eps = a->eps;
     p.inv_d = 1.0f / (float)d;
     p.w32 = a->weight_f32 != 0;
-    p.nt = (a->q_heads + a->k_heads) * (int64_t)p.tokens * d * 2 >= kNtStoreBytes;
+    // Non-temporal stores from half of the elementwise kernels' threshold on for
+    // the forward: alone 22.5 us against 27.5 with 59 MiB of results, 24.7
+    // against 25.9 with 44, and neutral with the attention behind it, which reads them
+    // (40 to 59 MiB: within 1 %).  The backward keeps the threshold (63 MiB:
+    // 55 us with them, 53 without).
+    p.nt = (a->q_heads + a->k_heads) * (int64_t)p.tokens * d * 2 >= (backward ? kNtStoreBytes : kNtStoreBytes / 2);
     return hipSuccess;
 }
 
-template <bool BF, int V, bool INTER, bool NORM, int HPT>
-void run_forward(QkParams& p, hipStream_t stream) {
-    p.q.groups = (p.q.heads + HPT - 1) / HPT;
-    p.k.groups = (p.k.heads + HPT - 1) / HPT;
-    const int64_t rows = kBlock >> p.log_lanes;
-    int64_t grid = (p.tokens + rows - 1) / rows;
-    const int64_t limit = 0xffffffffll / kBlock;  // a grid counts its threads in 32 bits
-    grid = grid < limit ? grid : limit;
-    hipLaunchKernelGGL((qk_rope_kernel<BF, V, INTER, NORM, HPT>), dim3((unsigned)grid, p.q.groups + p.k.groups),
-                       dim3(kBlock), 0, stream, p);
+// Cuts the heads of both sides: 8 heads to a split, fewer where the items would
+// not make two blocks a CU.  4 x 4096 tokens, 32 + 8 heads of 128, forward /
+// backward by heads to a split: 5 64.6 / 111 us, 8 66 / 101, 16 69 / 114, all 76 / -;
+// 6001 tokens forward: 2 37.9, 6 31.5, 8 to 11 29.7 (each with cached stores).
+void cut_heads(QkParams& p, int64_t chunks) {
+    const int64_t want = (2 * device_shape().cus + chunks - 1) / chunks, heads = p.q.heads + p.k.heads;
+    auto splits = [&](int n) {
+        const int64_t even = (want * n + heads - 1) / heads, full = (n + 8 - 1) / 8;
+        return (int)(even > n ? n : even < full ? full : even);
+    };
+    p.q.splits = splits(p.q.heads);
+    p.k.splits = splits(p.k.heads);
 }
 
 template <bool BF, int V, bool INTER, bool NORM>
-void pick_heads(QkParams& p, hipStream_t stream) {
-    run_forward<BF, V, INTER, NORM, 8>(p, stream);
+void run_forward(QkParams& p, hipStream_t stream) {
+    const int64_t rows = kBlock >> p.log_lanes, chunks = (p.tokens + rows - 1) / rows;
+    cut_heads(p, chunks);
+    const int64_t splits = p.q.splits + p.k.splits;
+    const int64_t most = 0xffffffffll / kBlock / splits;  // a grid counts its threads in 32 bits
+    const int64_t grid = (chunks < most ? chunks : most) * splits;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kBlock), 0, stream, p); };
+    p.nt ? go(qk_rope_kernel<BF, V, INTER, NORM, true, 2>) : go(qk_rope_kernel<BF, V, INTER, NORM, false, 2>);
 }
 
 template <bool BF, bool NORM>
 int forward(QkParams& p, int V, bool inter, hipStream_t stream) {
     if (V == 0) return hipSuccess;
-    if (V == 8) inter ? pick_heads<BF, 8, true, NORM>(p, stream) : pick_heads<BF, 8, false, NORM>(p, stream);
-    else inter ? pick_heads<BF, 4, true, NORM>(p, stream) : pick_heads<BF, 4, false, NORM>(p, stream);
+    if (V == 8) inter ? run_forward<BF, 8, true, NORM>(p, stream) : run_forward<BF, 8, false, NORM>(p, stream);
+    else inter ? run_forward<BF, 4, true, NORM>(p, stream) : run_forward<BF, 4, false, NORM>(p, stream);
     return hipGetLastError();
 }
 
-constexpr int kBwdHeads = 4;
-constexpr int kBwdBlocks = 2048;  // of both sides, so partial rows are at most as many
+// Blocks of both sides, which bounds the partial rows (1024: 119 us at the size
+// above, where items make 2.5 rounds of them).
+constexpr int kBwdBlocks = 2048;
 
 template <bool BF>
 int backward(const spline_hip_qk_rope* a, QkParams& p, int V, hipStream_t stream) {
     if (V == 0) return hipSuccess;
     const int64_t rows = kBlock >> p.log_lanes, chunks = (p.tokens + rows - 1) / rows;
-    p.q.groups = (p.q.heads + kBwdHeads - 1) / kBwdHeads;
-    p.k.groups = (p.k.heads + kBwdHeads - 1) / kBwdHeads;
-    const int64_t items = chunks * (p.q.groups + p.k.groups);
+    cut_heads(p, chunks);
+    const int64_t items = chunks * (p.q.splits + p.k.splits);
     const int64_t each = (items + kBwdBlocks - 1) / kBwdBlocks;  // per block
-    p.q.blocks = (int)((chunks * p.q.groups + each - 1) / each);
-    p.k.blocks = (int)((chunks * p.k.groups + each - 1) / each);
+    p.q.blocks = (int)((chunks * p.q.splits + each - 1) / each);
+    p.k.blocks = (int)((chunks * p.k.splits + each - 1) / each);
     float* ws = a->dw_workspace;
     if (p.q.w) p.q.dw = ws, ws += (int64_t)p.q.blocks * p.head_dim;
     if (p.k.w) p.k.dw = ws;
@@ -539,11 +596,15 @@ int backward(const spline_hip_qk_rope* a, QkParams& p, int V, hipStream_t stream
     const dim3 grid((unsigned)(p.q.blocks + p.k.blocks));
     const bool inter = a->interleaved != 0;
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, stream, p); };
-    if (V == 8) inter ? go(qk_rope_bwd_kernel<BF, 8, true, kBwdHeads>) : go(qk_rope_bwd_kernel<BF, 8, false, kBwdHeads>);
-    else inter ? go(qk_rope_bwd_kernel<BF, 4, true, kBwdHeads>) : go(qk_rope_bwd_kernel<BF, 4, false, kBwdHeads>);
+    auto pick = [&](auto nt) {
+        constexpr bool NT = decltype(nt)::value;
+        if (V == 8) inter ? go(qk_rope_bwd_kernel<BF, 8, true, NT, 2>) : go(qk_rope_bwd_kernel<BF, 8, false, NT, 2>);
+        else inter ? go(qk_rope_bwd_kernel<BF, 4, true, NT, 2>) : go(qk_rope_bwd_kernel<BF, 4, false, NT, 2>);
+    };
+    p.nt ? pick(std::integral_constant<bool, true>{}) : pick(std::integral_constant<bool, false>{});
     int rc = hipGetLastError();
     if (rc != hipSuccess || (!p.q.w && !p.k.w)) return rc;
-    hipLaunchKernelGGL((qk_dw_kernel<BF>), dim3((p.head_dim + 31) / 32, 2), dim3(1024), 0, stream,
+    hipLaunchKernelGGL((qk_dw_kernel<BF>), dim3((p.head_dim + 15) / 16, 2), dim3(1024), 0, stream,
                        DwSide{p.q.dw, a->dq_weight, p.q.blocks}, DwSide{p.k.dw, a->dk_weight, p.k.blocks},
                        p.head_dim, p.w32);
     return hipGetLastError();

@@ -49,38 +49,6 @@ def axis_sections(sections, *, device=None) -> torch.Tensor:
     return torch.cat([torch.full((n,), axis, dtype=torch.int32) for axis, n in enumerate(counts)]).to(device)
 
 
-def _records(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, increments, positions, frequency_axes, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, increments, positions, frequency_axes)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return tuple(_ops().qk_norm_rope_fwd(q, k, q_weight, k_weight, increments, positions, frequency_axes, eps,
-                                             interleaved))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq_out, dk_out):
-        grads = _ops().qk_norm_rope_bwd(*ctx.saved_tensors, dq_out, dk_out, ctx.eps, ctx.interleaved)
-        return (*grads, None, None, None, None, None)
-
-
-class _RopeAxes(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, increments, positions, frequency_axes, interleaved):
-        ctx.save_for_backward(increments, positions, frequency_axes)
-        ctx.interleaved = interleaved
-        return tuple(_ops().rope_axes_fwd(q, k, increments, positions, frequency_axes, interleaved))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq_out, dk_out):
-        return (*_ops().rope_axes_bwd(dq_out, dk_out, *ctx.saved_tensors, ctx.interleaved), None, None, None, None)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
                  phase_increments: torch.Tensor, positions: torch.Tensor | None = None, *,
                  frequency_axes: torch.Tensor | None = None, eps: float = 1e-6,
@@ -98,11 +66,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     ``[B, S]``, ``None`` for 0..S-1, or ``[axes, B, S]`` with ``frequency_axes``
     (see :func:`rope_axes`).
     """
-    if _records(q, k, q_weight, k_weight):
-        return _QkNormRope.apply(q, k, q_weight, k_weight, phase_increments, positions, frequency_axes, float(eps),
-                                 bool(interleaved))
-    return tuple(_ops().qk_norm_rope_fwd(q, k, q_weight, k_weight, phase_increments, positions, frequency_axes,
-                                         float(eps), bool(interleaved)))
+    return tuple(_ops().qk_norm_rope_ag(q, k, q_weight, k_weight, phase_increments, positions, frequency_axes,
+                                        float(eps), bool(interleaved)))
 
 
 def rope_axes(q: torch.Tensor, k: torch.Tensor, phase_increments: torch.Tensor, positions: torch.Tensor,
@@ -115,9 +80,7 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, phase_increments: torch.Tensor, 
     :func:`axis_sections` builds one of consecutive sections).  Operands, pairs
     and layouts are those of :func:`qk_norm_rope`.
     """
-    if _records(q, k):
-        return _RopeAxes.apply(q, k, phase_increments, positions, frequency_axes, bool(interleaved))
-    return tuple(_ops().rope_axes_fwd(q, k, phase_increments, positions, frequency_axes, bool(interleaved)))
+    return tuple(_ops().rope_axes_ag(q, k, phase_increments, positions, frequency_axes, bool(interleaved)))
 
 
 __all__ = ["axis_sections", "phase_increments", "qk_norm_rope", "rope_axes"]

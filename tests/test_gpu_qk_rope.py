@@ -416,3 +416,38 @@ def test_refusals_on_the_device(cuda):
     ]:
         with pytest.raises(RuntimeError, match=message):
             rope.qk_norm_rope(**{**ok, **change})
+
+
+def test_second_derivatives_are_refused(cuda):
+    """A graph through the gradients raises where it is used, not before."""
+    from sfu_repro import rope
+
+    g = torch.Generator().manual_seed(14)
+    q, k = (torch.randn(1, 5, h, 64, generator=g).to(torch.float16).to(cuda).requires_grad_(True) for h in (4, 2))
+    inc, pos = _increments(64).to(cuda), torch.arange(5, device=cuda).expand(1, 1, 5)
+    zero = torch.zeros(32, dtype=torch.int32, device=cuda)
+    for out, name in ((rope.qk_norm_rope(q, k, None, None, inc), "qk_norm_rope"),
+                      (rope.rope_axes(q, k, inc, pos, zero), "rope_axes")):
+        d = [torch.ones_like(o).requires_grad_(True) for o in out]
+        want = torch.autograd.grad(out, [q, k], d, retain_graph=True)
+        for use in (lambda x: x.backward(), lambda x: torch.autograd.grad(x, d[0])):
+            grads = torch.autograd.grad(out, [q, k], d, create_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(grads, want))
+            with pytest.raises(RuntimeError, match=f"{name} has no second derivative"):
+                use(grads[0].sum())
+    grads = torch.autograd.grad(rope.qk_norm_rope(q, k, None, None, inc)[0].sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(grads[0].sum(), q)
+
+
+def test_saved_operands_may_not_change(cuda):
+    """An operand edited between forward and backward is refused, as elsewhere in autograd."""
+    from sfu_repro import rope
+
+    q = torch.randn(1, 5, 4, 64, device=cuda).half().requires_grad_(True)
+    k = torch.randn(1, 5, 4, 64, device=cuda).half()
+    pos = torch.arange(5, device=cuda)[None].contiguous()
+    out = rope.qk_norm_rope(q, k, None, None, _increments(64).to(cuda), pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out[0].sum().backward()
