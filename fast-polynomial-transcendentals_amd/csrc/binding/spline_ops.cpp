@@ -1901,7 +1901,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("suffix_k"), py::arg("suffix_v"), py::arg("suffix_lens"), py::arg("mode"),
           py::arg("softmax_scale"), py::arg("softcap") = 0.0,
           "Attention of new tokens [B,T,Hq,D] over a prefix [P,Hkv,D] that the batch shares and each sequence's "
-          "own cache [B,L,Hkv,D] -> [out [B,T,Hq,D], lse [B,Hq,T] FP32]; mode 0 softmax, 3 softcap");
+          "own cache [B,L,Hkv,D] -> [out [B,T,Hq,D], lse [B,Hq,T] FP32]; mode 0 softmax, 3 softcap, "
+          "4 D4 softcap (BF16)");
 
     // RoPE reference evaluator (sfu_repro.rope.polynomial_sincos on the device)
     m.def("polynomial_sincos_f32", &polynomial_sincos_f32, py::arg("angles"),

@@ -139,6 +139,39 @@ __device__ __forceinline__ float vgpr(float x) {
     return x;
 }
 
+// Launch constants of the score programs, in VGPRs (vgpr()).
+struct ScoreConsts {
+    float scale;    // s = q.k * scale
+    float sl;       // softmax modes: log2 e times the unit of the exponents
+    float cap, inv_cap, bias;
+    float tanh[SoftcapConsts::T::P.deg + 1];  // softcap D4
+};
+
+// Softmax scores of 16 accumulator registers (one 32-key tile), in the
+// units the caller's exponent FMA scales by sl: the raw dot products for
+// plain softmax (sl = scale * log2 e), the capped score y for the softcap
+// modes (sl = log2 e, so the product by log2 e is the exponent FMA's own).
+// The D4 program runs on BF16 pairs: u = bf16(bf16(s) * (1/cap)),
+// y = bf16(cap * TANH_D4_BF16(u)), the B2 program on the BF16 score.
+template <int MODE>
+__device__ __forceinline__ void softmax_exponents(const f32x16_t& acc, const ScoreConsts& k, float (&x)[16]) {
+    if constexpr (MODE == kAttnSoftcapD4) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const uint32_t u = pack_bf(rbf(acc[r] * k.scale) * k.inv_cap, rbf(acc[r + 1] * k.scale) * k.inv_cap);
+            float t0, t1;
+            SoftcapConsts::T::eval2(u, k.tanh, t0, t1);
+            x[r] = rbf(t0 * k.cap);
+            x[r + 1] = rbf(t1 * k.cap);
+        }
+    } else {
+        static_assert(MODE == kAttnSoftcapNative, "plain softmax keeps the raw dot products");
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            x[r] = k.cap * native_lane<kTanh, kFwd>(acc[r] * k.scale * k.inv_cap);
+    }
+}
+
 // x of lane l ^ 32 combined with this lane's (v_permlane32_swap_b32).
 __device__ __forceinline__ float half_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);

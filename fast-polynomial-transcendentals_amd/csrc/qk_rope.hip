@@ -31,7 +31,6 @@
 #include "spline_ops_hip.h"
 
 namespace pt {
-namespace {
 
 // sin and cos of a Q0.32 phase, FP32: the nearest quarter turn is taken off in
 // integers, t = the rest in units of 1/8 turn, |t| <= 1, and sin(pi/4 t) = t S(t^2),
@@ -332,8 +331,9 @@ __global__ void __launch_bounds__(kBlock, 4) qk_rope_kernel(QkParams p) {
 
 // Grid q.blocks + k.blocks; a block takes items (a split of the side's heads of a
 // chunk of tokens) blocks apart, and a thread evaluates its angles once an item.
+// Three waves a SIMD (168 registers), two where FP16's conversions need more.
 template <bool BF, int V, bool INTER, bool NT, int HPT>
-__global__ void __launch_bounds__(kBlock, 3) qk_rope_bwd_kernel(QkParams p) {
+__global__ void __launch_bounds__(kBlock, !BF && V == 8 ? 2 : 3) qk_rope_bwd_kernel(QkParams p) {
     using Part = LanePart<V, INTER>;
     const bool is_k = (int)blockIdx.x >= p.q.blocks;
     const uint16_t* x = is_k ? p.k.x : p.q.x;
@@ -460,6 +460,8 @@ __global__ void __launch_bounds__(1024) qk_dw_kernel(DwSide q, DwSide k, int hea
 }
 
 // ---- host side -----------------------------------------------------------------
+
+namespace {
 
 bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 

@@ -19,8 +19,8 @@
 //    the next tile flies while the scores are turned into probabilities, V of the
 //    next while the next scores are made, and no wave waits for another;
 //  * more ("wide"): each wave has 32 of 128 rows and all waves share 64-key tiles,
-//    one staged ahead (two at head_dim 64); with up to 64 rows two waves share a
-//    row and halve each tile's keys.
+//    K two and V one staged ahead (three and two at head_dim 64); with up to 64 rows
+//    two waves share a row and halve each tile's keys.
 // Products are S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16, so a lane
 // keeps one row (query) and a row's reductions stay in two lanes
 // (flash_attn.hpp).
@@ -35,7 +35,6 @@
 #include "spline_ops_hip.h"
 
 namespace pt {
-namespace {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
@@ -63,7 +62,7 @@ struct PrefixParams {
     int64_t blocks_p;
     int narrow_p, narrow_s, wide_strides;
     int once;                  // K and V do not stay in the caches
-    float sl, cap, unit;  // log2 e scale; softcap: cap, scale / cap
+    float scale, cap;
 };
 
 template <bool BF>
@@ -91,14 +90,15 @@ struct RowState {
 // keeps the exponents at 8 and below.  MASKED: keys k0 + 32 kt + 8(r/4) + 4h + r%4
 // past klast count nothing; diag = k0 + 4h - klast.
 template <int MODE, int HD, int NT, bool MASKED>
-__device__ __forceinline__ void score_tile(f32x16_t (&s)[NT], RowState<HD>& st, const PrefixParams& p, int diag) {
-    const float sl = MODE == kAttnSoftcapNative ? kLog2e : p.sl;
-    if constexpr (MODE == kAttnSoftcapNative) {
-        const float cap = p.cap, unit = p.unit;
+__device__ __forceinline__ void score_state(f32x16_t (&s)[NT], RowState<HD>& st, const ScoreConsts& k, int diag) {
+    if constexpr (!attn_is_plain_softmax(MODE)) {
 #pragma unroll
-        for (int kt = 0; kt < NT; ++kt)
+        for (int kt = 0; kt < NT; ++kt) {
+            float x[16];
+            softmax_exponents<MODE>(s[kt], k, x);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[kt][r] = cap * native_lane<kTanh, kFwd>(s[kt][r] * unit);
+            for (int r = 0; r < 16; ++r) s[kt][r] = x[r];
+        }
     }
     float mx[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
 #pragma unroll
@@ -108,7 +108,7 @@ __device__ __forceinline__ void score_tile(f32x16_t (&s)[NT], RowState<HD>& st, 
             if (MASKED && diag + kt * 32 + 8 * (r >> 2) + (r & 3) > 0) s[kt][r] = -__builtin_inff();
             mx[r & 3] = __builtin_fmaxf(mx[r & 3], s[kt][r]);
         }
-    const float mt = half_max(__builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]))) * sl;
+    const float mt = half_max(__builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]))) * k.sl;
     const bool move = mt > st.m + 8.0f;  // both lanes of a row decide alike
     __builtin_amdgcn_sched_barrier(0);
     if (__any(move)) {
@@ -120,20 +120,22 @@ __device__ __forceinline__ void score_tile(f32x16_t (&s)[NT], RowState<HD>& st, 
         for (int dt = 0; dt < HD / 32; ++dt) st.o[dt] *= alpha;
     }
     __builtin_amdgcn_sched_barrier(0);
+}
+template <int HD, int NT>
+__device__ __forceinline__ void score_exps(f32x16_t (&s)[NT], RowState<HD>& st, const ScoreConsts& k) {
     float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], sl, -st.m));
+            s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], k.sl, -st.m));
             ls[r & 3] += s[kt][r];
         }
     st.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 }
 
-// Probabilities 8 cc .. 8 cc + 7 of an accumulator as the B operand of P V,
-// rounded to the operands' 16-bit type for the matrix cores (l adds them
-// unrounded; the roundings average out over the keys).
+// Probabilities 8 cc .. 8 cc + 7 of an accumulator as the B operand of P V, in
+// the operands' 16-bit type (l adds them unrounded).
 template <bool BF>
 __device__ __forceinline__ bf16x8_t prob_frag(const f32x16_t& s, int cc) {
     if constexpr (BF) {
@@ -146,6 +148,42 @@ __device__ __forceinline__ bf16x8_t prob_frag(const f32x16_t& s, int cc) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = (_Float16)s[8 * cc + e];
         return __builtin_bit_cast(bf16x8_t, f);
+    }
+}
+// What that rounding left, as a second operand.
+template <bool BF>
+__device__ __forceinline__ bf16x8_t prob_rest(const f32x16_t& s, int cc, bf16x8_t hi) {
+    f32x16_t r = s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        r[8 * cc + e] -= BF ? (float)hi[e] : (float)__builtin_bit_cast(f16x8_t, hi)[e];
+    return prob_frag<BF>(r, cc);
+}
+
+// N loads of a wave, STEP rows apart, from row0 on, to their rows of a tile (the
+// first is tile_row).  Whole tiles take one decision for all loads; a tile with
+// rows past `last`, or rows too far apart for a lane's offset, one for each.
+template <int HD, int N, int STEP, bool ONCE>
+__device__ __forceinline__ void stage_rows(const RowLoader<HD>& loader, uint32_t tile, int tile_row, const uint16_t* base,
+                                           int64_t stride, int row0, int last) {
+    constexpr int kLoadRows = RowLoader<HD>::kLoadRows;
+    if (row0 + STEP * (N - 1) + kLoadRows - 1 <= last && !loader.wide) {  // wave-uniform
+        const uint16_t* rows = base + row0 * stride;
+        const uint32_t lane = (uint32_t)loader.lr * (uint32_t)(int)stride * 2;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = tile_row + STEP * j;
+            const uint32_t offset = lane + (uint32_t)((loader.lc ^ row_swizzle<HD>((r & 7) + loader.lr)) * 16);
+            if constexpr (ONCE) load_to_lds_once(tile + lds_row<HD>(r), rows, offset);
+            else load_to_lds(tile + lds_row<HD>(r), rows, offset);
+            rows += STEP * stride;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = tile_row + STEP * j;
+            loader.template load<ONCE>(tile + lds_row<HD>(r), r & 7, base, stride, row0 + STEP * j, last);
+        }
     }
 }
 
@@ -177,8 +215,11 @@ __device__ __forceinline__ void spill_rows(unsigned char* region, const RowState
                 (f32x4_t){st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
 }
 
+// Blocks to a CU: two at head_dim 128 (220 registers), three at 64 (168), where
+// the D4 softcap needs 172.
 template <int MODE, int HD, bool BF>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2))) shared_prefix_kernel(PrefixParams p) {
+__global__ void __launch_bounds__(256) __attribute__((
+    amdgpu_waves_per_eu(HD == 64 && MODE != kAttnSoftcapD4 ? 3 : 2))) shared_prefix_kernel(PrefixParams p) {
     using F = PrefixShape<HD>;
     constexpr int kC = HD / 16, kD = HD / 32;
     __shared__ __align__(1024) unsigned char smem[F::kLds];
@@ -241,6 +282,48 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
     const bool narrow = own ? p.narrow_s : p.narrow_p, half = !narrow && nrows <= 64;
     const int rbase = narrow ? 0 : half ? (wave & 1) * 32 : wave * 32;  // the wave's rows in the block
     const bool rin = rbase + c32 < nrows;                                // this lane has a row
+
+    // ---- staging; the first tiles fly while the rows are found
+    const RowLoader<HD> loader(lane, p.wide_strides);
+    constexpr int kLoadRows = RowLoader<HD>::kLoadRows;
+    const int all = kend > k0 ? kend - k0 : 0;
+    // narrow: wave w moves tiles w, w + 4, .. to its own place
+    constexpr int kNarrowKeys = F::kNarrowKeys, kNarrowLoads = kNarrowKeys / kLoadRows;
+    constexpr int NK = kAttnBlockK, kWideLoads = NK / kLoadRows / 4, kRing = F::kWideRing;
+    const int tiles = narrow ? (all + kNarrowKeys - 1) / kNarrowKeys : (all + NK - 1) / NK;
+    const uint32_t own_k = lds0 + (uint32_t)(wave * F::kNarrowB), own_v = own_k + F::kNarrowTileB;
+    auto load_own = [&](uint32_t lds, const uint16_t* base, int64_t stride, int i) __attribute__((always_inline)) {
+        const int row0 = k0 + i * kNarrowKeys;
+        if (p.once) stage_rows<HD, kNarrowLoads, kLoadRows, true>(loader, lds, 0, base, stride, row0, kend - 1);
+        else stage_rows<HD, kNarrowLoads, kLoadRows, false>(loader, lds, 0, base, stride, row0, kend - 1);
+    };
+    // wide: the block's rings, K a tile further ahead than V
+    constexpr uint32_t kV = kRing * F::kWideTileB;
+    auto stage_k = [&](int i) __attribute__((always_inline)) {
+        const int r = kLoadRows * wave;
+        if (i < tiles)
+            stage_rows<HD, kWideLoads, 4 * kLoadRows, false>(loader, lds0 + (uint32_t)(i % kRing * F::kWideTileB), r, kp,
+                                                             kstride, k0 + i * NK + r, kend - 1);
+    };
+    auto stage_v = [&](int i) __attribute__((always_inline)) {
+        const int r = kLoadRows * wave;
+        if (i < tiles)
+            stage_rows<HD, kWideLoads, 4 * kLoadRows, false>(loader, lds0 + kV + (uint32_t)(i % kRing * F::kWideTileB), r,
+                                                             vp, vstride, k0 + i * NK + r, kend - 1);
+    };
+    if (narrow) {
+        if (wave < tiles) {
+            load_own(own_k, kp, kstride, wave);
+            load_own(own_v, vp, vstride, wave);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) {
+            stage_k(i);
+            if (i > 0) stage_v(i - 1);
+        }
+    }
+
     // row m of a KV head is (b, t, head in the group); fewer than 2^31 of them
     const uint32_t mrow = (uint32_t)m0 + (uint32_t)(rin ? rbase + c32 : 0);
     const uint32_t bt = mrow / (uint32_t)p.group;
@@ -260,12 +343,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
         qf[c] = (bf16x8_t){};
         if (rin) qf[c] = *reinterpret_cast<const bf16x8_t*>(qrow + 16 * c + 8 * h);
     }
-    const RowLoader<HD> loader(lane, p.wide_strides);
     const TileReader<HD> reader(lane);
-    constexpr int kLoadRows = RowLoader<HD>::kLoadRows;
+    ScoreConsts consts;
+    consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
+    if constexpr (!attn_is_plain_softmax(MODE)) {
+        // in VGPRs (faster operands) where there is room
+        auto hold = [](float x) __attribute__((always_inline)) { return HD == 128 ? vgpr(x) : x; };
+        consts.scale = hold(p.scale);
+        consts.cap = hold(p.cap);
+        consts.inv_cap = hold(1.0f / p.cap);
+        if constexpr (MODE == kAttnSoftcapD4)
+#pragma unroll
+            for (int i = 1; i <= SoftcapConsts::T::P.deg; ++i) consts.tanh[i] = hold(bf16_value(SoftcapConsts::T::P.c[i]));
+    }
 
     // S^T of the NT 32-key accumulators at kt0, fragments read six ahead
-    auto scores = [&](auto& s, const unsigned char* kt0) {
+    auto scores = [&](auto& s, const unsigned char* kt0) __attribute__((always_inline)) {
         constexpr int NT = sizeof(s) / sizeof(f32x16_t), kN = NT * kC;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -285,129 +378,155 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
         __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    // O^T += V^T P^T, three fragments (two reads each) ahead
-    auto accumulate = [&](const auto& s, const unsigned char* vt0) {
+    // O^T += V^T P^T, three fragments (two reads each) ahead.  One rounding of P
+    // costs as much as the result's own (their sum is 1.4 times it).  Narrow blocks
+    // wait for memory, so they add the product with what it left (exact); in wide ones it
+    // would be a quarter of the time.
+    auto accumulate = [&](auto exact, const auto& s, const unsigned char* vt0) __attribute__((always_inline)) {
+        constexpr bool EXACT = decltype(exact)::value;
         constexpr int NT = sizeof(s) / sizeof(f32x16_t), kN = 2 * NT * kD;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 2 * NT; ++g) {
             const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
+            bf16x8_t rest;
+            if constexpr (EXACT) rest = prob_rest<BF>(s[g >> 1], g & 1, pf);
 #pragma unroll
-            for (int dt = 0; dt < kD; ++dt)
-                st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
+            for (int dt = 0; dt < kD; ++dt) {
+                const bf16x8_t v = reader.col_frag(vt0 + lds_row<HD>(16 * g), dt);
+                st.o[dt] = mfma<BF>(v, pf, st.o[dt]);
+                if constexpr (EXACT) st.o[dt] = mfma<BF>(v, rest, st.o[dt]);
+            }
         }
         __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
         for (int g = 0; g < kN - 3; ++g) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, EXACT ? 2 : 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, EXACT ? 6 : 3, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
     // the first and the last key that bound what the wave's rows see: tiles that
     // end ahead of the first need no mask, tiles behind the last no arithmetic
-    int kfull = klast, kmost = klast;
+    int kfull = kend - 1, kmost = kend - 1;
+    if (own && p.tokens > 1) {
+        kfull = kmost = klast;
 #pragma unroll
-    for (int step = 1; step < 32; step *= 2) {
-        const int x = __shfl_xor(kfull, step), y = __shfl_xor(kmost, step);
-        kfull = x < kfull ? x : kfull;
-        kmost = y > kmost ? y : kmost;
+        for (int step = 1; step < 32; step *= 2) {
+            const int x = __shfl_xor(kfull, step), y = __shfl_xor(kmost, step);
+            kfull = x < kfull ? x : kfull;
+            kmost = y > kmost ? y : kmost;
+        }
+        kfull = __builtin_amdgcn_readfirstlane(kfull);
+        kmost = __builtin_amdgcn_readfirstlane(kmost);
     }
-    kfull = __builtin_amdgcn_readfirstlane(kfull);
-    kmost = __builtin_amdgcn_readfirstlane(kmost);
 
     if (narrow) {
-        constexpr int NK = F::kNarrowKeys, NT = NK / 32, kL = NK / kLoadRows;
-        const int all = kend - k0, tiles = all > 0 ? (all + NK - 1) / NK : 0;
-        // wave w takes tiles w, w + 4, ..
-        const uint32_t ldsk = lds0 + (uint32_t)(wave * F::kNarrowB), ldsv = ldsk + F::kNarrowTileB;
+        constexpr int NT = kNarrowKeys / 32;
         const unsigned char* kt0 = smem + wave * F::kNarrowB;
         const unsigned char* vt0 = kt0 + F::kNarrowTileB;
-        auto load = [&](uint32_t lds, const uint16_t* base, int64_t stride, int tile) {
-            auto rows = [&](auto once) {
-#pragma unroll
-                for (int j = 0; j < kL; ++j)
-                    loader.template load<decltype(once)::value>(lds + lds_row<HD>(kLoadRows * j), kLoadRows * j & 7, base,
-                                                                stride, k0 + tile * NK + kLoadRows * j, kend - 1);
-            };
-            if (p.once) rows(std::integral_constant<bool, true>{});
-            else rows(std::integral_constant<bool, false>{});
-        };
-        if (wave < tiles) {
-            load(ldsk, kp, kstride, wave);
-            load(ldsv, vp, vstride, wave);
-        }
         f32x16_t s[NT];
-        auto tile = [&](auto masked, int i) {
-            wait_loads<kL>();  // K(i) has landed; V(i) may fly
+        auto tile = [&](auto masked, int i) __attribute__((always_inline)) {
+            wait_loads<kNarrowLoads>();  // K(i) has landed; V(i) may fly
             scores(s, kt0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(i) is read: its place is free
             const bool more = i + 4 < tiles;
-            if (more) load(ldsk, kp, kstride, i + 4);
-            score_tile<MODE, HD, NT, decltype(masked)::value>(s, st, p, k0 + i * NK + 4 * h - klast);
-            if (more) wait_loads<kL>();  // V(i) has landed; K(i + 4) may fly
+            if (more) load_own(own_k, kp, kstride, i + 4);
+            score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, k0 + i * kNarrowKeys + 4 * h - klast);
+            score_exps<HD, NT>(s, st, consts);
+            if (more) wait_loads<kNarrowLoads>();  // V(i) has landed; K(i + 4) may fly
             else wait_loads<0>();
-            accumulate(s, vt0);
+            accumulate(std::integral_constant<bool, true>{}, s, vt0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (more) load(ldsv, vp, vstride, i + 4);
+            if (more) load_own(own_v, vp, vstride, i + 4);
         };
-        const int full = (kfull + 1 - k0) / NK;  // tiles without a masked key (negative: none)
+        const int full = (kfull + 1 - k0) / kNarrowKeys;  // tiles without a masked key (negative: none)
         int i = wave;
         for (; i < tiles && i < full; i += 4) tile(std::integral_constant<bool, false>{}, i);
         for (; i < tiles; i += 4) tile(std::integral_constant<bool, true>{}, i);
     } else {
-        constexpr int NK = kAttnBlockK, kL = NK / kLoadRows / 4, kRing = F::kWideRing;
-        const int all = kend - k0, tiles = all > 0 ? (all + NK - 1) / NK : 0;
-        constexpr uint32_t kV = kRing * F::kWideTileB;
-        auto load = [&](uint32_t lds, const uint16_t* base, int64_t stride, int tile) {
-#pragma unroll
-            for (int j = 0; j < kL; ++j) {
-                const int r = kLoadRows * (j * 4 + wave);
-                loader.load(lds + lds_row<HD>(r), kLoadRows * wave & 7, base, stride, k0 + tile * NK + r, kend - 1);
-            }
-        };
-        auto stage = [&](int i) {
-            load(lds0 + (uint32_t)(i % kRing * F::kWideTileB), kp, kstride, i);
-            load(lds0 + kV + (uint32_t)(i % kRing * F::kWideTileB), vp, vstride, i);
-        };
-#pragma unroll
-        for (int t = 0; t < kRing - 1; ++t)
-            if (t < tiles) stage(t);
-        auto sync = [&](int i) {
-            // the loads of the kRing - 2 tiles behind tile i may still fly
-            if (kRing > 2 && i + kRing - 2 < tiles) wait_loads<2 * kL * (kRing - 2)>();
+        // sync(i), i = 0 .. tiles: K(i) and V(i - 1) are whole, and every wave is
+        // done with K(i - 1) and V(i - 2), whose places the next loads take.  The
+        // loads of the sync before may still fly where the rings hold three tiles.
+        auto sync = [&](int i) __attribute__((always_inline)) {
+            if (kRing > 2 && i + 1 < tiles) wait_loads<2 * kWideLoads * (kRing - 2)>();
             else wait_loads<0>();
-            block_barrier();  // tile i is whole, and every wave is done with tile i - 1
-            if (i + kRing - 1 < tiles) stage(i + kRing - 1);
+            block_barrier();
+            stage_k(i + kRing - 1);
+            stage_v(i + kRing - 2);
         };
         // the wave's keys of a tile: all 64, or with half of the rows 32 of them
-        auto run = [&](auto nt_c, int off) {
+        auto run = [&](auto nt_c, int off) __attribute__((always_inline)) {
             constexpr int NT = decltype(nt_c)::value;
-            f32x16_t s[NT];
-            auto tile = [&](auto masked, int i) {
-                const unsigned char* kt0 = smem + i % kRing * F::kWideTileB + lds_row<HD>(off);
-                __builtin_amdgcn_s_setprio(1);  // the other block keeps the VALU busy meanwhile
-                scores(s, kt0);
-                __builtin_amdgcn_s_setprio(0);
-                score_tile<MODE, HD, NT, decltype(masked)::value>(s, st, p, k0 + i * NK + off + 4 * h - klast);
-                accumulate(s, kt0 + kV);
-            };
+            constexpr int kFirst = 1;  // K chunks whose products go with the maximum
             // tiles without a masked key, and with one that a row sees; a wave
             // without rows only stages
             const int x = kfull + 1 - k0 - off - 32 * NT, y = kmost - k0 - off;
             const int whole = x < 0 ? 0 : x / NK + 1, most = y < 0 || rbase >= nrows ? 0 : y / NK + 1;
             const int last = most < tiles ? most : tiles;
-            int i = 0;
-            for (; i < last && i < whole; ++i) {
-                sync(i);
-                tile(std::integral_constant<bool, false>{}, i);
+            const unsigned char* ks = smem + lds_row<HD>(off);
+            auto k_tile = [&](int i) __attribute__((always_inline)) { return ks + i % kRing * F::kWideTileB; };
+            // S of tile i + 1 between the maximum and the exponentials of tile i, so
+            // that the matrix cores work while scores become probabilities.  At
+            // head_dim 64, which has 168 registers for it, it spills.  16 x 100
+            // tokens behind 8192 keys 253 us against 271, 256 sequences behind 8192
+            // 69 against 76, memory-bound cases alike; 512 tokens of one sequence
+            // 95 against 92.
+            auto step = [&](f32x16_t (&cur)[NT], f32x16_t (&nxt)[NT], int i) __attribute__((always_inline)) {
+                sync(i + 1);
+                const unsigned char *kt0 = k_tile(i + 1), *vt0 = k_tile(i) + kV;
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt) nxt[kt] = (f32x16_t){};
+#pragma unroll
+                for (int c = 0; c < kFirst; ++c)
+#pragma unroll
+                    for (int kt = 0; kt < NT; ++kt)
+                        nxt[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], nxt[kt]);
+                score_state<MODE, HD, NT, false>(cur, st, consts, 0);
+#pragma unroll
+                for (int c = kFirst; c < kC; ++c)
+#pragma unroll
+                    for (int kt = 0; kt < NT; ++kt)
+                        nxt[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], nxt[kt]);
+                score_exps<HD, NT>(cur, st, consts);
+#pragma unroll
+                for (int g = 0; g < 2 * NT; ++g) {
+                    const bf16x8_t pf = prob_frag<BF>(cur[g >> 1], g & 1);
+#pragma unroll
+                    for (int dt = 0; dt < kD; ++dt)
+                        st.o[dt] = mfma<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), pf, st.o[dt]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // one thing after the other
+            auto finish = [&](auto masked, f32x16_t (&s)[NT], int i) __attribute__((always_inline)) {
+                sync(i + 1);
+                score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, k0 + i * NK + off + 4 * h - klast);
+                score_exps<HD, NT>(s, st, consts);
+                accumulate(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);
+                if (i + 1 < last) scores(s, k_tile(i + 1));
+            };
+            int synced = 0;  // syncs met
+            if (last > 0) {
+                f32x16_t s[NT];
+                sync(0);
+                scores(s, k_tile(0));
+                int i = 0;
+                if constexpr (HD == 128) {
+                    f32x16_t s2[NT];
+                    for (; i + 2 < last && i + 1 < whole; i += 2) {
+                        step(s, s2, i);
+                        step(s2, s, i + 1);
+                    }
+                }
+                for (; i < last && i < whole; ++i) finish(std::integral_constant<bool, false>{}, s, i);
+                for (; i < last; ++i) finish(std::integral_constant<bool, true>{}, s, i);
+                synced = last + 1;
             }
-            for (; i < last; ++i) {
-                sync(i);
-                tile(std::integral_constant<bool, true>{}, i);
-            }
-            for (; i < tiles; ++i) sync(i);
+            if (tiles > 0)
+                for (int i = synced; i <= tiles; ++i) sync(i);
         };
         if (half) run(std::integral_constant<int, 1>{}, (wave >> 1) * 32);
         else run(std::integral_constant<int, 2>{}, 0);
@@ -516,6 +635,8 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(PrefixParams p)
 
 // ---- host side -----------------------------------------------------------------
 
+namespace {
+
 constexpr int64_t kMaxBlocks = 0xffffffffll / 256;  // a grid counts its threads in 32 bits
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -580,8 +701,9 @@ void go(const PrefixParams& p, int64_t blocks, hipStream_t st) {
 template <bool BF>
 int run(const spline_hip_shared_prefix* a, void* stream) {
     if (!sizes_ok(a) || !(a->scale > 0.0f && a->scale <= __FLT_MAX__)) return hipErrorInvalidValue;
-    if (a->mode != kAttnSoftmaxNative && a->mode != kAttnSoftcapNative) return hipErrorInvalidValue;
-    if (a->mode == kAttnSoftcapNative && !(a->cap > 0.0f && a->cap <= __FLT_MAX__)) return hipErrorInvalidValue;
+    if (a->mode != kAttnSoftmaxNative && a->mode != kAttnSoftcapNative && !(BF && a->mode == kAttnSoftcapD4))
+        return hipErrorInvalidValue;
+    if (a->mode != kAttnSoftmaxNative && !(a->cap > 0.0f && a->cap <= __FLT_MAX__)) return hipErrorInvalidValue;
     if (a->batch == 0 || a->tokens == 0) return hipSuccess;
     PrefixParams p{};
     int64_t blocks = 0;
@@ -617,17 +739,16 @@ int run(const spline_hip_shared_prefix* a, void* stream) {
     p.svs = {a->suffix_v_strides[0], a->suffix_v_strides[2], a->suffix_v_strides[1]};
     // staging adds up to 7 rows to a wave's address as a 32-bit byte offset
     for (const AttnStrides* s : {&p.pks, &p.pvs, &p.sks, &p.svs}) p.wide_strides |= s->s > (int64_t(1) << 27);
-    p.sl = a->scale * kLog2e;
+    p.scale = a->scale;
     p.cap = a->cap;
-    p.unit = a->scale / a->cap;
     const hipStream_t st = hs(stream);
-    if (a->head_dim == 128) {
-        if (a->mode == kAttnSoftmaxNative) go<kAttnSoftmaxNative, 128, BF>(p, blocks, st);
-        else go<kAttnSoftcapNative, 128, BF>(p, blocks, st);
-    } else {
-        if (a->mode == kAttnSoftmaxNative) go<kAttnSoftmaxNative, 64, BF>(p, blocks, st);
-        else go<kAttnSoftcapNative, 64, BF>(p, blocks, st);
-    }
+    auto head = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        a->head_dim == 128 ? go<MODE, 128, BF>(p, blocks, st) : go<MODE, 64, BF>(p, blocks, st);
+    };
+    if (a->mode == kAttnSoftmaxNative) head(std::integral_constant<int, kAttnSoftmaxNative>{});
+    else if (a->mode == kAttnSoftcapNative) head(std::integral_constant<int, kAttnSoftcapNative>{});
+    else if constexpr (BF) head(std::integral_constant<int, kAttnSoftcapD4>{});
     return hipGetLastError();
 }
 

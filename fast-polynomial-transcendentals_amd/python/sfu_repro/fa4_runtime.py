@@ -407,8 +407,9 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
 
     Any strides over a contiguous head dimension in whole multiples of 8
     elements (nothing is copied); float16 or bfloat16; head_dim 64 or 128.  The
-    score program is that of :func:`flash_attn_fwd`'s arguments; hardware softmax
-    and hardware softcap are built.  There is no backward: the operands'
+    score program is that of :func:`flash_attn_fwd`'s arguments; built are the
+    hardware softmax, the hardware softcap (``softcap``) and, for bfloat16, the D4
+    softcap (``score_mod``).  There is no backward: operands that require
     gradients are refused.
     """
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, prefix_k, prefix_v, suffix_k, suffix_v)):
@@ -416,8 +417,11 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
     if program:
         mode, _, cap, _ = select_forward(seqlen=max(1, prefix_k.shape[0]), softcap=softcap, **program)
-        if mode not in (MODE_SOFTMAX_NATIVE, MODE_SOFTCAP_NATIVE):
-            raise NotImplementedError("the shared-prefix attention is built with the hardware softmax and softcap")
+        if mode not in (MODE_SOFTMAX_NATIVE, MODE_SOFTCAP_NATIVE, MODE_SOFTCAP_D4):
+            raise NotImplementedError(
+                "the shared-prefix attention is built with the hardware softmax, the hardware softcap and the D4 softcap")
+        if mode == MODE_SOFTCAP_D4 and q.dtype != torch.bfloat16:
+            raise TypeError(f"the D4 softcap is a bfloat16 program, got {q.dtype}")
     else:
         mode, cap = (MODE_SOFTCAP_NATIVE, float(softcap)) if softcap and softcap > 0 else (MODE_SOFTMAX_NATIVE, 1.0)
     return tuple(_ops().shared_prefix_attn_fwd(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, mode, scale, cap))

@@ -748,7 +748,8 @@ int launch_flash_attention_bwd_strided_bf16_noalloc(void* dq, void* dk, void* dv
  * null: ln of the row's sum of exp(s').  A row that sees no key is zero with
  * lse -inf.  D 64 or 128, Hq a multiple of Hkv, 16-bit (P is rounded to the
  * operands' type ahead of P V; sums are FP32).  mode: 0 softmax of q.k scale,
- * 3 of cap tanh(q.k scale / cap), as in launch_flash_attention_fwd_bf16.
+ * 3 of cap tanh(q.k scale / cap), 4 (BF16 operands) of the same with the D4
+ * BF16 tanh program, as in launch_flash_attention_fwd_bf16.
  * Pointers 16-byte aligned, strides (elements) multiples of 8, head dimension
  * contiguous.  workspace: spline_hip_shared_prefix_workspace_bytes of the same
  * sizes on the same device (-1: sizes that are refused), 16-byte aligned; calls

@@ -451,3 +451,27 @@ def test_saved_operands_may_not_change(cuda):
     pos.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out[0].sum().backward()
+
+
+def test_capture_beside_a_living_eager_graph(cuda):
+    """Forward and backward captured while an eager graph of the same leaves is alive."""
+    from sfu_repro import rope
+
+    g = torch.Generator(device=cuda).manual_seed(16)
+    q, k = (torch.randn(2, 30, h, 64, generator=g, device=cuda).half().requires_grad_(True) for h in (4, 2))
+    w = torch.ones(64, device=cuda).requires_grad_(True)
+    inc = _increments(64).to(cuda)
+    d = [torch.randn(2, h, 30, 64, generator=g, device=cuda).half() for h in (4, 2)]
+    alive = rope.qk_norm_rope(q, k, w, w, inc)
+    want = torch.autograd.grad(alive, [q, k, w], d, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rope.qk_norm_rope(q, k, w, w, inc)
+        held = torch.autograd.grad(out, [q, k, w], d)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+    again = torch.autograd.grad(alive, [q, k, w], d)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))

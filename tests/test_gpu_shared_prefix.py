@@ -161,18 +161,45 @@ def test_offsets_past_32_bits(cuda):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-def test_without_prefix_is_causal_attention(spline_ops, cuda):
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("program", ["softmax", "softcap", "d4"])
+def test_without_prefix_is_causal_attention(spline_ops, cuda, program, dim):
+    """Also the D4 softcap, whose scores are the same bits in both kernels."""
     from sfu_repro import fa4_runtime
 
     g = torch.Generator().manual_seed(5)
-    q, k, v = (torch.randn(2, 200, h, 128, generator=g).to(torch.bfloat16).to(cuda) for h in (8, 2, 2))
-    none = torch.empty(0, 2, 128, dtype=torch.bfloat16, device=cuda)
+    q, k, v = (torch.randn(2, 200, h, dim, generator=g).to(torch.bfloat16).to(cuda) for h in (8, 2, 2))
+    q = q * (1 if program == "softmax" else 8)
+    args = {"softmax": {}, "softcap": {"softcap": 30.0},
+            "d4": {"score_mod": fa4_runtime.create_softcap_scoremod_backend(30.0, 4)}}[program]
+    none = torch.empty(0, 2, dim, dtype=torch.bfloat16, device=cuda)
     lens = torch.full((2,), 200, dtype=torch.int32, device=cuda)
-    out, lse = fa4_runtime.flash_attn_shared_prefix(q, none, none, k, v, lens)
-    want, want_lse = fa4_runtime.flash_attn_fwd(q, k, v, causal=True)
+    out, lse = fa4_runtime.flash_attn_shared_prefix(q, none, none, k, v, lens, **args)
+    want, want_lse = fa4_runtime.flash_attn_fwd(q, k, v, causal=True, **args)
     # both round P and the result to BF16
     assert float((out.float() - want.float()).abs().max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
     assert float((lse - want_lse).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_d4_softcap_decoding(cuda, dim):
+    """One token behind a prefix, as the last row of causal attention over the
+    whole sequence: the D4 program's scores are the same bits."""
+    from sfu_repro import fa4_runtime
+
+    g = torch.Generator().manual_seed(15)
+    s, p = 700, 600
+    q, k, v = (torch.randn(3, s, h, dim, generator=g).to(torch.bfloat16).to(cuda) for h in (8, 2, 2))
+    k, v, q = k.clone(), v.clone(), q * 8
+    k[1:, :p], v[1:, :p] = k[:1, :p], v[:1, :p]
+    mod = fa4_runtime.create_softcap_scoremod_backend(50.0, 4)
+    want, want_lse = fa4_runtime.flash_attn_fwd(q, k, v, causal=True, score_mod=mod)
+    for tokens in (1, 40):
+        lens = torch.full((3,), s - p, dtype=torch.int32, device=cuda)
+        out, lse = fa4_runtime.flash_attn_shared_prefix(q[:, -tokens:], k[0, :p], v[0, :p], k[:, p:], v[:, p:], lens,
+                                                        score_mod=mod)
+        assert float((out.float() - want[:, -tokens:].float()).abs().max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
+        assert float((lse - want_lse[..., -tokens:]).abs().max()) <= 1e-4
 
 
 def test_prefix_equals_its_copy_in_every_cache(cuda):
@@ -305,5 +332,11 @@ def test_refusals_on_the_device(cuda):
             fa4_runtime.flash_attn_shared_prefix(**{**ok, **change})
     with pytest.raises(NotImplementedError, match="hardware"):
         fa4_runtime.flash_attn_shared_prefix(**ok, exp2_emu_backend="d3", exp2_emu_freq=4)
+    mod = fa4_runtime.create_softcap_scoremod_backend(30.0, 4)
+    with pytest.raises(TypeError, match="bfloat16 program"):
+        half = {n: t.half() if t.dtype == torch.bfloat16 else t for n, t in ok.items()}
+        fa4_runtime.flash_attn_shared_prefix(**half, score_mod=mod)
+    with pytest.raises(TypeError, match="unexpected keyword"):
+        fa4_runtime.flash_attn_shared_prefix(**ok, causal=True)
     with pytest.raises(RuntimeError, match="no backward"):
         fa4_runtime.flash_attn_shared_prefix(**{**ok, "q": q.clone().requires_grad_(True)})

@@ -56,6 +56,11 @@ def test_refuses(lib, name, bad):
     assert getattr(lib, name)(ctypes.byref(_args(**bad)), None) == 1
 
 
+def test_d4_softcap_takes_bf16(lib):
+    assert lib.launch_shared_prefix_attention_fp16(ctypes.byref(_args(mode=4)), None) == 1
+    assert lib.launch_shared_prefix_attention_bf16(ctypes.byref(_args(mode=4, cap=0.0)), None) == 1
+
+
 def test_nothing_to_do(lib):
     for empty in (dict(batch=0), dict(tokens=0)):
         assert lib.launch_shared_prefix_attention_bf16(ctypes.byref(_args(**empty)), None) == 0
