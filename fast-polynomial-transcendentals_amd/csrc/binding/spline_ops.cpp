@@ -7,6 +7,7 @@
 // AutogradCUDA / CUDA split (on ROCm the HIP device uses the CUDA dispatch
 // keys).  All compute goes through the C ABI of libspline_hip.so
 // (include/spline_ops_hip.h); nothing here computes on the host.
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -19,6 +20,7 @@
 #include <cstring>
 #include <limits>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "spline_ops_hip.h"
@@ -1337,6 +1339,31 @@ struct GeluVariantFwd : public torch::autograd::Function<GeluVariantFwd> {
     }
 };
 
+// While a stream is captured into a graph, no gradient may flow into a leaf's
+// accumulation node of another stream: such a node, kept alive by an eager graph of the
+// same leaf, makes its stream wait for the captured one, which joins the capture
+// and never leaves it, and ending the capture then ends the process.
+void refuse_foreign_leaves(const at::Tensor& like, const char* what) {
+    const auto stream = c10::hip::getCurrentHIPStream(like.device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    TORCH_CHECK(hipStreamIsCapturing(stream.stream(), &status) == hipSuccess, "hipStreamIsCapturing failed");
+    if (status == hipStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    std::vector<torch::autograd::Node*> todo{node.get()};
+    std::unordered_set<torch::autograd::Node*> seen{node.get()};
+    while (!todo.empty()) {
+        torch::autograd::Node* n = todo.back();
+        todo.pop_back();
+        const auto at = n->stream();
+        TORCH_CHECK(n->name().find("AccumulateGrad") == std::string::npos || !at.has_value() || at->id() == stream.id(),
+                    what, ": cannot capture this backward pass: an eager graph of the same leaves is alive on another "
+                          "stream; delete it before the capture");
+        for (const auto& edge : n->next_edges())
+            if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+    }
+}
+
 // Gradients whose own gradients are not built: a graph through them, to what
 // they were made from or only through them, raises.
 variable_list once_differentiable(variable_list grads, const variable_list& from, const char* what) {
@@ -1374,6 +1401,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
         return qk_norm_rope_fwd(q, k, q_weight, k_weight, increments, positions, frequency_axes, eps, interleaved);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_foreign_leaves(grads[0], "qk_norm_rope");
         const auto v = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         auto g = qk_norm_rope_bwd(v[0], v[1], or_none(v[2]), or_none(v[3]), v[4], or_none(v[5]), or_none(v[6]),
@@ -1393,6 +1421,7 @@ struct RopeAxes : public torch::autograd::Function<RopeAxes> {
         return rope_axes_fwd(q, k, increments, positions, frequency_axes, interleaved);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_foreign_leaves(grads[0], "rope_axes");
         const auto v = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         auto g = rope_axes_bwd(grads[0], grads[1], v[0], v[1], v[2], ctx->saved_data["interleaved"].toBool());
