@@ -39,7 +39,11 @@ namespace pt {
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kWideRows = 128, kNarrowRows = 32;
-constexpr int kLeastKeys = 128;  // of a part: a tile for each wave of a narrow block
+constexpr int kLeastKeys = 128;   // of a part: a tile for each wave of a narrow block
+// Of a part of a cache with few rows: 64 caches of 1 to 2048 keys take 57 us in parts
+// of up to 768, 64 in one, 64 to 73 in parts of 256 to 512 (a block costs 5 us
+// beside its keys).
+constexpr int kMostOwnKeys = 768;
 constexpr float kEmptyMax = -1e30f;  // log2 units: below any score, and no infinity
 
 struct PrefixParams {
@@ -670,7 +674,12 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
         p.chunk = (int)(ceil_div(ceil_div(p.prefix, parts_of(p.prefix)), 64) * 64);
         p.parts_p = (int)ceil_div(p.prefix, p.chunk);
     }
-    if (p.suffix > 0) p.parts_s = (int)parts_of(p.suffix);
+    if (p.suffix > 0) {
+        // caches differ in length: blocks with few rows take short enough parts to
+        // even that out
+        const int64_t parts = parts_of(p.suffix), least = p.narrow_s ? ceil_div(p.suffix, kMostOwnKeys) : 1;
+        p.parts_s = (int)(parts > least ? parts : least);
+    }
     p.once = 4 * a->head_dim * p.hkv * (a->prefix + a->batch * a->suffix) >= kMallBytes;
     p.groups_p = p.hkv * p.parts_p;
     p.blocks_p = ceil_div(p.groups_p, 8) * 8 * p.tiles_p;
