@@ -12,17 +12,22 @@
 // elements, and elements from R on are only normalised.  The phase of position
 // p is p * increment in Q0.32 turns, exact modulo a turn for every position.
 //
-// A row is spread over L lanes (a power of two) that own two vectors of V
-// elements each, so both elements of every pair lie in one lane and the mean
-// takes log2 L lane exchanges.  A thread evaluates its V sines and cosines once
-// for a token and applies them to the heads of a group, whose loads it issues
-// ahead of all arithmetic.  Lanes of neighbouring rows are neighbouring tokens.
+// A lane owns one vector of V elements of a row, so that a wave's accesses are
+// whole rows of neighbouring tokens (halves of rows: a copy of rows of 64, 80 or 96
+// elements takes a quarter longer).  The other elements of its pairs lie in the same
+// vector, or in the lane half a rotated row away, which sends them (ds_bpermute).
+// With the norm a row takes a power of two of lanes, for the mean's exchanges,
+// else as many as it fills.  A thread evaluates its sines and cosines once for a
+// token and applies them to the heads of its split.
 //
 // The gradient of w sums over every row: a block keeps its sums in registers
 // over all its tokens, adds its rows through LDS and stores one partial row;
 // a second launch adds the partial rows.  Every order of addition is fixed.
 //
-// What bounds it: memory, 4 bytes an element forward and 6 backward.
+// What bounds it: memory, 4 bytes an element forward and 6 backward.  Measured at
+// 4 x 4096 tokens, 32 + 8 heads of 128 in BF16: forward 62.7 us, 5.4 TB/s, backward
+// 97.7 us, 5.2 TB/s (a copy of as much: 6.6 TB/s); the rotation alone by three axes,
+// 2 x 8190 tokens: 61.4 us, 5.5 TB/s.  Few tokens take a launch, 4 us.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -149,100 +154,140 @@ struct QkParams {
     int axis_count;
     uint32_t tokens, seq;
     int head_dim, rotary;
-    int lanes, log_lanes;   // lanes that own vectors, and log2 of the lanes of a row
+    int lanes, log_lanes;   // lanes that own vectors; log2 of the lanes between rows (with the norm)
+    int wave_rows, rows;    // rows of a wave, of a block
     float eps, inv_d;
     bool w32, neg, nt;      // FP32 weights; the inverse rotation; non-temporal stores
 };
 
-// Where a lane's two vectors lie in a row and what they turn by.
+// Where a lane's vector lies in a row, and what it turns by: y_i = c_i x_i + s_i x_i',
+// i' the other element of i's pair.
 template <int V, bool INTER>
 struct LanePart {
-    int e[2];
-    bool rot[2];
+    int e, pe;    // first element, and that of the lane with the other halves of the pairs
+    int partner;  // its lane in the wave, times 4
+    bool rot, first;
 
-    __device__ __forceinline__ LanePart(const QkParams& p, int l) {
-        if constexpr (INTER) {
-            e[0] = V * l;
-            e[1] = (p.head_dim >> 1) + V * l;
-            rot[0] = e[0] < p.rotary;
-            rot[1] = e[1] < p.rotary;
-        } else {
-            const int half = p.rotary / (2 * V);
-            rot[0] = rot[1] = l < half;
-            e[0] = l < half ? V * l : p.rotary + 2 * V * (l - half);
-            e[1] = l < half ? (p.rotary >> 1) + V * l : e[0] + V;
-        }
+    __device__ __forceinline__ LanePart(const QkParams& p, int l, int lane) {
+        const int half = p.rotary >> 1;
+        e = V * l;
+        rot = e < p.rotary;
+        first = e < half;
+        pe = INTER || !rot ? e : first ? e + half : e - half;
+        partner = 4 * (lane + (pe - e) / V);
     }
-    // Pair j < V of the lane: elements first(j), second(j) of its 2 V.
-    __device__ __forceinline__ static constexpr int first(int j) { return INTER ? 2 * j : j; }
-    __device__ __forceinline__ static constexpr int second(int j) { return INTER ? 2 * j + 1 : V + j; }
 
     __device__ __forceinline__ void angles(const QkParams& p, uint32_t b, uint32_t s, float (&cs)[V],
                                            float (&sn)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            cs[i] = 1.0f;
+            sn[i] = 0.0f;
+        }
+        if (!rot) return;
         const uint32_t* pos = p.pos == nullptr ? nullptr : p.pos + b * p.poss.b + s * p.poss.s;
         const uint32_t one = pos == nullptr ? s : p.axes == nullptr ? *pos : 0u;
+        // V / 2 angles a lane: of halves, the lane with the other half evaluates the rest
+        const int f0 = INTER ? e >> 1 : first ? e : pe + V / 2;
+        float c[V / 2], t[V / 2];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            cs[j] = 1.0f;
-            sn[j] = 0.0f;
-            if (rot[INTER && j >= V / 2]) {
-                const int f = INTER ? (j < V / 2 ? (e[0] >> 1) + j : (e[1] >> 1) + j - V / 2) : e[0] + j;
-                uint32_t at = one;
-                if (p.axes != nullptr) {
-                    const int a = p.axes[f];  // held to the axes that there are
-                    at = pos[(a < 0 ? 0 : a < p.axis_count ? a : p.axis_count - 1) * p.poss.h];
-                }
-                const uint32_t phase = at * p.inc[f];
-                phase_sincos(p.neg ? 0u - phase : phase, cs[j], sn[j]);
+        for (int j = 0; j < V / 2; ++j) {
+            uint32_t at = one;
+            if (p.axes != nullptr) {
+                const int a = p.axes[f0 + j];  // held to the axes that there are
+                at = pos[(a < 0 ? 0 : a < p.axis_count ? a : p.axis_count - 1) * p.poss.h];
+            }
+            const uint32_t phase = at * p.inc[f0 + j];
+            phase_sincos(p.neg ? 0u - phase : phase, c[j], t[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            if constexpr (INTER) {
+                cs[2 * j] = cs[2 * j + 1] = c[j];
+                sn[2 * j] = -t[j];
+                sn[2 * j + 1] = t[j];
+            } else {
+                // both lanes of a pair are here or neither is
+                const float c2 = as_f32((uint32_t)__builtin_amdgcn_ds_bpermute(partner, (int)as_u32(c[j])));
+                const float t2 = as_f32((uint32_t)__builtin_amdgcn_ds_bpermute(partner, (int)as_u32(t[j])));
+                cs[j] = first ? c[j] : c2;
+                cs[V / 2 + j] = first ? c2 : c[j];
+                sn[j] = first ? -t[j] : t2;
+                sn[V / 2 + j] = first ? -t2 : t[j];
             }
         }
     }
 
+    // w[start ..], ones without a weight.
     template <bool BF>
-    __device__ __forceinline__ void weights(const QkParams& p, const void* w, float (&out)[2 * V]) const {
+    __device__ __forceinline__ void weights(const QkParams& p, const void* w, int start, float (&out)[V]) const {
+        if (w == nullptr) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (w == nullptr) {
+            for (int i = 0; i < V; ++i) out[i] = 1.0f;
+        } else if (p.w32) {
+            const float* t = static_cast<const float*>(w) + start;
+            if (((uintptr_t)w & 15) == 0) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) out[c * V + i] = 1.0f;
-            } else if (p.w32) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) out[c * V + i] = static_cast<const float*>(w)[e[c] + i];
+                for (int i = 0; i < V; i += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(t + i);
+                    out[i] = v.x, out[i + 1] = v.y, out[i + 2] = v.z, out[i + 3] = v.w;
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const uint16_t* t = static_cast<const uint16_t*>(w) + e[c] + i;
-                    widen<BF>((uint32_t)t[0] | (uint32_t)t[1] << 16, out[c * V + i], out[c * V + i + 1]);
-                }
+                for (int i = 0; i < V; ++i) out[i] = t[i];
             }
+        } else {
+            const uint16_t* t = static_cast<const uint16_t*>(w) + start;
+            Words<V> o;
+            if (((uintptr_t)w & 15) == 0) {
+                o = load_words<V>(t);
+            } else {  // a view of other weights
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) o.w[i] = (uint32_t)t[2 * i] | (uint32_t)t[2 * i + 1] << 16;
+            }
+#pragma unroll
+            for (int i = 0; i < V; i += 2) widen<BF>(o.w[i / 2], out[i], out[i + 1]);
+        }
+    }
+
+    // The other elements of the pairs; zeros where nothing turns (an infinity
+    // there stays where it is).  All lanes take part.
+    template <bool BF>
+    __device__ __forceinline__ void others(const QkParams& p, const Words<V>& raw, const float (&f)[V],
+                                           float (&out)[V]) const {
+        if constexpr (INTER) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[i] = f[i ^ 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i)
+                widen<BF>((uint32_t)__builtin_amdgcn_ds_bpermute(partner, (int)raw.w[i]), out[2 * i], out[2 * i + 1]);
+        }
+        if (p.rotary < p.head_dim) {  // the same for every thread
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[i] = rot ? out[i] : 0.0f;
         }
     }
 };
 
 template <bool BF, int V>
-__device__ __forceinline__ void widen_row(const Words<V> (&raw)[2], float (&f)[2 * V]) {
+__device__ __forceinline__ void widen_row(const Words<V>& raw, float (&f)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-        widen<BF>(raw[0].w[i / 2], f[i], f[i + 1]);
-        widen<BF>(raw[1].w[i / 2], f[V + i], f[V + i + 1]);
-    }
+    for (int i = 0; i < V; i += 2) widen<BF>(raw.w[i / 2], f[i], f[i + 1]);
 }
 template <bool BF, int V, bool NT>
-__device__ __forceinline__ void store_row(uint16_t* row, const int (&e)[2], const float (&f)[2 * V]) {
+__device__ __forceinline__ void store_row(uint16_t* at, const float (&f)[V]) {
+    Words<V> o;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        Words<V> o;
-#pragma unroll
-        for (int i = 0; i < V; i += 2) o.w[i / 2] = narrow<BF>(f[c * V + i], f[c * V + i + 1]);
-        store_words<V, NT>(row + e[c], o);
-    }
+    for (int i = 0; i < V; i += 2) o.w[i / 2] = narrow<BF>(f[i], f[i + 1]);
+    store_words<V, NT>(at, o);
 }
 
 template <int V>
-__device__ __forceinline__ float sum_squares(const float (&f)[2 * V]) {
+__device__ __forceinline__ float sum_squares(const float (&f)[V]) {
     float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) t[i & 3] = __builtin_fmaf(f[i], f[i], t[i & 3]);
+    for (int i = 0; i < V; ++i) t[i & 3] = __builtin_fmaf(f[i], f[i], t[i & 3]);
     return (t[0] + t[1]) + (t[2] + t[3]);
 }
 
@@ -255,9 +300,12 @@ __device__ __forceinline__ float sum_squares(const float (&f)[2 * V]) {
 template <bool BF, int V, bool INTER, bool NORM, bool NT, int HPT>
 __global__ void __launch_bounds__(kBlock, 4) qk_rope_kernel(QkParams p) {
     using Part = LanePart<V, INTER>;
-    const int l = threadIdx.x & ((1 << p.log_lanes) - 1);
-    const bool own = l < p.lanes;
-    const Part part(p, l);
+    const int lane = threadIdx.x & 63;
+    const int wrow = NORM ? lane >> p.log_lanes : lane / (uint32_t)p.lanes;
+    const int l = NORM ? lane & ((1 << p.log_lanes) - 1) : lane - wrow * p.lanes;
+    const bool own = NORM ? l < p.lanes : wrow < p.wave_rows;
+    const int row = (int)(threadIdx.x >> 6) * p.wave_rows + wrow;
+    const Part part(p, own ? l : 0, own ? lane : 0);
     const uint32_t splits = p.q.splits + p.k.splits;
     const uint32_t chunk0 = blockIdx.x / splits;
     int split = (int)(blockIdx.x - chunk0 * splits);
@@ -266,57 +314,52 @@ __global__ void __launch_bounds__(kBlock, 4) qk_rope_kernel(QkParams p) {
     const int heads = is_k ? p.k.heads : p.q.heads, parts = is_k ? p.k.splits : p.q.splits;
     const int h_begin = heads * split / parts, h_end = heads * (split + 1) / parts;
     const Strides xs = is_k ? p.k.xs : p.q.xs, ys = is_k ? p.k.ys : p.q.ys;
-    const int64_t rows = kBlock >> p.log_lanes, stride = gridDim.x / splits * rows;
-    for (int64_t t0 = chunk0 * rows; t0 < p.tokens; t0 += stride) {
-        const int64_t token = t0 + (threadIdx.x >> p.log_lanes);
+    const int64_t stride = gridDim.x / splits * (int64_t)p.rows;
+    for (int64_t t0 = chunk0 * (int64_t)p.rows; t0 < p.tokens; t0 += stride) {
+        const int64_t token = t0 + row;
         const bool in = own && token < p.tokens;
         const uint32_t b = (uint32_t)token / p.seq, s = (uint32_t)token - b * p.seq;
-        const uint16_t* x = (is_k ? p.k.x : p.q.x) + b * xs.b + s * xs.s;
-        uint16_t* y = (is_k ? p.k.y : p.q.y) + b * ys.b + s * ys.s;
-        auto load = [&](int h, Words<V> (&raw)[HPT][2]) {
+        const uint16_t* x = (is_k ? p.k.x : p.q.x) + b * xs.b + s * xs.s + part.e;
+        uint16_t* y = (is_k ? p.k.y : p.q.y) + b * ys.b + s * ys.s + part.e;
+        auto load = [&](int h, Words<V> (&raw)[HPT]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < HPT; ++u)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    raw[u][c] = Words<V>{};
-                    if (in && h + u < h_end) raw[u][c] = load_words<V>(x + (h + u) * xs.h + part.e[c]);
-                }
+            for (int u = 0; u < HPT; ++u) {
+                raw[u] = Words<V>{};
+                if (in && h + u < h_end) raw[u] = load_words<V>(x + (h + u) * xs.h);
+            }
         };
-        Words<V> raw[2][HPT][2];
+        Words<V> raw[2][HPT];
         load(h_begin, raw[0]);
-        // y_a = ca x_a - sb x_b, y_b = sa x_a + cb x_b
-        float ca[V] = {}, sa[V] = {}, cb[V], sb[V];
-        if (in) part.angles(p, b, s, ca, sa);
+        float cs[V] = {}, sn[V] = {};
+        if (in) part.angles(p, b, s, cs, sn);
         if constexpr (NORM) {
-            float w[2 * V] = {};
-            if (own) part.template weights<BF>(p, is_k ? p.k.w : p.q.w, w);
+            const void* w = is_k ? p.k.w : p.q.w;
+            float mine[V] = {}, other[V] = {};
+            if (own) part.template weights<BF>(p, w, part.e, mine);
+            if (!INTER && own) part.template weights<BF>(p, w, part.pe, other);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                cb[j] = ca[j] * w[Part::second(j)];
-                sb[j] = sa[j] * w[Part::second(j)];
-                ca[j] *= w[Part::first(j)];
-                sa[j] *= w[Part::first(j)];
+            for (int i = 0; i < V; ++i) {
+                cs[i] *= mine[i];
+                sn[i] *= INTER ? mine[i ^ 1] : other[i];
             }
         }
-        auto turn = [&](int h, const Words<V> (&now)[HPT][2]) {
+        auto turn = [&](int h, const Words<V> (&now)[HPT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < HPT; ++u) {
                 if (h + u >= h_end) break;  // the same for every thread of the block
-                float f[2 * V];
+                float f[V], o[V];
                 widen_row<BF, V>(now[u], f);
+                part.template others<BF>(p, now[u], f, o);
                 float r = 1.0f;
                 if constexpr (NORM)
                     r = __builtin_amdgcn_rsqf(
                         __builtin_fmaf(group_sum(sum_squares<V>(f), p.log_lanes), p.inv_d, p.eps));
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float a = f[Part::first(j)], d = f[Part::second(j)];
-                    const float ya = __builtin_fmaf(a, ca[j], -(d * (NORM ? sb[j] : sa[j])));
-                    const float yb = __builtin_fmaf(a, sa[j], d * (NORM ? cb[j] : ca[j]));
-                    f[Part::first(j)] = NORM ? ya * r : ya;
-                    f[Part::second(j)] = NORM ? yb * r : yb;
+                for (int i = 0; i < V; ++i) {
+                    const float t = __builtin_fmaf(cs[i], f[i], sn[i] * o[i]);
+                    f[i] = NORM ? t * r : t;
                 }
-                if (in) store_row<BF, V, NT>(y + (h + u) * ys.h, part.e, f);
+                if (in) store_row<BF, V, NT>(y + (h + u) * ys.h, f);
             }
         };
         for (int h = h_begin; h < h_end; h += 2 * HPT) {
@@ -331,9 +374,8 @@ __global__ void __launch_bounds__(kBlock, 4) qk_rope_kernel(QkParams p) {
 
 // Grid q.blocks + k.blocks; a block takes items (a split of the side's heads of a
 // chunk of tokens) blocks apart, and a thread evaluates its angles once an item.
-// Three waves a SIMD (168 registers), two where FP16's conversions need more.
 template <bool BF, int V, bool INTER, bool NT, int HPT>
-__global__ void __launch_bounds__(kBlock, !BF && V == 8 ? 2 : 3) qk_rope_bwd_kernel(QkParams p) {
+__global__ void __launch_bounds__(kBlock, 4) qk_rope_bwd_kernel(QkParams p) {
     using Part = LanePart<V, INTER>;
     const bool is_k = (int)blockIdx.x >= p.q.blocks;
     const uint16_t* x = is_k ? p.k.x : p.q.x;
@@ -344,12 +386,12 @@ __global__ void __launch_bounds__(kBlock, !BF && V == 8 ? 2 : 3) qk_rope_bwd_ker
     const int heads = is_k ? p.k.heads : p.q.heads;
     const uint32_t blocks = is_k ? p.k.blocks : p.q.blocks, splits = is_k ? p.k.splits : p.q.splits;
     const uint32_t block = (uint32_t)((int)blockIdx.x - (is_k ? p.q.blocks : 0));
-    const int l = threadIdx.x & ((1 << p.log_lanes) - 1), row = threadIdx.x >> p.log_lanes;
-    const int rows = kBlock >> p.log_lanes;
+    const int lane = threadIdx.x & 63, l = lane & ((1 << p.log_lanes) - 1), rows = p.rows;
+    const int row = (int)(threadIdx.x >> 6) * p.wave_rows + (lane >> p.log_lanes);
     const bool own = l < p.lanes;
-    const Part part(p, l);
-    float w[2 * V] = {}, acc[2 * V] = {};
-    if (own) part.template weights<BF>(p, is_k ? p.k.w : p.q.w, w);
+    const Part part(p, own ? l : 0, own ? lane : 0);
+    float w[V] = {}, acc[V] = {};
+    if (own) part.template weights<BF>(p, is_k ? p.k.w : p.q.w, part.e, w);
 
     // item = chunk * splits + split, stepped without a division
     const int64_t chunks = ((int64_t)p.tokens + rows - 1) / rows;
@@ -360,41 +402,35 @@ __global__ void __launch_bounds__(kBlock, !BF && V == 8 ? 2 : 3) qk_rope_bwd_ker
         const int64_t token = chunk * rows + row;
         const bool in = own && token < p.tokens;
         const uint32_t b = (uint32_t)token / p.seq, s = (uint32_t)token - b * p.seq;
-        const int h_begin = heads * (int)split / (int)splits, h1 = heads * ((int)split + 1) / (int)splits;
-        const uint16_t* xtoken = x + b * xs.b + s * xs.s;
-        const uint16_t* dytoken = dy + b * dys.b + s * dys.s;
-        uint16_t* dxtoken = dx + b * ys.b + s * ys.s;
+        const int h_begin = heads * (int)split / (int)splits, h_end = heads * ((int)split + 1) / (int)splits;
+        const uint16_t* xtoken = x + b * xs.b + s * xs.s + part.e;
+        const uint16_t* dytoken = dy + b * dys.b + s * dys.s + part.e;
+        uint16_t* dxtoken = dx + b * ys.b + s * ys.s + part.e;
         float cs[V] = {}, sn[V] = {};
-        for (int h0 = h_begin; h0 < h1; h0 += HPT) {
-            Words<V> rx[HPT][2], rdy[HPT][2];
-#pragma unroll
-            for (int u = 0; u < HPT; ++u)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    rx[u][c] = rdy[u][c] = Words<V>{};
-                    if (in && h0 + u < h1) {
-                        rx[u][c] = load_words<V>(xtoken + (h0 + u) * xs.h + part.e[c]);
-                        rdy[u][c] = load_words<V>(dytoken + (h0 + u) * dys.h + part.e[c]);
-                    }
-                }
-            if (in && h0 == h_begin) part.angles(p, b, s, cs, sn);
+        for (int h = h_begin; h < h_end; h += HPT) {
+            Words<V> rx[HPT], rdy[HPT];
 #pragma unroll
             for (int u = 0; u < HPT; ++u) {
-                if (h0 + u >= h1) break;  // the same for every thread of the block
-                float n[2 * V], g[2 * V];
+                rx[u] = rdy[u] = Words<V>{};
+                if (in && h + u < h_end) {
+                    rx[u] = load_words<V>(xtoken + (h + u) * xs.h);
+                    rdy[u] = load_words<V>(dytoken + (h + u) * dys.h);
+                }
+            }
+            if (in && h == h_begin) part.angles(p, b, s, cs, sn);
+#pragma unroll
+            for (int u = 0; u < HPT; ++u) {
+                if (h + u >= h_end) break;  // the same for every thread of the block
+                float n[V], g[V], o[V];
                 widen_row<BF, V>(rx[u], n);
                 widen_row<BF, V>(rdy[u], g);
+                part.template others<BF>(p, rdy[u], g, o);
                 const float r = __builtin_amdgcn_rsqf(
                     __builtin_fmaf(group_sum(sum_squares<V>(n), p.log_lanes), p.inv_d, p.eps));
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float a = g[Part::first(j)], d = g[Part::second(j)];
-                    g[Part::first(j)] = __builtin_fmaf(a, cs[j], d * sn[j]);
-                    g[Part::second(j)] = __builtin_fmaf(d, cs[j], -(a * sn[j]));
-                }
                 float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < 2 * V; ++i) {
+                for (int i = 0; i < V; ++i) {
+                    g[i] = __builtin_fmaf(cs[i], g[i], -(sn[i] * o[i]));  // the rotation by -t
                     n[i] *= r;
                     if (in) acc[i] = __builtin_fmaf(g[i], n[i], acc[i]);
                     g[i] *= w[i];
@@ -402,8 +438,8 @@ __global__ void __launch_bounds__(kBlock, !BF && V == 8 ? 2 : 3) qk_rope_bwd_ker
                 }
                 const float mean = group_sum((t[0] + t[1]) + (t[2] + t[3]), p.log_lanes) * p.inv_d;
 #pragma unroll
-                for (int i = 0; i < 2 * V; ++i) g[i] = r * __builtin_fmaf(n[i], -mean, g[i]);
-                if (in) store_row<BF, V, NT>(dxtoken + (h0 + u) * ys.h, part.e, g);
+                for (int i = 0; i < V; ++i) g[i] = r * __builtin_fmaf(n[i], -mean, g[i]);
+                if (in) store_row<BF, V, NT>(dxtoken + (h + u) * ys.h, g);
             }
         }
         chunk += chunk_step;
@@ -416,12 +452,10 @@ __global__ void __launch_bounds__(kBlock, !BF && V == 8 ? 2 : 3) qk_rope_bwd_ker
     if (dw == nullptr) return;  // the same for every thread of the block
 
     // acc of every row to LDS, then one thread a column adds the rows
-    __shared__ float sums[kBlock * 2 * V];
+    __shared__ float sums[kBlock * V];
     if (own) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) sums[row * p.head_dim + part.e[c] + i] = acc[c * V + i];
+        for (int i = 0; i < V; ++i) sums[row * p.head_dim + part.e + i] = acc[i];
     }
     __syncthreads();
     for (int e = threadIdx.x; e < p.head_dim; e += kBlock) {
@@ -495,7 +529,7 @@ int make_params(const spline_hip_qk_rope* a, bool norm, bool backward, QkParams&
     if (!aligned_to(a->q_weight, wa) || !aligned_to(a->k_weight, wa)) return hipErrorInvalidValue;
 
     p = QkParams{};
-    V = d % 16 == 0 && r % 16 == 0 ? 8 : 4;
+    V = a->interleaved || r % 16 == 0 ? 8 : 4;  // a vector holds pairs, or one half of its pairs
     auto side = [&](QkSide& s, int64_t heads, const void* x, void* y, const void* w, const void* dy,
                     const int64_t (&xs)[3], const int64_t (&ys)[3], const int64_t (&dys)[3]) {
         s.heads = (int)heads;
@@ -530,28 +564,32 @@ int make_params(const spline_hip_qk_rope* a, bool norm, bool backward, QkParams&
     p.seq = (uint32_t)a->sequence_length;
     p.head_dim = (int)d;
     p.rotary = (int)r;
-    p.lanes = (int)d / (2 * V);
+    p.lanes = (int)d / V;
     while ((1 << p.log_lanes) < p.lanes) ++p.log_lanes;
+    p.wave_rows = norm ? 64 >> p.log_lanes : 64 / p.lanes;
+    p.rows = kBlock / 64 * p.wave_rows;
     p.eps = a->eps;
     p.inv_d = 1.0f / (float)d;
     p.w32 = a->weight_f32 != 0;
-    // Non-temporal stores from half of the elementwise kernels' threshold on for
-    // the forward: alone 22.5 us against 27.5 with 59 MiB of results, 24.7
-    // against 25.9 with 44, and neutral with the attention behind it, which reads them
-    // (40 to 59 MiB: within 1 %).  The backward keeps the threshold (63 MiB:
-    // 55 us with them, 53 without).
-    p.nt = (a->q_heads + a->k_heads) * (int64_t)p.tokens * d * 2 >= (backward ? kNtStoreBytes : kNtStoreBytes / 2);
+    // Non-temporal stores from half of the elementwise kernels' threshold on:
+    // forward 22.3 us against 28.6 with 59 MiB of results, 19.4 against 21.9 with 44,
+    // and neutral with the attention behind it, which reads them (40 to 59 MiB:
+    // within 1 %); backward 46.1 against 48.3 with 62 MiB, 36.4 against 40.8 with 44.
+    p.nt = (a->q_heads + a->k_heads) * (int64_t)p.tokens * d * 2 >= kNtStoreBytes / 2;
     return hipSuccess;
 }
 
-// Cuts the heads of both sides: 8 heads to a split, fewer where the items would
-// not make two blocks a CU.  4 x 4096 tokens, 32 + 8 heads of 128, forward /
-// backward by heads to a split: 5 64.6 / 111 us, 8 66 / 101, 16 69 / 114, all 76 / -;
-// 6001 tokens forward: 2 37.9, 6 31.5, 8 to 11 29.7 (each with cached stores).
-void cut_heads(QkParams& p, int64_t chunks) {
+// Cuts the heads of both sides: `each` heads to a split, 8 forward and 12 backward,
+// fewer where the items would not make two blocks a CU.  Forward / backward by heads
+// to a split, us: 4 x 4096 tokens, 32 + 8 heads of 128: 4 64.4 / 104, 8 64.7 / 103,
+// 12 63.0 / 98, 16 64.4 / 108; 2 x 4096 tokens, heads of 96: 4 30.7 / 51.6,
+// 8 24.6 / 51.9, 12 23.4 / 47.6, 16 25.1 / 47.5; 6001 tokens forward: 4 27.7, 8 22.1,
+// 12 23.4, 16 26.0.  1000 tokens, forward / backward at 2, 4 and 8 blocks a CU:
+// 7.7 / 14.8, 9.8 / 17.3, 12.3 / 18.9; 300 tokens 5.6 / 11.3, 5.5 / 9.9, 5.5 / 9.9.
+void cut_heads(QkParams& p, int64_t chunks, int each) {
     const int64_t want = (2 * device_shape().cus + chunks - 1) / chunks, heads = p.q.heads + p.k.heads;
     auto splits = [&](int n) {
-        const int64_t even = (want * n + heads - 1) / heads, full = (n + 8 - 1) / 8;
+        const int64_t even = (want * n + heads - 1) / heads, full = (n + each - 1) / each;
         return (int)(even > n ? n : even < full ? full : even);
     };
     p.q.splits = splits(p.q.heads);
@@ -560,13 +598,13 @@ void cut_heads(QkParams& p, int64_t chunks) {
 
 template <bool BF, int V, bool INTER, bool NORM>
 void run_forward(QkParams& p, hipStream_t stream) {
-    const int64_t rows = kBlock >> p.log_lanes, chunks = (p.tokens + rows - 1) / rows;
-    cut_heads(p, chunks);
+    const int64_t chunks = (p.tokens + (int64_t)p.rows - 1) / p.rows;
+    cut_heads(p, chunks, 8);
     const int64_t splits = p.q.splits + p.k.splits;
     const int64_t most = 0xffffffffll / kBlock / splits;  // a grid counts its threads in 32 bits
     const int64_t grid = (chunks < most ? chunks : most) * splits;
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kBlock), 0, stream, p); };
-    p.nt ? go(qk_rope_kernel<BF, V, INTER, NORM, true, 2>) : go(qk_rope_kernel<BF, V, INTER, NORM, false, 2>);
+    p.nt ? go(qk_rope_kernel<BF, V, INTER, NORM, true, 4>) : go(qk_rope_kernel<BF, V, INTER, NORM, false, 4>);
 }
 
 template <bool BF, bool NORM>
@@ -577,15 +615,15 @@ int forward(QkParams& p, int V, bool inter, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// Blocks of both sides, which bounds the partial rows (1024: 119 us at the size
-// above, where items make 2.5 rounds of them).
+// Blocks of both sides, which bounds the partial rows.  1024 instead: 98.8 us against
+// 97.7 at the first size above, 21.5 against 19.4 with 3003 tokens of 16 + 16 heads of 80.
 constexpr int kBwdBlocks = 2048;
 
 template <bool BF>
 int backward(const spline_hip_qk_rope* a, QkParams& p, int V, hipStream_t stream) {
     if (V == 0) return hipSuccess;
-    const int64_t rows = kBlock >> p.log_lanes, chunks = (p.tokens + rows - 1) / rows;
-    cut_heads(p, chunks);
+    const int64_t chunks = (p.tokens + (int64_t)p.rows - 1) / p.rows;
+    cut_heads(p, chunks, 12);
     const int64_t items = chunks * (p.q.splits + p.k.splits);
     const int64_t each = (items + kBwdBlocks - 1) / kBwdBlocks;  // per block
     p.q.blocks = (int)((chunks * p.q.splits + each - 1) / each);

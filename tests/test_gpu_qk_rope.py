@@ -336,6 +336,59 @@ def test_infinities_and_nan_stay_in_their_heads(cuda):
         assert torch.equal(c[0][keep], b[0][keep]) and not b[0, h, s].isfinite().all()
 
 
+@pytest.mark.parametrize("rotary", [16, 24, 40])
+@pytest.mark.parametrize("inter", [True, False])
+def test_infinities_behind_the_rotated_elements(cuda, inter, rotary):
+    """What is not turned is copied: an infinity or a NaN there reaches nothing else, and
+    one in a pair reaches that pair alone; forward and backward."""
+    from sfu_repro import rope
+
+    g = torch.Generator().manual_seed(18)
+    q, k = (torch.randn(1, 7, h, 48, generator=g).to(torch.float16).to(cuda) for h in (3, 2))
+    pos = torch.randint(0, 9999, (2, 1, 7), generator=g).to(cuda)
+    axes, inc = (torch.arange(rotary // 2) % 2).to(torch.int32).to(cuda), _increments(rotary).to(cuda)
+    other = 1 if inter else rotary // 2
+
+    def run(q, k):
+        q, k = (t.clone().requires_grad_(True) for t in (q, k))
+        out = rope.rope_axes(q, k, inc, pos, axes, interleaved=inter)
+        # the gradients at the results are the operands' values
+        return [*(o.detach().transpose(1, 2) for o in out),
+                *torch.autograd.grad(out, [q, k], [t.detach().transpose(1, 2) for t in (q, k)])]
+
+    clean = run(q, k)
+    for at, value in ((47, math.inf), (rotary, math.nan), (44, -math.inf)):
+        q[0, 2, 1, at] = k[0, 5, 0, at] = value
+    q[0, 3, 2, 0] = math.nan
+    for i, (c, b) in enumerate(zip(clean, run(q, k))):
+        where = torch.zeros(c.shape, dtype=torch.bool, device=cuda)
+        t, h = (5, 0) if i % 2 else (2, 1)
+        for at in (47, rotary, 44):
+            where[0, t, h, at] = True
+            assert torch.equal(b[0, t, h, at].nan_to_num(7.0), (q, k)[i % 2][0, t, h, at].nan_to_num(7.0))
+        if i % 2 == 0:
+            where[0, 3, 2, [0, other]] = True
+            assert bool(b[0, 3, 2, [0, other]].isnan().all())
+        assert torch.equal(c[~where], b[~where])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_at_any_address(cuda, dtype):
+    from sfu_repro import rope
+
+    g = torch.Generator().manual_seed(20)
+    q, k = (torch.randn(2, 9, h, 64, generator=g).to(torch.bfloat16).to(cuda) for h in (4, 2))
+    w = torch.randn(64, generator=g).to(dtype).to(cuda)
+    inc, d = _increments(64).to(cuda), None
+    results = []
+    for off in (0, 1, 2, 4):
+        at = torch.empty(68, dtype=dtype, device=cuda)[off: off + 64].copy_(w).requires_grad_(True)
+        out = rope.qk_norm_rope(q, k, at, at, inc, interleaved=False)
+        d = d or [torch.randn_like(o) for o in out]
+        results.append([*out, *torch.autograd.grad(out, at, d)])
+        assert all(torch.equal(a, b) for a, b in zip(results[0], results[-1]))
+
+
 def test_stream_and_graph(cuda):
     """On a stream of the caller's, and captured forward and backward: replays
     with new inputs equal eager calls bit for bit."""
