@@ -164,6 +164,24 @@ __device__ __forceinline__ bf16x8_t prob_rest(const f32x16_t& s, int cc, bf16x8_
     return prob_frag<BF>(r, cc);
 }
 
+// Values that are no finite numbers: bit 15 of each half of the result.
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & (BF ? 0x7f807f80u : 0x7c007c00u)) + (BF ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+// A BF16 fragment whose largest finite value stands for the infinities of V of one
+// sign (0 or 0x8000) and for its NaN; zeros elsewhere.
+typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
+template <bool BF>
+__device__ __forceinline__ bf16x8_t infinities(bf16x8_t f, uint16_t sign) {
+    constexpr uint16_t kInf = BF ? 0x7f80 : 0x7c00;
+    u16x8_t u = __builtin_bit_cast(u16x8_t, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        u[e] = u[e] == (kInf | sign) || (u[e] & 0x7fff) > kInf ? (uint16_t)(0x7f7f | sign) : (uint16_t)0;
+    return __builtin_bit_cast(bf16x8_t, u);
+}
+
 // N loads of a wave, STEP rows apart, from row0 on, to their rows of a tile (the
 // first is tile_row).  Whole tiles take one decision for all loads; a tile with
 // rows past `last`, or rows too far apart for a lane's offset, one for each.
@@ -411,10 +429,53 @@ __global__ void __launch_bounds__(256) __attribute__((
         __builtin_amdgcn_sched_group_barrier(0x008, EXACT ? 6 : 3, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
+    // The same for a tile with keys that some of the rows do not see: 0 * Inf is NaN,
+    // so what is not finite in V is taken out, and the rows that see it (a
+    // probability above zero) get the infinity, as four times the largest BF16
+    // value, or the NaN, as one of each sign.
+    auto accumulate_seen = [&](auto exact, const auto& s, const unsigned char* vt0) __attribute__((always_inline)) {
+        constexpr bool EXACT = decltype(exact)::value;
+        constexpr int NT = sizeof(s) / sizeof(f32x16_t);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int g = 0; g < 2 * NT; ++g) {
+            __builtin_amdgcn_sched_barrier(0);  // here and below: few registers at a time
+            const bf16x8_t pf = prob_frag<BF>(s[g >> 1], g & 1);
+            bf16x8_t rest;
+            if constexpr (EXACT) rest = prob_rest<BF>(s[g >> 1], g & 1, pf);
+#pragma unroll
+            for (int dt = 0; dt < kD; ++dt) {
+                u32x4_t v = __builtin_bit_cast(u32x4_t, reader.col_frag(vt0 + lds_row<HD>(16 * g), dt));
+                const u32x4_t t = {not_finite<BF>(v.x), not_finite<BF>(v.y), not_finite<BF>(v.z), not_finite<BF>(v.w)};
+                bad |= t.x | t.y | t.z | t.w;
+                v &= ~((t << 1) - (t >> 15));
+                st.o[dt] = mfma<BF>(__builtin_bit_cast(bf16x8_t, v), pf, st.o[dt]);
+                if constexpr (EXACT) st.o[dt] = mfma<BF>(__builtin_bit_cast(bf16x8_t, v), rest, st.o[dt]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!__any(bad != 0)) return;
+        for (uint16_t sign = 0;; sign = 0x8000) {
+#pragma unroll
+            for (int g = 0; g < 2 * NT; ++g) {
+                bf16x8_t seen;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) seen[e] = (__bf16)(s[g >> 1][8 * (g & 1) + e] > 0.0f ? 4.0f : 0.0f);
+#pragma unroll
+                for (int dt = 0; dt < kD; ++dt) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    st.o[dt] = mfma<true>(infinities<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), sign), seen, st.o[dt]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (sign) break;
+        }
+    };
+    const bool some_see = own && p.tokens > 1;
     // the first and the last key that bound what the wave's rows see: tiles that
     // end ahead of the first need no mask, tiles behind the last no arithmetic
     int kfull = kend - 1, kmost = kend - 1;
-    if (own && p.tokens > 1) {
+    if (some_see) {
         kfull = kmost = klast;
 #pragma unroll
         for (int step = 1; step < 32; step *= 2) {
@@ -441,7 +502,8 @@ __global__ void __launch_bounds__(256) __attribute__((
             score_exps<HD, NT>(s, st, consts);
             if (more) wait_loads<kNarrowLoads>();  // V(i) has landed; K(i + 4) may fly
             else wait_loads<0>();
-            accumulate(std::integral_constant<bool, true>{}, s, vt0);
+            if constexpr (decltype(masked)::value) accumulate_seen(std::integral_constant<bool, true>{}, s, vt0);
+            else accumulate(std::integral_constant<bool, true>{}, s, vt0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (more) load_own(own_v, vp, vstride, i + 4);
         };
@@ -509,7 +571,9 @@ __global__ void __launch_bounds__(256) __attribute__((
                 sync(i + 1);
                 score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, k0 + i * NK + off + 4 * h - klast);
                 score_exps<HD, NT>(s, st, consts);
-                accumulate(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);
+                if constexpr (decltype(masked)::value)
+                    accumulate_seen(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);
+                else accumulate(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);
                 if (i + 1 < last) scores(s, k_tile(i + 1));
             };
             int synced = 0;  // syncs met
@@ -689,7 +753,7 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
 }
 
 bool sizes_ok(const spline_hip_shared_prefix* a) {
-    const int64_t limit = 0x7fffffff - 4096;  // keys and tokens, with what a tile adds to them
+    const int64_t limit = 1 << 30;  // keys and tokens: those of a part's end stay within 32 bits
     return a && a->batch >= 0 && a->tokens >= 0 && a->q_heads > 0 && a->kv_heads > 0 && a->q_heads % a->kv_heads == 0 &&
            a->q_heads <= 65536 && (a->head_dim == 64 || a->head_dim == 128) && a->prefix >= 0 && a->prefix <= limit &&
            a->suffix >= 0 && a->suffix <= limit && a->tokens <= limit / 65536;

@@ -743,8 +743,8 @@ int launch_flash_attention_bwd_strided_bf16_noalloc(void* dq, void* dk, void* dv
  * sequences share, prefix_k and prefix_v [P, Hkv, D], and to the keys of their
  * own caches, suffix_k and suffix_v [B, L, Hkv, D], whose lens[b] first rows are
  * valid, the last T of them the new tokens': token t sees suffix keys
- * 0 .. lens[b] - T + t.  lens are held to 0 .. L; rows from lens[b] on may
- * hold anything.  out [B, T, Hq, D] contiguous, and lse, float [B, Hq, T] or
+ * 0 .. lens[b] - T + t.  lens are held to 0 .. L; rows that a token does not
+ * see may hold anything.  At most 2^30 keys and 2^14 tokens.  out [B, T, Hq, D] contiguous, and lse, float [B, Hq, T] or
  * null: ln of the row's sum of exp(s').  A row that sees no key is zero with
  * lse -inf.  D 64 or 128, Hq a multiple of Hkv, 16-bit (P is rounded to the
  * operands' type ahead of P V; sums are FP32).  mode: 0 softmax of q.k scale,

@@ -124,6 +124,45 @@ def test_scores_of_any_size(cuda):
     _check(fa4_runtime.flash_attn_shared_prefix(*(x.to(cuda) for x in t)), _reference(*t, 1 / math.sqrt(128), 0.0))
 
 
+# dtype, tokens, suffix, hq, hkv, dim: up to 32 rows a sequence, up to 64, 128 and more
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("case", [("bf16", 3, 40, 4, 2, 128), ("f16", 5, 33, 4, 1, 64), ("bf16", 25, 70, 4, 2, 64),
+                                  ("f16", 30, 64, 2, 1, 128), ("bf16", 100, 130, 2, 2, 128), ("f16", 90, 100, 2, 1, 64)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_what_other_tokens_see(cuda, case, cap):
+    """A key or value that is no number, ahead of the token that brings it: that
+    token and those behind it get what their sums hold, the others the same bits."""
+    from sfu_repro import fa4_runtime
+
+    dtype, tokens, suffix, hq, hkv, dim = case
+    t = [x.to(cuda) for x in _make((dtype, 2, tokens, 70, suffix, hq, hkv, dim, cap, [suffix, suffix - 2]))]
+    q, pk, pv, sk, sv, lens = t
+    clean = fa4_runtime.flash_attn_shared_prefix(*t, softcap=cap)
+    assert bool(clean[0].isfinite().all())
+    h = hkv - 1
+    heads = slice(h * hq // hkv, None)
+    for b in range(2):
+        own = int(lens[b])                      # the last token's row is own - 1
+        first, late = tokens - 2, tokens - 1    # tokens that bring what is no number
+        sv[b, own - 2, h, 5], sv[b, own - 2, h, 9], sv[b, own - 2, h, dim - 1] = math.inf, -math.inf, math.nan
+        sv[b, own - 1, h, 5], sv[b, own - 1, h, 40] = -math.inf, math.inf
+    bad = fa4_runtime.flash_attn_shared_prefix(*t, softcap=cap)
+    assert torch.equal(bad[1], clean[1])
+    want = clean[0].clone()
+    want[:, first:, heads, 5], want[:, first:, heads, 9], want[:, first:, heads, dim - 1] = math.inf, -math.inf, math.nan
+    want[:, late:, heads, 5], want[:, late:, heads, 40] = math.nan, math.inf
+    assert torch.equal(bad[0].isnan(), want.isnan())
+    assert torch.equal(bad[0].nan_to_num(7.0), want.nan_to_num(7.0))
+    # keys
+    sv[~sv.isfinite()] = 0
+    clean = fa4_runtime.flash_attn_shared_prefix(*t, softcap=cap)
+    for b in range(2):
+        sk[b, int(lens[b]) - 1, h] = math.nan
+    bad = fa4_runtime.flash_attn_shared_prefix(*t, softcap=cap)
+    assert torch.equal(bad[0][:, :late], clean[0][:, :late]) and torch.equal(bad[1][..., :late], clean[1][..., :late])
+    assert bool(bad[0][:, late:, heads].isnan().all()) and torch.equal(bad[0][:, late:, :heads.start], clean[0][:, late:, :heads.start])
+
+
 def test_layouts(cuda):
     """Heads-first caches, a query view of a packed projection, a shared cache row
     behind an expanded batch: the same bits."""

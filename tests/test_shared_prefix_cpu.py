@@ -86,3 +86,12 @@ def test_python_refuses_host_tensors():
     q, k = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         fa4_runtime.flash_attn_shared_prefix(q, k, k, k[None], k[None], torch.zeros(1, dtype=torch.int32))
+
+
+def test_limits(lib):
+    """2^30 keys and 2^14 tokens: where a part ends is counted in 32 bits."""
+    size = lambda **c: lib.spline_hip_shared_prefix_workspace_bytes(ctypes.byref(_args(**c)))
+    one = dict(batch=1, q_heads=1, kv_heads=1, head_dim=64)
+    for most in (dict(prefix=2 ** 30), dict(suffix=2 ** 30), dict(tokens=2 ** 14)):
+        assert size(**one, **most) > 0
+        assert size(**one, **{k: v + 1 for k, v in most.items()}) == -1
