@@ -44,6 +44,7 @@ constexpr int kLeastKeys = 128;   // of a part: a tile for each wave of a narrow
 // of up to 768, 64 in one, 64 to 73 in parts of 256 to 512 (a block costs 5 us
 // beside its keys).
 constexpr int kMostOwnKeys = 768;
+constexpr int kBlockKeys = 128;
 constexpr float kEmptyMax = -1e30f;  // log2 units: below any score, and no infinity
 
 struct PrefixParams {
@@ -726,9 +727,13 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
     p.narrow_s = per <= kNarrowRows;
     p.tiles_p = (int)ceil_div(p.mrows, kWideRows);
     p.tiles_s = (int)ceil_div(per, kWideRows);
-    // one round of blocks, two to a CU, if the caches are half full
+    // one round of blocks, two to a CU, if the caches are half full; a narrow block
+    // counts kBlockKeys more than its keys.  64 sequences behind 8192 keys, caches of 256:
+    // 29.5 us with 128 of them, 31.6 with none, 27.5 with 256; heads of 64: 20.5, 23.4,
+    // 22.6; 33 sequences, ungrouped heads of 64: 21.1, 22.5, 22.7.
     const int64_t slots = 2 * (int64_t)device_shape().cus;
-    const int64_t keys = p.hkv * (p.tiles_p * a->prefix + (a->batch * p.tiles_s * a->suffix + 1) / 2);
+    const int64_t per_cache = a->suffix > 0 ? (a->suffix + 1) / 2 + (p.narrow_s ? kBlockKeys : 0) : 0;
+    const int64_t keys = p.hkv * (p.tiles_p * a->prefix + a->batch * p.tiles_s * per_cache);
     int64_t each = ceil_div(keys, slots);
     each = each < kLeastKeys ? kLeastKeys : each;
     auto parts_of = [&](int64_t n) { return n <= each ? 1 : n / each; };
