@@ -734,9 +734,10 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
     // one round of blocks, two to a CU, if the caches are half full; a narrow block
     // counts kBlockKeys more than its keys.  64 sequences behind 8192 keys, caches of 256:
     // 29.5 us with 128 of them, 31.6 with none, 27.5 with 256; heads of 64: 20.5, 23.4,
-    // 22.6; 33 sequences, ungrouped heads of 64: 21.1, 22.5, 22.7.
+    // 22.6; 33 sequences, ungrouped heads of 64: 21.1, 22.5, 22.7.  32 behind 65536,
+    // caches of 3000, heads of 64: 57.8 counting each of a cache's blocks, 64.5 one.
     const int64_t slots = 2 * (int64_t)device_shape().cus;
-    const int64_t per_cache = a->suffix > 0 ? (a->suffix + 1) / 2 + (p.narrow_s ? kBlockKeys : 0) : 0;
+    const int64_t per_cache = a->suffix > 0 ? (a->suffix + 1) / 2 + (p.narrow_s ? kBlockKeys * ceil_div(a->suffix, kMostOwnKeys) : 0) : 0;
     const int64_t keys = p.hkv * (p.tiles_p * a->prefix + a->batch * p.tiles_s * per_cache);
     int64_t each = ceil_div(keys, slots);
     each = each < kLeastKeys ? kLeastKeys : each;
