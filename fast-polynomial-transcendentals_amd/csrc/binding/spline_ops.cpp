@@ -1012,6 +1012,10 @@ std::vector<at::Tensor> flash_attn_fwd_heads_first_bf16(at::Tensor q, at::Tensor
 std::vector<at::Tensor> shared_prefix_attn_fwd(at::Tensor q, at::Tensor prefix_k, at::Tensor prefix_v,
                                                at::Tensor suffix_k, at::Tensor suffix_v, at::Tensor suffix_lens,
                                                int64_t mode, double softmax_scale, double softcap) {
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || prefix_k.requires_grad() ||
+                                                 prefix_v.requires_grad() || suffix_k.requires_grad() ||
+                                                 suffix_v.requires_grad()),
+                "flash_attn_shared_prefix has no backward; call it under torch.no_grad()");
     const at::ScalarType dtype = q.scalar_type();
     TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
     TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "q must be float16 or bfloat16");

@@ -412,8 +412,6 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
     softcap (``score_mod``).  There is no backward: operands that require
     gradients are refused.
     """
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, prefix_k, prefix_v, suffix_k, suffix_v)):
-        raise RuntimeError("flash_attn_shared_prefix has no backward; call it under torch.no_grad()")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
     if program:
         mode, _, cap, _ = select_forward(seqlen=max(1, prefix_k.shape[0]), softcap=softcap, **program)
