@@ -28,9 +28,9 @@
 // What bounds it: up to about 128 rows a KV head the bytes of K and V, beyond
 // that the matrix cores and the exponentials beside them.  Measured (BF16, 32 / 8
 // heads, both launches): 2 sequences behind 131072 keys, heads of 64, 57 us, 4.7 TB/s (5.4
-// in the first launch); 64 behind 32768 with caches of up to 2048 keys, heads of 128, 95 to
-// 101 us (402 MB, 34 GFLOP); 16 x 100 tokens behind 8192 240 to 248 us, 900 TFLOP/s; 8
-// sequences behind 1024, caches of 256, 10.5 us.
+// in the first launch); 64 behind 32768 with caches of up to 2048 keys, heads of 128, 95 us
+// (403 MB, 35 GFLOP); 16 x 100 tokens behind 8192 247 us, 900 TFLOP/s; 8 sequences
+// behind 1024, caches of 256, 11 us.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -737,7 +737,8 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
     // 22.6; 33 sequences, ungrouped heads of 64: 21.1, 22.5, 22.7.  32 behind 65536,
     // caches of 3000, heads of 64: 57.8 counting each of a cache's blocks, 64.5 one.
     const int64_t slots = 2 * (int64_t)device_shape().cus;
-    const int64_t per_cache = a->suffix > 0 ? (a->suffix + 1) / 2 + (p.narrow_s ? kBlockKeys * ceil_div(a->suffix, kMostOwnKeys) : 0) : 0;
+    const int64_t own_blocks = p.narrow_s ? ceil_div(a->suffix, kMostOwnKeys) : 0;
+    const int64_t per_cache = (a->suffix + 1) / 2 + kBlockKeys * own_blocks;
     const int64_t keys = p.hkv * (p.tiles_p * a->prefix + a->batch * p.tiles_s * per_cache);
     int64_t each = ceil_div(keys, slots);
     each = each < kLeastKeys ? kLeastKeys : each;
@@ -751,7 +752,7 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
     if (p.suffix > 0) {
         // caches differ in length: blocks with few rows take short enough parts to
         // even that out
-        const int64_t parts = parts_of(p.suffix), least = p.narrow_s ? ceil_div(p.suffix, kMostOwnKeys) : 1;
+        const int64_t parts = parts_of(p.suffix), least = own_blocks > 1 ? own_blocks : 1;
         p.parts_s = (int)(parts > least ? parts : least);
     }
     p.once = 4 * a->head_dim * p.hkv * (a->prefix + a->batch * a->suffix) >= kMallBytes;
