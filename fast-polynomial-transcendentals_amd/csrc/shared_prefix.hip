@@ -755,7 +755,7 @@ bool plan(const spline_hip_shared_prefix* a, PrefixParams& p, int64_t& blocks) {
         const int64_t parts = parts_of(p.suffix), least = own_blocks > 1 ? own_blocks : 1;
         p.parts_s = (int)(parts > least ? parts : least);
     }
-    p.once = 4 * a->head_dim * p.hkv * (a->prefix + a->batch * a->suffix) >= kMallBytes;
+    p.once = 4.0 * a->head_dim * p.hkv * ((double)a->prefix + (double)a->batch * a->suffix) >= kMallBytes;
     p.groups_p = p.hkv * p.parts_p;
     p.blocks_p = ceil_div(p.groups_p, 8) * 8 * p.tiles_p;
     const int64_t blocks_s = a->batch * p.parts_s * p.hkv * p.tiles_s;
