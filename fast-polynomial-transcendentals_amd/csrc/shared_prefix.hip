@@ -174,16 +174,15 @@ template <bool BF>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return ((w & (BF ? 0x7f807f80u : 0x7c007c00u)) + (BF ? 0x00800080u : 0x04000400u)) & 0x80008000u;
 }
-// A BF16 fragment whose largest finite value stands for the infinities of V of one
-// sign (0 or 0x8000) and for its NaN; zeros elsewhere.
+// A BF16 fragment with the largest finite value in the place of what is not finite
+// in V, and zeros elsewhere.
 typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
 template <bool BF>
-__device__ __forceinline__ bf16x8_t infinities(bf16x8_t f, uint16_t sign) {
+__device__ __forceinline__ bf16x8_t where_not_finite(bf16x8_t f) {
     constexpr uint16_t kInf = BF ? 0x7f80 : 0x7c00;
     u16x8_t u = __builtin_bit_cast(u16x8_t, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        u[e] = u[e] == (kInf | sign) || (u[e] & 0x7fff) > kInf ? (uint16_t)(0x7f7f | sign) : (uint16_t)0;
+    for (int e = 0; e < 8; ++e) u[e] = (u[e] & kInf) == kInf ? (uint16_t)0x7f7f : (uint16_t)0;
     return __builtin_bit_cast(bf16x8_t, u);
 }
 
@@ -242,6 +241,23 @@ __device__ __forceinline__ void spill_rows(unsigned char* region, const RowState
                 (f32x4_t){st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
 }
 
+// The keys of part s of a cache, for rows r0 .. r0 + nrows - 1 of a sequence; seen:
+// keys that its token 0 sees (token t: t more).
+struct SuffixPart {
+    int seen, k0, kend;
+
+    __device__ __forceinline__ SuffixPart(const PrefixParams& p, int b, int s, int r0, int nrows) {
+        int len = p.lens[b];
+        len = len < 0 ? 0 : len < p.suffix ? len : p.suffix;  // held to the cache
+        seen = len - p.tokens + 1;
+        const int last_token = (r0 + nrows - 1) / p.group;
+        const int visible = seen + last_token > 0 ? seen + last_token : 0;  // keys that any row sees
+        const int each = ((visible + p.parts_s - 1) / p.parts_s + 63) & ~63;
+        k0 = s * each;
+        kend = k0 + each < visible ? k0 + each : visible;
+    }
+};
+
 // Blocks to a CU: two at head_dim 128 (220 registers), three at 64 (168), where
 // the D4 softcap needs 172.
 template <int MODE, int HD, bool BF>
@@ -296,14 +312,10 @@ __global__ void __launch_bounds__(256) __attribute__((
         vp = p.sv + b * p.svs.b + kvh * p.svs.h;
         kstride = p.sks.s;
         vstride = p.svs.s;
-        int len = p.lens[b];
-        len = len < 0 ? 0 : len < p.suffix ? len : p.suffix;  // held to the cache
-        seen = len - p.tokens + 1;
-        const int last_token = (r0 + nrows - 1) / p.group;
-        const int visible = seen + last_token > 0 ? seen + last_token : 0;  // keys that any row sees
-        const int each = ((visible + p.parts_s - 1) / p.parts_s + 63) & ~63;
-        k0 = s * each;
-        kend = k0 + each < visible ? k0 + each : visible;
+        const SuffixPart keys(p, b, s, r0, nrows);
+        seen = keys.seen;
+        k0 = keys.k0;
+        kend = keys.kend;
     }
     // the waves that share a row's keys among them: narrow four, half two, else one
     const bool narrow = own ? p.narrow_s : p.narrow_p, half = !narrow && nrows <= 64;
@@ -435,10 +447,11 @@ __global__ void __launch_bounds__(256) __attribute__((
         __builtin_amdgcn_sched_barrier(0);
     };
     // The same for a tile with keys that some of the rows do not see: 0 * Inf is NaN,
-    // so what is not finite in V is taken out, and the rows that see it (a
-    // probability above zero) get the infinity, as four times the largest BF16
-    // value, or the NaN, as one of each sign.
-    auto accumulate_seen = [&](auto exact, const auto& s, const unsigned char* vt0) __attribute__((always_inline)) {
+    // so what is not finite in V is taken out, and the rows that see its key (diag as
+    // in score_state) get an infinity, as four times the largest BF16 value.  It marks
+    // the element: the join looks up what it has to be.
+    auto accumulate_seen = [&](auto exact, const auto& s, const unsigned char* vt0, int diag)
+                               __attribute__((always_inline)) {
         constexpr bool EXACT = decltype(exact)::value;
         constexpr int NT = sizeof(s) / sizeof(f32x16_t);
         uint32_t bad = 0;
@@ -460,21 +473,20 @@ __global__ void __launch_bounds__(256) __attribute__((
         }
         __builtin_amdgcn_sched_barrier(0);
         if (!__any(bad != 0)) return;
-        for (uint16_t sign = 0;; sign = 0x8000) {
+        asm("" : "+v"(diag));  // no comparison with it is made ahead of the branch
 #pragma unroll
-            for (int g = 0; g < 2 * NT; ++g) {
-                bf16x8_t seen;
+        for (int g = 0; g < 2 * NT; ++g) {
+            bf16x8_t seen;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) seen[e] = (__bf16)(s[g >> 1][8 * (g & 1) + e] > 0.0f ? 4.0f : 0.0f);
+            for (int e = 0; e < 8; ++e)
+                seen[e] = (__bf16)(diag + 16 * g + 8 * (e >> 2) + (e & 3) > 0 ? 0.0f : 4.0f);
 #pragma unroll
-                for (int dt = 0; dt < kD; ++dt) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    st.o[dt] = mfma<true>(infinities<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt), sign), seen, st.o[dt]);
-                }
+            for (int dt = 0; dt < kD; ++dt) {
+                __builtin_amdgcn_sched_barrier(0);
+                st.o[dt] = mfma<true>(where_not_finite<BF>(reader.col_frag(vt0 + lds_row<HD>(16 * g), dt)), seen, st.o[dt]);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (sign) break;
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
     const bool some_see = own && p.tokens > 1;
     // the first and the last key that bound what the wave's rows see: tiles that
@@ -503,11 +515,12 @@ __global__ void __launch_bounds__(256) __attribute__((
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(i) is read: its place is free
             const bool more = i + 4 < tiles;
             if (more) load_own(own_k, kp, kstride, i + 4);
-            score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, k0 + i * kNarrowKeys + 4 * h - klast);
+            const int diag = k0 + i * kNarrowKeys + 4 * h - klast;
+            score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
             score_exps<HD, NT>(s, st, consts);
             if (more) wait_loads<kNarrowLoads>();  // V(i) has landed; K(i + 4) may fly
             else wait_loads<0>();
-            if constexpr (decltype(masked)::value) accumulate_seen(std::integral_constant<bool, true>{}, s, vt0);
+            if constexpr (decltype(masked)::value) accumulate_seen(std::integral_constant<bool, true>{}, s, vt0, diag);
             else accumulate(std::integral_constant<bool, true>{}, s, vt0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (more) load_own(own_v, vp, vstride, i + 4);
@@ -574,10 +587,11 @@ __global__ void __launch_bounds__(256) __attribute__((
             // one thing after the other
             auto finish = [&](auto masked, f32x16_t (&s)[NT], int i) __attribute__((always_inline)) {
                 sync(i + 1);
-                score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, k0 + i * NK + off + 4 * h - klast);
+                const int diag = k0 + i * NK + off + 4 * h - klast;
+                score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
                 score_exps<HD, NT>(s, st, consts);
                 if constexpr (decltype(masked)::value)
-                    accumulate_seen(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);
+                    accumulate_seen(std::integral_constant<bool, false>{}, s, k_tile(i) + kV, diag);
                 else accumulate(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);
                 if (i + 1 < last) scores(s, k_tile(i + 1));
             };
@@ -639,6 +653,58 @@ __global__ void __launch_bounds__(256) __attribute__((
     }
 }
 
+// Elements 4 chunk .. of a row whose sum is a number while they are not: each
+// infinity and NaN that the row sees in V, from the parts that hold one (Inf for
+// infinities of one sign, NaN otherwise).  What the parts' products made of them depends on
+// rounding: an infinity times the zero that a probability was rounded to, or times
+// what that rounding left, is a NaN or has the other sign.  An element that sees none
+// (its finite values overflowed) keeps what it has.
+template <int HD, bool BF>
+__device__ __forceinline__ void look_up_values(const PrefixParams& p, int64_t row, int chunk, f32x4_t& o) {
+    const int kvh = (int)(row / p.mrows), per = p.tokens * p.group;
+    const int64_t mrow = row - kvh * p.mrows;
+    const int b = (int)(mrow / per), r = (int)(mrow - (int64_t)b * per), t = r / p.group;
+    const int r0 = r & ~(kWideRows - 1), nrows = per - r0 < kWideRows ? per - r0 : kWideRows;
+    uint32_t plus = 0, minus = 0, nan = 0;  // a bit for each element
+    for (int i = 0; i < p.parts_p + p.parts_s; ++i) {
+        const f32x4_t x =
+            *reinterpret_cast<const f32x4_t*>(p.part_o + ((int64_t)i * p.rows + row) * HD + chunk * 4) * 0.0f;
+        if (x[0] + x[1] + x[2] + x[3] == 0.0f) continue;
+        int k, kend;
+        const uint16_t* v;
+        int64_t stride;
+        if (i < p.parts_p) {
+            k = i * p.chunk;
+            kend = k + p.chunk < p.prefix ? k + p.chunk : p.prefix;
+            v = p.pv + kvh * p.pvs.h;
+            stride = p.pvs.s;
+        } else {
+            const SuffixPart keys(p, b, i - p.parts_p, r0, nrows);
+            k = keys.k0;
+            kend = keys.kend < keys.seen + t ? keys.kend : keys.seen + t;
+            v = p.sv + b * p.svs.b + kvh * p.svs.h;
+            stride = p.svs.s;
+        }
+        constexpr uint32_t kInf = BF ? 0x7f80 : 0x7c00;
+#pragma unroll 2
+        for (; k < kend; ++k) {
+            const uint2 w = *reinterpret_cast<const uint2*>(v + k * stride + chunk * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t u = (e < 2 ? w.x : w.y) >> (e & 1) * 16 & 0xffffu;
+                plus |= (uint32_t)(u == kInf) << e;
+                minus |= (uint32_t)(u == (kInf | 0x8000u)) << e;
+                nan |= (uint32_t)((u & 0x7fffu) > kInf) << e;
+            }
+        }
+    }
+    nan |= plus & minus;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if ((plus | minus | nan) >> e & 1)
+            o[e] = as_f32(nan >> e & 1 ? 0x7fc00000u : plus >> e & 1 ? 0x7f800000u : 0xff800000u);
+}
+
 // Joins the parts of each row.  HD / 4 lanes hold a row, and G groups of them
 // take the parts in turn, four loads in flight each, so that few rows with many
 // parts do not wait for one load after the other.
@@ -687,6 +753,8 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(PrefixParams p)
         }
     }
     if (row >= p.rows) return;
+    const f32x4_t zero = o * 0.0f;  // NaN where not finite; a sum that is none makes the row NaN
+    if (zero[0] + zero[1] + zero[2] + zero[3] != 0.0f && l - l == 0.0f) look_up_values<HD, BF>(p, row, chunk, o);
     // a row that sees no key is zero
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t kvh = row / p.mrows, mrow = row - kvh * p.mrows, bt = mrow / p.group;
