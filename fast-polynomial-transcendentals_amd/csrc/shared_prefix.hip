@@ -49,7 +49,11 @@ constexpr int kLeastKeys = 128;   // of a part: a tile for each wave of a narrow
 // beside its keys).
 constexpr int kMostOwnKeys = 768;
 constexpr int kBlockKeys = 128;
-constexpr float kEmptyMax = -1e30f;  // log2 units: below any score, and no infinity
+constexpr float kEmptyMax = -__FLT_MAX__;  // log2 units: below any score, and no infinity
+// From this maximum on (log2 units) scores lose the maximum in a step of its own: an FMA
+// keeps the product's rounding, half a step of the maximum, which passes the exponents'
+// range beyond 2^30, and is 2^-4 here.
+constexpr float kFarMax = 0x1p20f;
 
 struct PrefixParams {
     const uint16_t* q;
@@ -94,12 +98,12 @@ struct RowState {
     }
 };
 
-// One tile of NT 32-key accumulators of scores: s becomes probabilities, O and
-// l are rescaled if the tile raises the maximum by more than 8 (log2), which
-// keeps the exponents at 8 and below.  MASKED: keys k0 + 32 kt + 8(r/4) + 4h + r%4
+// One tile of NT 32-key accumulators of scores, to become probabilities 2^(s f - m)
+// with the factor f that score_state returns.  O and l are rescaled if the tile raises
+// the maximum by more than 8 (log2), which keeps the exponents at 8 and below.  MASKED: keys k0 + 32 kt + 8(r/4) + 4h + r%4
 // past klast count nothing; diag = k0 + 4h - klast.
 template <int MODE, int HD, int NT, bool MASKED>
-__device__ __forceinline__ void score_state(f32x16_t (&s)[NT], RowState<HD>& st, const ScoreConsts& k, int diag) {
+__device__ __forceinline__ float score_state(f32x16_t (&s)[NT], RowState<HD>& st, const ScoreConsts& k, int diag) {
     if constexpr (!attn_is_plain_softmax(MODE)) {
 #pragma unroll
         for (int kt = 0; kt < NT; ++kt) {
@@ -118,7 +122,7 @@ __device__ __forceinline__ void score_state(f32x16_t (&s)[NT], RowState<HD>& st,
             mx[r & 3] = __builtin_fmaxf(mx[r & 3], s[kt][r]);
         }
     const float mt = half_max(__builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]))) * k.sl;
-    const bool move = mt > st.m + 8.0f;  // both lanes of a row decide alike
+    const bool move = mt - st.m > 8.0f;  // both lanes of a row decide alike
     __builtin_amdgcn_sched_barrier(0);
     if (__any(move)) {
         const float m = move ? mt : st.m;
@@ -128,16 +132,26 @@ __device__ __forceinline__ void score_state(f32x16_t (&s)[NT], RowState<HD>& st,
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) st.o[dt] *= alpha;
     }
+    float mul = k.sl;
+    const bool far = __builtin_fabsf(st.m) >= kFarMax;
+    if (__any(far)) {
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kt][r] = far ? s[kt][r] * mul : s[kt][r];
+        mul = far ? 1.0f : mul;
+    }
     __builtin_amdgcn_sched_barrier(0);
+    return mul;
 }
 template <int HD, int NT>
-__device__ __forceinline__ void score_exps(f32x16_t (&s)[NT], RowState<HD>& st, const ScoreConsts& k) {
+__device__ __forceinline__ void score_exps(f32x16_t (&s)[NT], RowState<HD>& st, float mul) {
     float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], k.sl, -st.m));
+            s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], mul, -st.m));
             ls[r & 3] += s[kt][r];
         }
     st.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
@@ -516,8 +530,8 @@ __global__ void __launch_bounds__(256) __attribute__((
             const bool more = i + 4 < tiles;
             if (more) load_own(own_k, kp, kstride, i + 4);
             const int diag = k0 + i * kNarrowKeys + 4 * h - klast;
-            score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
-            score_exps<HD, NT>(s, st, consts);
+            const float mul = score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
+            score_exps<HD, NT>(s, st, mul);
             if (more) wait_loads<kNarrowLoads>();  // V(i) has landed; K(i + 4) may fly
             else wait_loads<0>();
             if constexpr (decltype(masked)::value) accumulate_seen(std::integral_constant<bool, true>{}, s, vt0, diag);
@@ -568,13 +582,13 @@ __global__ void __launch_bounds__(256) __attribute__((
 #pragma unroll
                     for (int kt = 0; kt < NT; ++kt)
                         nxt[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], nxt[kt]);
-                score_state<MODE, HD, NT, false>(cur, st, consts, 0);
+                const float mul = score_state<MODE, HD, NT, false>(cur, st, consts, 0);
 #pragma unroll
                 for (int c = kFirst; c < kC; ++c)
 #pragma unroll
                     for (int kt = 0; kt < NT; ++kt)
                         nxt[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], nxt[kt]);
-                score_exps<HD, NT>(cur, st, consts);
+                score_exps<HD, NT>(cur, st, mul);
 #pragma unroll
                 for (int g = 0; g < 2 * NT; ++g) {
                     const bf16x8_t pf = prob_frag<BF>(cur[g >> 1], g & 1);
@@ -588,8 +602,8 @@ __global__ void __launch_bounds__(256) __attribute__((
             auto finish = [&](auto masked, f32x16_t (&s)[NT], int i) __attribute__((always_inline)) {
                 sync(i + 1);
                 const int diag = k0 + i * NK + off + 4 * h - klast;
-                score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
-                score_exps<HD, NT>(s, st, consts);
+                const float mul = score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
+                score_exps<HD, NT>(s, st, mul);
                 if constexpr (decltype(masked)::value)
                     accumulate_seen(std::integral_constant<bool, false>{}, s, k_tile(i) + kV, diag);
                 else accumulate(std::integral_constant<bool, false>{}, s, k_tile(i) + kV);

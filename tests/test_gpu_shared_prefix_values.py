@@ -68,3 +68,69 @@ def test_infinities_that_tokens_see(cuda, case, cap):
     assert torch.equal(got[1], clean[1])
     assert torch.equal(got[0].isnan(), want.isnan())
     assert torch.equal(got[0].nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+def _definition(q, pk, pv, sk, sv, lens, scale):
+    """out, sum p |v| and sum |v| [B, T, Hq, D], lse [B, Hq, T], in 64 bits."""
+    b, t, hq, d = q.shape
+    out, size, total = (torch.zeros(b, t, hq, d, dtype=torch.float64, device=q.device) for _ in range(3))
+    lse = torch.zeros(b, hq, t, dtype=torch.float64, device=q.device)
+    group, own = hq // pk.shape[1], torch.arange(sk.shape[1], device=q.device)
+    for i in range(b):
+        hidden = own[None] > (int(lens[i]) - t + torch.arange(t, device=q.device))[:, None]         # [t, own]
+        hidden = torch.cat([torch.zeros(t, pk.shape[0], dtype=torch.bool, device=q.device), hidden], 1)
+        for h in range(hq):
+            k, v = (torch.cat([x[:, h // group], y[i, :, h // group]]).double() for x, y in ((pk, sk), (pv, sv)))
+            s = (q[i, :, h].double() @ k.t().contiguous() * scale).masked_fill(hidden, -math.inf)
+            z = torch.logsumexp(s, -1)
+            p = torch.exp(s - s.amax(-1, keepdim=True))  # z may be too large to hold the sum
+            p = p / p.sum(-1, keepdim=True)
+            out[i, :, h], size[i, :, h], total[i, :, h], lse[i, h] = p @ v, p @ v.abs(), (~hidden).double() @ v.abs(), z
+    return out, size, total, lse
+
+
+@pytest.mark.parametrize("case", ROWS, ids=lambda c: "-".join(map(str, c)))
+def test_scores_of_any_magnitude(cuda, case):
+    """Scores of both signs, from 1 to 2^106 (2^30 in FP16), the sizes and signs side
+    by side in the rows: each row is the mean over the keys of its largest score, or
+    an ordinary softmax.  Keys are whole multiples of one vector, so that scores are exact
+    but for the scale.  An output is off by the rounding of P (half a step u of sum p |v|,
+    and in FP16 2^-25 of each |v| below the normal range), of itself, and 2e-5 for the
+    exponents; lse by 2e-5 and eight roundings of 2^-24."""
+    from sfu_repro import fa4_runtime
+
+    q, pk, pv, sk, sv, lens = _operands(case, cuda, seed=3)
+    bf = q.dtype == torch.bfloat16
+    sizes = [2.0 ** n for n in ((-4, 0, 14, 18, 30, 60, 100) if bf else (-12, -9, 0, 5, 10, 15))]
+    step = 1.0 if bf else 512.0
+    b, t, hq, d = q.shape
+    signed = torch.tensor([sign * x for x in sizes for sign in (1.0, -1.0)], device=cuda)
+    rows = torch.arange(b * t * hq, device=cuda).view(b, t, hq) * 5 + 3  # every size meets every row of a tile
+    q = signed[rows % len(signed)][..., None].expand(q.shape).to(q.dtype).contiguous()
+    for k in (pk, sk):
+        g = torch.Generator(device=cuda).manual_seed(k.dim())
+        k.copy_((torch.randint(1, 8, k.shape[:-1], generator=g, device=cuda) * step)[..., None].expand(k.shape))
+    scale = float(torch.tensor(1 / math.sqrt(d), dtype=torch.float32))
+    out, lse = fa4_runtime.flash_attn_shared_prefix(q, pk, pv, sk, sv, lens, softmax_scale=scale)
+    want, size, total, want_lse = _definition(q, pk, pv, sk, sv, lens, scale)
+    u = torch.finfo(q.dtype).eps / 2
+    tol = (u + 2e-5) * size + u * (1 + u) * want.abs()
+    if not bf:
+        tol = tol + 2.0 ** -25 * (total + 1)
+    off = (out.double() - want).abs()
+    assert bool((off <= tol).all()), float((off / tol).nan_to_num(math.inf).max())
+    assert bool(((lse.double() - want_lse).abs() <= 2e-5 + 2.0 ** -21 * want_lse.abs()).all())
+
+
+def test_a_row_whose_scores_lie_below_all_others(cuda):
+    """One key with a score of -1e31: the row is its value."""
+    from sfu_repro import fa4_runtime
+
+    for d in (64, 128):
+        q = torch.full((2, 1, 4, d), -1e15, dtype=torch.bfloat16, device=cuda)
+        k = torch.full((2, 1, 2, d), 1e15, dtype=torch.bfloat16, device=cuda)
+        v = torch.randn(2, 1, 2, d, device=cuda).to(torch.bfloat16)
+        none = k[0, :0]
+        lens = torch.ones(2, dtype=torch.int32, device=cuda)
+        out, lse = fa4_runtime.flash_attn_shared_prefix(q, none, none, k, v, lens)
+        assert torch.equal(out[:, 0], v[:, 0].repeat_interleave(2, 1)) and bool(lse.isfinite().all())
