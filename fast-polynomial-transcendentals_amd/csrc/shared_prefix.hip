@@ -100,9 +100,11 @@ struct RowState {
 
 // One tile of NT 32-key accumulators of scores, to become probabilities 2^(s f - m)
 // with the factor f that score_state returns.  O and l are rescaled if the tile raises
-// the maximum by more than 8 (log2), which keeps the exponents at 8 and below.  MASKED: keys k0 + 32 kt + 8(r/4) + 4h + r%4
+// the maximum by more than 8 (log2).  BF16 probabilities have FP32's range, and m is a
+// maximum; FP16's end at 2^-24, so m lies 7 below one, which keeps what is 2^-31 of the
+// largest, and the exponents at 15 and below.  MASKED: keys k0 + 32 kt + 8(r/4) + 4h + r%4
 // past klast count nothing; diag = k0 + 4h - klast.
-template <int MODE, int HD, int NT, bool MASKED>
+template <int MODE, int HD, bool BF, int NT, bool MASKED>
 __device__ __forceinline__ float score_state(f32x16_t (&s)[NT], RowState<HD>& st, const ScoreConsts& k, int diag) {
     if constexpr (!attn_is_plain_softmax(MODE)) {
 #pragma unroll
@@ -122,10 +124,11 @@ __device__ __forceinline__ float score_state(f32x16_t (&s)[NT], RowState<HD>& st
             mx[r & 3] = __builtin_fmaxf(mx[r & 3], s[kt][r]);
         }
     const float mt = half_max(__builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]))) * k.sl;
-    const bool move = mt - st.m > 8.0f;  // both lanes of a row decide alike
+    constexpr float kBelow = BF ? 0.0f : 7.0f;
+    const bool move = mt - st.m > 8.0f + kBelow;  // both lanes of a row decide alike
     __builtin_amdgcn_sched_barrier(0);
     if (__any(move)) {
-        const float m = move ? mt : st.m;
+        const float m = move ? mt - kBelow : st.m;
         const float alpha = __builtin_amdgcn_exp2f(st.m - m);
         st.m = m;
         st.l *= alpha;
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(256) __attribute__((
             const bool more = i + 4 < tiles;
             if (more) load_own(own_k, kp, kstride, i + 4);
             const int diag = k0 + i * kNarrowKeys + 4 * h - klast;
-            const float mul = score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
+            const float mul = score_state<MODE, HD, BF, NT, decltype(masked)::value>(s, st, consts, diag);
             score_exps<HD, NT>(s, st, mul);
             if (more) wait_loads<kNarrowLoads>();  // V(i) has landed; K(i + 4) may fly
             else wait_loads<0>();
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(256) __attribute__((
 #pragma unroll
                     for (int kt = 0; kt < NT; ++kt)
                         nxt[kt] = mfma<BF>(reader.row_frag(kt0 + lds_row<HD>(kt * 32), c), qf[c], nxt[kt]);
-                const float mul = score_state<MODE, HD, NT, false>(cur, st, consts, 0);
+                const float mul = score_state<MODE, HD, BF, NT, false>(cur, st, consts, 0);
 #pragma unroll
                 for (int c = kFirst; c < kC; ++c)
 #pragma unroll
@@ -602,7 +605,7 @@ __global__ void __launch_bounds__(256) __attribute__((
             auto finish = [&](auto masked, f32x16_t (&s)[NT], int i) __attribute__((always_inline)) {
                 sync(i + 1);
                 const int diag = k0 + i * NK + off + 4 * h - klast;
-                const float mul = score_state<MODE, HD, NT, decltype(masked)::value>(s, st, consts, diag);
+                const float mul = score_state<MODE, HD, BF, NT, decltype(masked)::value>(s, st, consts, diag);
                 score_exps<HD, NT>(s, st, mul);
                 if constexpr (decltype(masked)::value)
                     accumulate_seen(std::integral_constant<bool, false>{}, s, k_tile(i) + kV, diag);

@@ -134,3 +134,27 @@ def test_a_row_whose_scores_lie_below_all_others(cuda):
         lens = torch.ones(2, dtype=torch.int32, device=cuda)
         out, lse = fa4_runtime.flash_attn_shared_prefix(q, none, none, k, v, lens)
         assert torch.equal(out[:, 0], v[:, 0].repeat_interleave(2, 1)) and bool(lse.isfinite().all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch", [1, 12, 33])
+def test_many_small_probabilities(cuda, batch, d):
+    """FP16: in every 32 keys 31 at 2^-26.5 of one whose value is zero.  Probabilities
+    below the normal range are off by 2^-25 in units of at most 2^-7 of the largest, so an
+    output by 2^-32 of sum |v| over the largest ones' number."""
+    from sfu_repro import fa4_runtime
+
+    q = torch.ones(batch, 1, 4, d, dtype=torch.float16, device=cuda)
+    k = torch.full((9600, 1, d), -1.625, dtype=torch.float16, device=cuda)
+    v = torch.randint(20000, 60000, (9600, 1, d), device=cuda).to(torch.float16)
+    k[5::32], v[5::32] = 0, 0
+    none = torch.zeros(batch, 0, 1, d, dtype=torch.float16, device=cuda)
+    lens = torch.zeros(batch, dtype=torch.int32, device=cuda)
+    scale = 18.375 / (1.625 * d)
+    out, _ = fa4_runtime.flash_attn_shared_prefix(q, k, v, none, none, lens, softmax_scale=scale)
+    want, size, total, _ = _definition(q, k, v, none, none, lens, scale)
+    u = 2.0 ** -11
+    tol = (u + 2e-5) * size + u * (1 + u) * want + 2.0 ** -32 * total / 300 + 2.0 ** -25
+    assert float(want.min()) > 0.01 and float((tol / want).max()) < 0.05
+    off = (out.double() - want).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
