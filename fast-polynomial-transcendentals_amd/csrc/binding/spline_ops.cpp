@@ -664,6 +664,14 @@ std::vector<at::Tensor> polynomial_sincos_f32(at::Tensor angles, std::vector<dou
 // query / key heads ahead of the attention: norm and rotation by positions
 // ---------------------------------------------------------------------------
 
+// Refuses operands with a tangent (forward-mode derivatives), which do not require
+// gradients and would lose it.
+void refuse_tangents(std::initializer_list<const at::Tensor*> operands, const char* what) {
+    for (const at::Tensor* t : operands)
+        TORCH_CHECK(t == nullptr || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
+                    " has no forward-mode derivative");
+}
+
 // The operand as the kernels take it: rows of a contiguous head dimension,
 // pointer and strides whole multiples of four elements, or a copy of it.
 at::Tensor head_rows(const at::Tensor& t) {
@@ -798,6 +806,7 @@ std::vector<at::Tensor> heads_forward(const at::Tensor& q, const at::Tensor& k, 
                                       const c10::optional<at::Tensor>& positions,
                                       const c10::optional<at::Tensor>& frequency_axes, double eps, bool interleaved,
                                       bool norm) {
+    refuse_tangents({&q, &k, qw ? &*qw : nullptr, kw ? &*kw : nullptr}, norm ? "qk_norm_rope" : "rope_axes");
     check_head_pair(q, k, "q", "k", 1, kTokensFirst);
     c10::OptionalDeviceGuard guard(q.device());
     const int64_t b = q.size(0), s = q.size(1), hq = q.size(2), hk = k.size(2), d = q.size(3);
@@ -843,6 +852,7 @@ std::vector<at::Tensor> rope_axes_fwd(at::Tensor q, at::Tensor k, at::Tensor pha
 // the rotation by the negative angles.
 std::vector<at::Tensor> rope_axes_bwd(at::Tensor dq_out, at::Tensor dk_out, at::Tensor phase_increments,
                                       at::Tensor positions, at::Tensor frequency_axes, bool interleaved) {
+    refuse_tangents({&dq_out, &dk_out}, "rope_axes");
     check_head_pair(dq_out, dk_out, "dq_out", "dk_out", 2, kHeadsFirst);
     c10::OptionalDeviceGuard guard(dq_out.device());
     const int64_t b = dq_out.size(0), s = dq_out.size(2), hq = dq_out.size(1), hk = dk_out.size(1), d = dq_out.size(3);
@@ -869,6 +879,8 @@ std::vector<c10::optional<at::Tensor>> qk_norm_rope_bwd(
     at::Tensor q, at::Tensor k, c10::optional<at::Tensor> q_weight, c10::optional<at::Tensor> k_weight,
     at::Tensor phase_increments, c10::optional<at::Tensor> positions, c10::optional<at::Tensor> frequency_axes,
     at::Tensor dq_out, at::Tensor dk_out, double eps, bool interleaved) {
+    refuse_tangents({&q, &k, q_weight ? &*q_weight : nullptr, k_weight ? &*k_weight : nullptr, &dq_out, &dk_out},
+                    "qk_norm_rope");
     check_head_pair(q, k, "q", "k", 1, kTokensFirst);
     check_head_pair(dq_out, dk_out, "dq_out", "dk_out", 2, kHeadsFirst);
     const int64_t b = q.size(0), s = q.size(1), hq = q.size(2), hk = k.size(2), d = q.size(3);
@@ -1016,6 +1028,7 @@ std::vector<at::Tensor> shared_prefix_attn_fwd(at::Tensor q, at::Tensor prefix_k
                                                  prefix_v.requires_grad() || suffix_k.requires_grad() ||
                                                  suffix_v.requires_grad()),
                 "flash_attn_shared_prefix has no backward; call it under torch.no_grad()");
+    refuse_tangents({&q, &prefix_k, &prefix_v, &suffix_k, &suffix_v}, "flash_attn_shared_prefix");
     const at::ScalarType dtype = q.scalar_type();
     TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
     TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "q must be float16 or bfloat16");

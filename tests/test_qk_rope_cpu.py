@@ -129,3 +129,37 @@ def test_reference_gradients(interleaved):
     w = torch.randn(16, generator=g, dtype=torch.float64, requires_grad=True)
     theta = torch.randn(1, 3, 1, 4, generator=g, dtype=torch.float64)
     assert torch.autograd.gradcheck(lambda a, b: ref.heads_out(a, b, theta, 1e-6, interleaved, True), (x, w))
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """A dual tensor does not require gradients; its tangent is not dropped."""
+    from torch.autograd import forward_ad
+    from sfu_repro import rope
+
+    q, inc = torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), rope.phase_increments(64)
+    w, pos = torch.ones(64), torch.zeros(2, 1, 2, dtype=torch.int64)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual, dual_w = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (q, w))
+        for args in ((dual, q, None, None), (q, dual, None, None), (q, q, dual_w, None), (q, q, w, dual_w)):
+            with pytest.raises(RuntimeError, match="qk_norm_rope has no forward-mode derivative"):
+                rope.qk_norm_rope(*args, inc)
+        for args in ((dual, q), (q, dual)):
+            with pytest.raises(RuntimeError, match="rope_axes has no forward-mode derivative"):
+                rope.rope_axes(*args, inc, pos, rope.axis_sections((16, 16)))
+
+
+def test_forward_mode_of_the_gradients_is_refused():
+    import spline_ops
+    from torch.autograd import forward_ad
+    from sfu_repro import rope
+
+    q, inc = torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), rope.phase_increments(64)
+    pos = torch.zeros(2, 1, 2, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for dq, dk in ((dual, q), (q, dual)):
+            with pytest.raises(RuntimeError, match="qk_norm_rope has no forward-mode derivative"):
+                spline_ops.qk_norm_rope_bwd(q, q, None, None, inc, None, None, dq, dk, 1e-6, True)
+            with pytest.raises(RuntimeError, match="rope_axes has no forward-mode derivative"):
+                spline_ops.rope_axes_bwd(dq, dk, inc, pos, rope.axis_sections((16, 16)), True)

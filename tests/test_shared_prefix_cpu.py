@@ -95,3 +95,18 @@ def test_limits(lib):
     for most in (dict(prefix=2 ** 30), dict(suffix=2 ** 30), dict(tokens=2 ** 14)):
         assert size(**one, **most) > 0
         assert size(**one, **{k: v + 1 for k, v in most.items()}) == -1
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor does not require gradients; its tangent is not dropped."""
+    from torch.autograd import forward_ad
+    from sfu_repro import fa4_runtime
+
+    q, k = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    operands = [q, k, k, k[None], k[None]]
+    with torch.no_grad(), forward_ad.dual_level():
+        for i, t in enumerate(operands):
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="flash_attn_shared_prefix has no forward-mode derivative"):
+                fa4_runtime.flash_attn_shared_prefix(*operands[:i], dual, *operands[i + 1:],
+                                                     torch.zeros(1, dtype=torch.int32))
