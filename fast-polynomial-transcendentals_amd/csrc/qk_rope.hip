@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(kBlock, 4) qk_rope_kernel(QkParams p) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 cs[i] *= mine[i];
-                sn[i] *= INTER ? mine[i ^ 1] : other[i];
+                // nothing is added where nothing turns: a weight there may be infinite
+                sn[i] = part.rot ? sn[i] * (INTER ? mine[i ^ 1] : other[i]) : 0.0f;
             }
         }
         auto turn = [&](int h, const Words<V> (&now)[HPT]) __attribute__((always_inline)) {
