@@ -897,10 +897,9 @@ std::vector<c10::optional<at::Tensor>> qk_norm_rope_bwd(
     check_weight_pair(qw, kw);
     const at::Tensor qr = head_rows(q), kr = head_rows(k), dqr = head_rows(dq_out), dkr = head_rows(dk_out);
     at::Tensor dq = at::empty({b, s, hq, d}, q.options()), dk = at::empty({b, s, hk, d}, k.options());
-    const bool empty = b == 0 || s == 0;  // a sum over no rows
     auto weight_grad = [&](const at::Tensor& w) -> c10::optional<at::Tensor> {
         if (!w.defined()) return c10::nullopt;
-        return empty ? at::zeros({d}, w.options()) : at::empty({d}, w.options());
+        return at::empty({d}, w.options());
     };
     const c10::optional<at::Tensor> dqw = weight_grad(qw), dkw = weight_grad(kw);
     at::Tensor ws;

@@ -476,7 +476,7 @@ struct DwSide {
 template <bool BF>
 __global__ void __launch_bounds__(1024) qk_dw_kernel(DwSide q, DwSide k, int head_dim, bool w32) {
     const DwSide s = blockIdx.y ? k : q;
-    if (s.part == nullptr) return;
+    if (s.out == nullptr) return;
     const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
     float t = 0.0f;
     if (e < head_dim) {
@@ -519,6 +519,7 @@ int make_params(const spline_hip_qk_rope* a, bool norm, bool backward, QkParams&
     if (d <= 0 || d > 256 || d % 8 != 0 || r < 0 || r > d || r % 8 != 0) return hipErrorInvalidValue;
     if (a->q_heads > kMaxHeads || a->k_heads > kMaxHeads) return hipErrorInvalidValue;
     V = 0;
+    p = QkParams{};
     if (a->batch == 0 || a->sequence_length == 0 || a->q_heads + a->k_heads == 0) return hipSuccess;
     if (a->batch > 0x7fffffff / a->sequence_length) return hipErrorInvalidValue;
     if (r > 0 && (!a->phase_increments || !aligned_to(a->phase_increments, 4))) return hipErrorInvalidValue;
@@ -529,7 +530,6 @@ int make_params(const spline_hip_qk_rope* a, bool norm, bool backward, QkParams&
     const int wa = a->weight_f32 ? 4 : 2;
     if (!aligned_to(a->q_weight, wa) || !aligned_to(a->k_weight, wa)) return hipErrorInvalidValue;
 
-    p = QkParams{};
     V = a->interleaved || r % 16 == 0 ? 8 : 4;  // a vector holds pairs, or one half of its pairs
     auto side = [&](QkSide& s, int64_t heads, const void* x, void* y, const void* w, const void* dy,
                     const int64_t (&xs)[3], const int64_t (&ys)[3], const int64_t (&dys)[3]) {
@@ -622,7 +622,19 @@ constexpr int kBwdBlocks = 2048;
 
 template <bool BF>
 int backward(const spline_hip_qk_rope* a, QkParams& p, int V, hipStream_t stream) {
-    if (V == 0) return hipSuccess;
+    // a side without rows has no partial rows either: its weight's gradient is zero
+    const bool qw = a->q_weight != nullptr, kw = a->k_weight != nullptr;
+    if ((qw && (!a->dq_weight || !a->dw_workspace)) || (kw && (!a->dk_weight || !a->dw_workspace)))
+        return hipErrorInvalidValue;
+    auto add_rows = [&]() -> int {
+        if (!qw && !kw) return hipSuccess;
+        hipLaunchKernelGGL((qk_dw_kernel<BF>), dim3((unsigned)(a->head_dim + 15) / 16, 2), dim3(1024), 0, stream,
+                           DwSide{p.q.dw, qw ? a->dq_weight : nullptr, p.q.dw ? p.q.blocks : 0},
+                           DwSide{p.k.dw, kw ? a->dk_weight : nullptr, p.k.dw ? p.k.blocks : 0}, (int)a->head_dim,
+                           a->weight_f32 != 0);
+        return hipGetLastError();
+    };
+    if (V == 0) return add_rows();
     const int64_t chunks = (p.tokens + (int64_t)p.rows - 1) / p.rows;
     cut_heads(p, chunks, 12);
     const int64_t items = chunks * (p.q.splits + p.k.splits);
@@ -632,8 +644,6 @@ int backward(const spline_hip_qk_rope* a, QkParams& p, int V, hipStream_t stream
     float* ws = a->dw_workspace;
     if (p.q.w) p.q.dw = ws, ws += (int64_t)p.q.blocks * p.head_dim;
     if (p.k.w) p.k.dw = ws;
-    if ((p.q.w && (!a->dq_weight || !a->dw_workspace)) || (p.k.w && (!a->dk_weight || !a->dw_workspace)))
-        return hipErrorInvalidValue;
     const dim3 grid((unsigned)(p.q.blocks + p.k.blocks));
     const bool inter = a->interleaved != 0;
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, stream, p); };
@@ -643,12 +653,8 @@ int backward(const spline_hip_qk_rope* a, QkParams& p, int V, hipStream_t stream
         else inter ? go(qk_rope_bwd_kernel<BF, 4, true, NT, 2>) : go(qk_rope_bwd_kernel<BF, 4, false, NT, 2>);
     };
     p.nt ? pick(std::integral_constant<bool, true>{}) : pick(std::integral_constant<bool, false>{});
-    int rc = hipGetLastError();
-    if (rc != hipSuccess || (!p.q.w && !p.k.w)) return rc;
-    hipLaunchKernelGGL((qk_dw_kernel<BF>), dim3((p.head_dim + 15) / 16, 2), dim3(1024), 0, stream,
-                       DwSide{p.q.dw, a->dq_weight, p.q.blocks}, DwSide{p.k.dw, a->dk_weight, p.k.blocks},
-                       p.head_dim, p.w32);
-    return hipGetLastError();
+    const int rc = hipGetLastError();
+    return rc != hipSuccess ? rc : add_rows();
 }
 
 template <bool BF>

@@ -532,7 +532,8 @@ SPLINE_HIP_ROPE_APPLY_LAUNCHERS(SPLINE_HIP_DECLARE_ROPE_APPLY)
  * launch_qk_norm_rope_bwd_*: q_out and k_out receive the gradients at q and k
  * (strides q_out_strides, k_out_strides), dq_out and dk_out hold those at the
  * forward's outputs, dq_weight and dk_weight receive those at the weights that
- * are not null (of the weights' type; summed in FP32 in a fixed order).
+ * are not null (of the weights' type; summed in FP32 in a fixed order; zeros
+ * where there is no row).
  * dw_workspace: spline_hip_qk_norm_rope_bwd_bytes(head_dim) bytes, with
  * weights only.  Calls that may overlap need workspaces of their own.
  *
