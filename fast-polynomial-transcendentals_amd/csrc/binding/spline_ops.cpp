@@ -9,6 +9,7 @@
 // (include/spline_ops_hip.h); nothing here computes on the host.
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 #include <torch/library.h>
 
@@ -1358,7 +1359,9 @@ struct GeluVariantFwd : public torch::autograd::Function<GeluVariantFwd> {
 // While a stream is captured into a graph, no gradient may flow into a leaf's
 // accumulation node of another stream: such a node, kept alive by an eager graph of the
 // same leaf, makes its stream wait for the captured one, which joins the capture
-// and never leaves it, and ending the capture then ends the process.
+// and need not leave it, and ending the capture then ends the process.  Only the nodes
+// that the running backward pass reaches count: with inputs given (autograd.grad) those on
+// the way to them, without all.
 void refuse_foreign_leaves(const at::Tensor& like, const char* what) {
     const auto stream = c10::hip::getCurrentHIPStream(like.device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -1366,17 +1369,25 @@ void refuse_foreign_leaves(const at::Tensor& like, const char* what) {
     if (status == hipStreamCaptureStatusNone) return;
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
+    const auto* plan = torch::autograd::get_current_graph_task_exec_info();
+    auto runs = [&](torch::autograd::Node* n) {
+        if (plan == nullptr || plan->empty()) return true;
+        const auto at = plan->find(n);
+        return at != plan->end() && at->second.should_execute();
+    };
     std::vector<torch::autograd::Node*> todo{node.get()};
     std::unordered_set<torch::autograd::Node*> seen{node.get()};
     while (!todo.empty()) {
         torch::autograd::Node* n = todo.back();
         todo.pop_back();
-        const auto at = n->stream();
-        TORCH_CHECK(n->name().find("AccumulateGrad") == std::string::npos || !at.has_value() || at->id() == stream.id(),
-                    what, ": cannot capture this backward pass: an eager graph of the same leaves is alive on another "
-                          "stream; delete it before the capture");
+        const auto at = n->stream();  // a default stream has the same id on every device
+        const bool same = !at.has_value() || (at->id() == stream.id() && at->device_index() == stream.device_index());
+        TORCH_CHECK(same || n->name().find("AccumulateGrad") == std::string::npos, what,
+                    ": cannot capture this backward pass: an eager graph of the same leaves is alive on another stream; "
+                    "delete it before the capture, or capture on its stream");
         for (const auto& edge : n->next_edges())
-            if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+            if (edge.function && runs(edge.function.get()) && seen.insert(edge.function.get()).second)
+                todo.push_back(edge.function.get());
     }
 }
 

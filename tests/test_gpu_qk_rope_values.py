@@ -1,5 +1,5 @@
 """Head norm at the ends of what its operands hold: weights that are no numbers,
-sides and batches without a row."""
+sides and batches without a row; and captured backward passes beside eager graphs."""
 
 import ctypes
 import math
@@ -62,3 +62,57 @@ def test_weight_gradients_without_rows(cuda, capi, empty, f32):
     rows = sizes["batch"] * sizes["sequence_length"]
     for got, heads in ((dqw, sizes["q_heads"]), (dkw, sizes["k_heads"])):  # x r = 1 for every row, dy = 1
         assert bool((got.double() - rows * heads).abs().max() <= rows * heads * 2.0 ** -20)
+
+
+def _captured_step(cuda):
+    from sfu_repro import rope
+
+    g = torch.Generator(device=cuda).manual_seed(31)
+    q, k = (torch.randn(2, 30, h, 64, generator=g, device=cuda).half().requires_grad_(True) for h in (4, 2))
+    w = torch.ones(64, device=cuda).requires_grad_(True)
+    inc = rope.phase_increments(64).to(cuda)
+    d = [torch.randn(2, h, 30, 64, generator=g, device=cuda).half() for h in (4, 2)]
+    return q, k, w, d, lambda *leaves: rope.qk_norm_rope(leaves[0], leaves[1], leaves[2], leaves[2], inc)
+
+
+def test_capture_of_gradients_that_other_leaves_do_not_take(cuda):
+    """An eager graph of leaves that the captured pass does not ask for is no
+    reason to refuse it: of a subset of them, or of activations alone."""
+    q, k, w, d, call = _captured_step(cuda)
+    alive = call(q, k, torch.ones_like(w))  # q and k, not w
+    want = torch.autograd.grad(call(q, k, w), w, d)[0]
+    scaled = (q.detach() * 0.5).requires_grad_(True)
+    want_q = torch.autograd.grad(call(scaled, k, w), scaled, d)[0]
+    del scaled
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = torch.autograd.grad(call(q, k, w), w, d)[0]
+        x = q * 0.5
+        held_q = torch.autograd.grad(call(x, k, w), x, d)[0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want) and torch.equal(held_q, want_q)
+    with pytest.raises(RuntimeError, match="capture on its stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(call(q, k, w), [w, q], d)
+    del alive
+
+
+def test_capture_on_the_stream_of_the_eager_graph(cuda):
+    q, k, w, d, call = _captured_step(cuda)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        alive = call(q, k, w)
+        want = torch.autograd.grad(alive, [q, k, w], d, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        held = torch.autograd.grad(call(q, k, w), [q, k, w], d)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+    del alive
