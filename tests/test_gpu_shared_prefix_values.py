@@ -6,6 +6,8 @@ import math
 import pytest
 import torch
 
+from shared_prefix_reference import definition
+
 pytestmark = pytest.mark.gpu
 
 
@@ -70,25 +72,6 @@ def test_infinities_that_tokens_see(cuda, case, cap):
     assert torch.equal(got[0].nan_to_num(7.0), want.nan_to_num(7.0))
 
 
-def _definition(q, pk, pv, sk, sv, lens, scale):
-    """out, sum p |v| and sum |v| [B, T, Hq, D], lse [B, Hq, T], in 64 bits."""
-    b, t, hq, d = q.shape
-    out, size, total = (torch.zeros(b, t, hq, d, dtype=torch.float64, device=q.device) for _ in range(3))
-    lse = torch.zeros(b, hq, t, dtype=torch.float64, device=q.device)
-    group, own = hq // pk.shape[1], torch.arange(sk.shape[1], device=q.device)
-    for i in range(b):
-        hidden = own[None] > (int(lens[i]) - t + torch.arange(t, device=q.device))[:, None]         # [t, own]
-        hidden = torch.cat([torch.zeros(t, pk.shape[0], dtype=torch.bool, device=q.device), hidden], 1)
-        for h in range(hq):
-            k, v = (torch.cat([x[:, h // group], y[i, :, h // group]]).double() for x, y in ((pk, sk), (pv, sv)))
-            s = (q[i, :, h].double() @ k.t().contiguous() * scale).masked_fill(hidden, -math.inf)
-            z = torch.logsumexp(s, -1)
-            p = torch.exp(s - s.amax(-1, keepdim=True))  # z may be too large to hold the sum
-            p = p / p.sum(-1, keepdim=True)
-            out[i, :, h], size[i, :, h], total[i, :, h], lse[i, h] = p @ v, p @ v.abs(), (~hidden).double() @ v.abs(), z
-    return out, size, total, lse
-
-
 @pytest.mark.parametrize("case", ROWS, ids=lambda c: "-".join(map(str, c)))
 def test_scores_of_any_magnitude(cuda, case):
     """Scores of both signs, from 1 to 2^106 (2^30 in FP16), the sizes and signs side
@@ -112,7 +95,7 @@ def test_scores_of_any_magnitude(cuda, case):
         k.copy_((torch.randint(1, 8, k.shape[:-1], generator=g, device=cuda) * step)[..., None].expand(k.shape))
     scale = float(torch.tensor(1 / math.sqrt(d), dtype=torch.float32))
     out, lse = fa4_runtime.flash_attn_shared_prefix(q, pk, pv, sk, sv, lens, softmax_scale=scale)
-    want, size, total, want_lse = _definition(q, pk, pv, sk, sv, lens, scale)
+    want, size, total, want_lse = definition(q, pk, pv, sk, sv, lens, scale)
     u = torch.finfo(q.dtype).eps / 2
     tol = (u + 2e-5) * size + u * (1 + u) * want.abs()
     if not bf:
@@ -152,7 +135,7 @@ def test_many_small_probabilities(cuda, batch, d):
     lens = torch.zeros(batch, dtype=torch.int32, device=cuda)
     scale = 18.375 / (1.625 * d)
     out, _ = fa4_runtime.flash_attn_shared_prefix(q, k, v, none, none, lens, softmax_scale=scale)
-    want, size, total, _ = _definition(q, k, v, none, none, lens, scale)
+    want, size, total, _ = definition(q, k, v, none, none, lens, scale)
     u = 2.0 ** -11
     tol = (u + 2e-5) * size + u * (1 + u) * want + 2.0 ** -32 * total / 300 + 2.0 ** -25
     assert float(want.min()) > 0.01 and float((tol / want).max()) < 0.05
