@@ -25,9 +25,14 @@
 // a second launch adds the partial rows.  Every order of addition is fixed.
 //
 // What bounds it: memory, 4 bytes an element forward and 6 backward.  Measured at
-// 4 x 4096 tokens, 32 + 8 heads of 128 in BF16: forward 62.7 us, 5.4 TB/s, backward
-// 97.7 us, 5.2 TB/s (a copy of as much: 6.6 TB/s); the rotation alone by three axes,
-// 2 x 8190 tokens: 61.4 us, 5.5 TB/s.  Few tokens take a launch, 4 us.
+// 4 x 4096 tokens, 32 + 8 heads of 128 in BF16, each by itself over inputs in turn:
+// forward 62.7 to 64.2 us, 5.3 TB/s, backward 97.7 to 99.0 us for both launches, 5.1 TB/s (a
+// copy of as much: 6.6 TB/s).  Behind the forward, which leaves part of x in the MALL, the
+// backward kernel takes 84 to 89 us and the sum of the partial rows 4 to 5, so that
+// one pass of both takes 153.  The rotation alone by three axes, 2 x 8190 tokens: 61.4 us,
+// 5.5 TB/s.  Few tokens take a launch, 4 us.  Rows of 80 elements with 40 rotated, by halves,
+// take 4-element vectors and 20 of 32 lanes: 11.8 us forward for 3003 tokens of 32
+// heads in FP16, where a copy takes 4.7, and 19.2 backward.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>

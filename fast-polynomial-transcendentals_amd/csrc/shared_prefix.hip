@@ -31,6 +31,11 @@
 // in the first launch); 64 behind 32768 with caches of up to 2048 keys, heads of 128, 95 us
 // (403 MB, 35 GFLOP); 16 x 100 tokens behind 8192 247 us, 900 TFLOP/s; 8 sequences
 // behind 1024, caches of 256, 11 us.
+//
+// The host does not know the caches' lengths: parts, workspace and launch go by what
+// they are allocated for, and a part without keys still writes its rows.  64 sequences
+// with 500 to 2000 keys behind 4096: 71 us in caches of 2048, 90 in 8192, 176 in 32768
+// (behind 32768 keys 96, 131, 541); views of the longest length keep it at 69 and 96.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -436,8 +441,10 @@ __global__ void __launch_bounds__(256) __attribute__((
     };
     // O^T += V^T P^T, three fragments (two reads each) ahead.  One rounding of P
     // costs as much as the result's own (their sum is 1.4 times it).  Narrow blocks
-    // wait for memory, so they add the product with what it left (exact); in wide ones it
-    // would be a quarter of the time.
+    // wait for memory, so they add the product with what it left (exact).  Wide ones round once,
+    // as the attention forward does; the same there took 341 us against 247 with
+    // 16 x 100 tokens behind 8192 keys, 72 against 59 with 64 decoding behind 32768, 77
+    // against 60 with 128 behind 16384, 101 against 98 with caches of 2048 besides.
     auto accumulate = [&](auto exact, const auto& s, const unsigned char* vt0) __attribute__((always_inline)) {
         constexpr bool EXACT = decltype(exact)::value;
         constexpr int NT = sizeof(s) / sizeof(f32x16_t), kN = 2 * NT * kD;

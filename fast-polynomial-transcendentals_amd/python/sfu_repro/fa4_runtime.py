@@ -406,11 +406,12 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
     sees no key gets zeros and an lse of -inf.
 
     Any strides over a contiguous head dimension in whole multiples of 8
-    elements (nothing is copied); float16 or bfloat16; head_dim 64 or 128.  The
-    score program is that of :func:`flash_attn_fwd`'s arguments; built are the
-    hardware softmax, the hardware softcap (``softcap``) and, for bfloat16, the D4
-    softcap (``score_mod``).  There is no backward: operands that require
-    gradients are refused.
+    elements (nothing is copied); float16 or bfloat16; head_dim 64 or 128.  Time and
+    workspace go by L, not by the lengths: pass views (``suffix_k[:, :n]``) of caches
+    that hold much more than the longest length in use.  The score program is that
+    of :func:`flash_attn_fwd`'s arguments; built are the hardware softmax, the
+    hardware softcap (``softcap``) and, for bfloat16, the D4 softcap (``score_mod``).
+    There is no backward: operands that require gradients are refused.
     """
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
     if program:

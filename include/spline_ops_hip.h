@@ -745,10 +745,15 @@ int launch_flash_attention_bwd_strided_bf16_noalloc(void* dq, void* dk, void* dv
  * own caches, suffix_k and suffix_v [B, L, Hkv, D], whose lens[b] first rows are
  * valid, the last T of them the new tokens': token t sees suffix keys
  * 0 .. lens[b] - T + t.  lens are held to 0 .. L; rows that a token does not
- * see may hold anything.  At most 2^30 keys and 2^14 tokens.  out [B, T, Hq, D] contiguous, and lse, float [B, Hq, T] or
- * null: ln of the row's sum of exp(s').  A row that sees no key is zero with
- * lse -inf.  D 64 or 128, Hq a multiple of Hkv, 16-bit (P is rounded to the
- * operands' type ahead of P V; sums are FP32).  mode: 0 softmax of q.k scale,
+ * see may hold anything.  An infinity or a NaN in a value that a token sees is
+ * one in its result.  The cost and the workspace go by L, not by lens: pass the
+ * longest length in use as L where the caches hold more.  At most 2^30 keys and
+ * 2^14 tokens.  out [B, T, Hq, D] contiguous, and lse, float [B, Hq, T] or null:
+ * ln of the row's sum of exp(s').  A row that sees no key is zero with lse -inf.
+ * D 64 or 128, Hq a multiple of Hkv, 16-bit.  Sums are FP32; ahead of P V the
+ * probabilities take the operands' type, in two terms where at most 32 rows meet
+ * the prefix (B T Hq / Hkv) or a cache (T Hq / Hkv), rounded once beyond that (as
+ * in launch_flash_attention_fwd_bf16).  mode: 0 softmax of q.k scale,
  * 3 of cap tanh(q.k scale / cap), 4 (BF16 operands) of the same with the D4
  * BF16 tanh program, as in launch_flash_attention_fwd_bf16.
  * Pointers 16-byte aligned, strides (elements) multiples of 8, head dimension
