@@ -677,19 +677,27 @@ __global__ void __launch_bounds__(256) __attribute__((
     }
 }
 
+typedef int16_t i16x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
 // Elements 4 chunk .. of a row whose sum is a number while they are not: each
 // infinity and NaN that the row sees in V, from the parts that hold one (Inf for
 // infinities of one sign, NaN otherwise).  What the parts' products made of them depends on
 // rounding: an infinity times the zero that a probability was rounded to, or times
 // what that rounding left, is a NaN or has the other sign.  An element that sees none
-// (its finite values overflowed) keeps what it has.
+// (its finite values overflowed) keeps what it has.  Each row looks for itself: an infinity in
+// the prefix takes 0.34 ms with 64 sequences behind 32768 keys, 6 ms with 16 x 100 tokens
+// behind 8192; finite values pay a comparison.
 template <int HD, bool BF>
 __device__ __forceinline__ void look_up_values(const PrefixParams& p, int64_t row, int chunk, f32x4_t& o) {
     const int kvh = (int)(row / p.mrows), per = p.tokens * p.group;
     const int64_t mrow = row - kvh * p.mrows;
     const int b = (int)(mrow / per), r = (int)(mrow - (int64_t)b * per), t = r / p.group;
     const int r0 = r & ~(kWideRows - 1), nrows = per - r0 < kWideRows ? per - r0 : kWideRows;
-    uint32_t plus = 0, minus = 0, nan = 0;  // a bit for each element
+    // the largest halves as signed numbers, which positive ones are ordered as, and as
+    // unsigned ones, negative
+    i16x2_t top[2] = {};
+    u16x2_t low[2] = {};
     for (int i = 0; i < p.parts_p + p.parts_s; ++i) {
         const f32x4_t x =
             *reinterpret_cast<const f32x4_t*>(p.part_o + ((int64_t)i * p.rows + row) * HD + chunk * 4) * 0.0f;
@@ -709,24 +717,27 @@ __device__ __forceinline__ void look_up_values(const PrefixParams& p, int64_t ro
             v = p.sv + b * p.svs.b + kvh * p.svs.h;
             stride = p.svs.s;
         }
-        constexpr uint32_t kInf = BF ? 0x7f80 : 0x7c00;
-#pragma unroll 2
-        for (; k < kend; ++k) {
-            const uint2 w = *reinterpret_cast<const uint2*>(v + k * stride + chunk * 4);
+        for (; k < kend; k += 6) {  // six loads in flight; the last key again past the end
+            uint2 w[6];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t u = (e < 2 ? w.x : w.y) >> (e & 1) * 16 & 0xffffu;
-                plus |= (uint32_t)(u == kInf) << e;
-                minus |= (uint32_t)(u == (kInf | 0x8000u)) << e;
-                nan |= (uint32_t)((u & 0x7fffu) > kInf) << e;
+            for (int u = 0; u < 6; ++u)
+                w[u] = *reinterpret_cast<const uint2*>(v + (k + u < kend ? k + u : kend - 1) * stride + chunk * 4);
+#pragma unroll
+            for (int u = 0; u < 6; ++u) {
+                top[0] = __builtin_elementwise_max(top[0], __builtin_bit_cast(i16x2_t, w[u].x));
+                top[1] = __builtin_elementwise_max(top[1], __builtin_bit_cast(i16x2_t, w[u].y));
+                low[0] = __builtin_elementwise_max(low[0], __builtin_bit_cast(u16x2_t, w[u].x));
+                low[1] = __builtin_elementwise_max(low[1], __builtin_bit_cast(u16x2_t, w[u].y));
             }
         }
     }
-    nan |= plus & minus;
+    constexpr int kInf = BF ? 0x7f80 : 0x7c00;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if ((plus | minus | nan) >> e & 1)
-            o[e] = as_f32(nan >> e & 1 ? 0x7fc00000u : plus >> e & 1 ? 0x7f800000u : 0xff800000u);
+    for (int e = 0; e < 4; ++e) {
+        const int plus = (int)top[e >> 1][e & 1] - kInf, minus = (int)low[e >> 1][e & 1] - (kInf | 0x8000);
+        if (plus > 0 || minus > 0 || (plus == 0 && minus == 0)) o[e] = __builtin_nanf("");
+        else if (plus == 0 || minus == 0) o[e] = plus == 0 ? __builtin_inff() : -__builtin_inff();
+    }
 }
 
 // Joins the parts of each row.  HD / 4 lanes hold a row, and G groups of them
