@@ -403,7 +403,7 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
     ``suffix_lens[b]`` (int32, on the device, held to 0..L) rows are valid, the
     new tokens' own last.  Token t sees the prefix and suffix rows 0 ..
     ``suffix_lens[b] - T + t``; rows past them may hold anything.  A token that
-    sees no key gets zeros and an lse of -inf.
+    sees no key, or none with a score above -inf, gets zeros and an lse of -inf.
 
     Any strides over a contiguous head dimension in whole multiples of 8
     elements (nothing is copied); float16 or bfloat16; head_dim 64 or 128.  Time and

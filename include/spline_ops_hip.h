@@ -521,7 +521,7 @@ SPLINE_HIP_ROPE_APPLY_LAUNCHERS(SPLINE_HIP_DECLARE_ROPE_APPLY)
  * interleaved, else (i, i + rotary_dim / 2); elements from rotary_dim on are
  * not rotated.  t = 2 pi 2^-32 (position * phase_increments[i] mod 2^32), so a
  * position may be any integer.  All arithmetic is FP32 with one rounding of
- * each result.
+ * each result (elements of 2^64 and more overflow the mean of squares).
  *
  * head_dim a multiple of 8, at most 256; rotary_dim a multiple of 8 up to
  * head_dim; at most 65536 heads and 2^31 - 1 tokens.  Strides are in elements;
@@ -749,7 +749,8 @@ int launch_flash_attention_bwd_strided_bf16_noalloc(void* dq, void* dk, void* dv
  * one in its result.  The cost and the workspace go by L, not by lens: pass the
  * longest length in use as L where the caches hold more.  At most 2^30 keys and
  * 2^14 tokens.  out [B, T, Hq, D] contiguous, and lse, float [B, Hq, T] or null:
- * ln of the row's sum of exp(s').  A row that sees no key is zero with lse -inf.
+ * ln of the row's sum of exp(s').  A row that sees no key, or none with a score
+ * above -inf, is zero with lse -inf.
  * D 64 or 128, Hq a multiple of Hkv, 16-bit.  Sums are FP32; ahead of P V the
  * probabilities take the operands' type, in two terms where at most 32 rows meet
  * the prefix (B T Hq / Hkv) or a cache (T Hq / Hkv), rounded once beyond that (as

@@ -141,3 +141,17 @@ def test_many_small_probabilities(cuda, batch, d):
     assert float(want.min()) > 0.01 and float((tol / want).max()) < 0.05
     off = (out.double() - want).abs()
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("batch", [2, 20])
+def test_rows_whose_scores_are_all_minus_infinity(cuda, batch):
+    """As a row that sees no key: zeros and an lse of -inf; the other rows are untouched."""
+    from sfu_repro import fa4_runtime
+
+    q, pk, pv, sk, sv, lens = _operands(("bf16", batch, 1, 90, 40, 4, 2, 128), cuda, seed=5)
+    q, pk, sk = q.abs(), pk.abs(), sk.abs()
+    clean = fa4_runtime.flash_attn_shared_prefix(q, pk, pv, sk, sv, lens)
+    pk[:, 1], sk[:, :, 1] = -math.inf, -math.inf
+    out, lse = fa4_runtime.flash_attn_shared_prefix(q, pk, pv, sk, sv, lens)
+    assert not bool(out[:, :, 2:].any()) and bool((lse[:, 2:] == -math.inf).all())
+    assert torch.equal(out[:, :, :2], clean[0][:, :, :2]) and torch.equal(lse[:, :2], clean[1][:, :2])
