@@ -1104,6 +1104,215 @@ std::vector<at::Tensor> shared_prefix_attn_fwd(at::Tensor q, at::Tensor prefix_k
     return {out, lse};
 }
 
+// ---------------------------------------------------------------------------
+// a serving cache in pages of 4-bit numbers (spline_hip_fp4_cache):
+// cache uint8 [pages, 2, Hkv, bytes], table int32 [B, entries], lens int32 [B]
+// ---------------------------------------------------------------------------
+
+// Fills the cache's part of a call; table and lens are kept alive by the caller.
+void fill_fp4_cache(spline_hip_fp4_cache& c, const at::Tensor& cache, at::Tensor& table, at::Tensor& lens,
+                    int64_t head_dim) {
+    TORCH_CHECK(cache.is_cuda(), "cache must be a CUDA tensor");
+    TORCH_CHECK(cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.size(1) == 2 && cache.is_contiguous(),
+                "cache must be a contiguous uint8 tensor [pages, 2, kv_heads, bytes]");
+    TORCH_CHECK(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128, got ", head_dim);
+    const int64_t row = head_dim / 2 + head_dim / 32, bytes = cache.size(3);
+    TORCH_CHECK(bytes > 0 && bytes % (16 * row) == 0, "a page of head_dim ", head_dim, " holds whole multiples of 16 rows of ",
+                row, " bytes, got ", bytes, " bytes");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, "cache must be 16-byte aligned");
+    for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>(table, "table"), {lens, "lens"}}) {
+        TORCH_CHECK(t.is_cuda() && t.get_device() == cache.get_device(), name, " must be on the same CUDA device as cache");
+        TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32");
+    }
+    TORCH_CHECK(table.dim() == 2, "table must have shape [batch, entries]");
+    TORCH_CHECK(lens.dim() == 1 && lens.size(0) == table.size(0), "lens must have shape [batch]");
+    if (table.size(1) > 1 && table.stride(1) != 1) table = table.contiguous();
+    lens = lens.contiguous();
+    c.cache = cache.data_ptr();
+    c.table = table.data_ptr<int32_t>();
+    c.lens = lens.data_ptr<int32_t>();
+    c.pages = cache.size(0);
+    c.page_size = bytes / row;
+    c.kv_heads = cache.size(2);
+    c.head_dim = head_dim;
+    c.batch = table.size(0);
+    c.entries = table.size(1);
+    c.table_stride = table.size(0) > 1 ? table.stride(0) : 0;
+}
+
+// The operand as rows of a contiguous head dimension, pointer and strides whole
+// multiples of 16 bytes, or a copy of it.
+at::Tensor wide_rows(const at::Tensor& t) {
+    bool ok = (t.size(3) <= 1 || t.stride(3) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void check_no_grad(std::initializer_list<const at::Tensor*> operands, const char* what) {
+    for (const at::Tensor* t : operands)
+        TORCH_CHECK(!at::GradMode::is_enabled() || !t->requires_grad(), what,
+                    " has no backward; call it under torch.no_grad()");
+    refuse_tangents(operands, what);
+}
+
+void paged_fp4_store(at::Tensor cache, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor lens) {
+    check_no_grad({&k, &v}, "store_fp4");
+    check_heads(k, "k", "[batch, tokens, kv_heads, head_dim]");
+    check_heads(v, "v", "[batch, tokens, kv_heads, head_dim]");
+    TORCH_CHECK(k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() && k.get_device() == v.get_device(),
+                "k and v must have the same shape, dtype and device");
+    spline_hip_fp4_cache c{};
+    fill_fp4_cache(c, cache, table, lens, k.size(3));
+    TORCH_CHECK(k.get_device() == cache.get_device(), "k must be on the same CUDA device as cache");
+    TORCH_CHECK(k.size(0) == c.batch, "table must hold k's batch");
+    TORCH_CHECK(k.size(2) == c.kv_heads, "k must have the cache's kv heads (", c.kv_heads, "), got ", k.size(2));
+    c10::OptionalDeviceGuard guard(cache.device());
+    const at::Tensor kr = wide_rows(k), vr = wide_rows(v);
+    int64_t ks[3], vs[3];
+    row_strides(ks, kr, 0, 1, 2);
+    row_strides(vs, vr, 0, 1, 2);
+    void* s = current_stream(cache);
+    check_launch((k.scalar_type() == at::kBFloat16 ? launch_paged_fp4_store_bf16 : launch_paged_fp4_store_fp16)(
+                     &c, kr.data_ptr(), vr.data_ptr(), ks, vs, k.size(1), s),
+                 s);
+}
+
+std::vector<at::Tensor> paged_fp4_load(at::Tensor cache, at::Tensor table, at::Tensor lens, int64_t tokens,
+                                       int64_t head_dim, at::ScalarType dtype) {
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be float16 or bfloat16");
+    TORCH_CHECK(tokens >= 0, "tokens must not be negative, got ", tokens);
+    spline_hip_fp4_cache c{};
+    fill_fp4_cache(c, cache, table, lens, head_dim);
+    c10::OptionalDeviceGuard guard(cache.device());
+    at::Tensor k = at::empty({c.batch, tokens, c.kv_heads, head_dim}, cache.options().dtype(dtype));
+    at::Tensor v = at::empty_like(k);
+    void* s = current_stream(cache);
+    check_launch((dtype == at::kBFloat16 ? launch_paged_fp4_load_bf16 : launch_paged_fp4_load_fp16)(
+                     &c, k.data_ptr(), v.data_ptr(), tokens, s),
+                 s);
+    return {k, v};
+}
+
+std::vector<at::Tensor> paged_fp4_attn_fwd(at::Tensor q, at::Tensor cache, at::Tensor table, at::Tensor lens,
+                                           int64_t mode, double softmax_scale, double softcap) {
+    check_no_grad({&q}, "flash_attn_paged_fp4");
+    check_heads(q, "q", "[batch, tokens, heads, head_dim]");
+    spline_hip_fp4_cache c{};
+    fill_fp4_cache(c, cache, table, lens, q.size(3));
+    TORCH_CHECK(q.get_device() == cache.get_device(), "q must be on the same CUDA device as cache");
+    TORCH_CHECK(q.size(0) == c.batch, "table must hold q's batch");
+    const int64_t b = q.size(0), tokens = q.size(1), hq = q.size(2), d = q.size(3);
+    TORCH_CHECK(c.kv_heads > 0 && hq > 0 && hq % c.kv_heads == 0, "q heads (", hq,
+                ") must be a positive multiple of kv heads (", c.kv_heads, ")");
+    TORCH_CHECK(softmax_scale > 0 && softmax_scale <= std::numeric_limits<float>::max(),
+                "softmax_scale must be positive and finite");
+    c10::OptionalDeviceGuard guard(cache.device());
+    const at::Tensor qr = wide_rows(q);
+    at::Tensor out = at::empty({b, tokens, hq, d}, q.options());
+    at::Tensor lse = at::empty({b, hq, tokens}, q.options().dtype(at::kFloat));
+    spline_hip_fp4_attention a{};
+    a.out = out.data_ptr();
+    a.lse = lse.data_ptr<float>();
+    a.q = qr.data_ptr();
+    a.tokens = tokens;
+    a.q_heads = hq;
+    row_strides(a.q_strides, qr, 0, 1, 2);
+    a.mode = (int32_t)mode;
+    a.scale = (float)softmax_scale;
+    a.cap = (float)softcap;
+    const int64_t bytes = spline_hip_paged_fp4_workspace_bytes(&c, &a);
+    TORCH_CHECK(bytes >= 0, "too many rows, keys, pages or heads for the attention over 4-bit pages");
+    at::Tensor ws = at::empty({bytes}, cache.options());
+    a.workspace = ws.data_ptr();
+    void* s = current_stream(cache);
+    check_launch((q.scalar_type() == at::kBFloat16 ? launch_paged_fp4_attention_bf16 : launch_paged_fp4_attention_fp16)(
+                     &c, &a, s),
+                 s);
+    return {out, lse};
+}
+
+// The caches whose pages move with a table, and the table.
+struct PageCall {
+    spline_hip_pages a{};
+    std::vector<void*> at;
+    std::vector<int64_t> bytes;
+    at::Tensor table, out, count, workspace;
+
+    PageCall(const std::vector<at::Tensor>& caches, const at::Tensor& table_) : table(table_) {
+        TORCH_CHECK(!caches.empty(), "caches must hold at least one cache");
+        TORCH_CHECK(table.is_cuda() && table.scalar_type() == at::kInt && table.dim() == 2,
+                    "table must be an int32 CUDA tensor [rows, entries]");
+        a.pages = caches[0].dim() > 0 ? caches[0].size(0) : 0;
+        for (const at::Tensor& t : caches) {
+            TORCH_CHECK(t.is_cuda() && t.get_device() == table.get_device(),
+                        "every cache must be on the same CUDA device as table");
+            TORCH_CHECK(t.dim() > 0 && t.is_contiguous() && t.size(0) == a.pages,
+                        "every cache must be contiguous, its first dimension the same pages");
+            TORCH_CHECK(!t.requires_grad(), "a cache whose pages move must not require gradients");
+            const int64_t page = a.pages > 0 ? (int64_t)t.nbytes() / a.pages : 0;
+            TORCH_CHECK(page % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                        "pages must be whole multiples of 16 bytes, aligned to them");
+            at.push_back(t.data_ptr());
+            bytes.push_back(page);
+        }
+        if (table.size(1) > 1 && table.stride(1) != 1) table = table.contiguous();
+        a.caches = at.data();
+        a.cache_page_bytes = bytes.data();
+        a.num_caches = (int64_t)at.size();
+        a.table = table.data_ptr<int32_t>();
+        a.old_rows = a.rows = table.size(0);
+        a.entries = table.size(1);
+        a.table_stride = a.old_rows > 1 ? table.stride(0) : 0;
+    }
+    void launch(int64_t (*size)(const spline_hip_pages*), int (*fn)(const spline_hip_pages*, void*)) {
+        out = at::empty({a.rows, a.entries}, table.options());
+        count = at::empty({1}, table.options());
+        a.out_table = out.data_ptr<int32_t>();
+        a.out_count = count.data_ptr<int32_t>();
+        const int64_t n = size(&a);
+        TORCH_CHECK(n >= 0, "too many rows, entries, pages or tokens");
+        workspace = at::empty({n}, table.options().dtype(at::kByte));
+        a.workspace = workspace.data_ptr();
+        void* s = current_stream(table);
+        check_launch(fn(&a, s), s);
+    }
+};
+
+std::vector<at::Tensor> fork_pages(std::vector<at::Tensor> caches, at::Tensor table, at::Tensor lens,
+                                   c10::optional<at::Tensor> parents, int64_t tokens, int64_t page_size) {
+    PageCall call(caches, table);
+    TORCH_CHECK(lens.is_cuda() && lens.get_device() == table.get_device() && lens.scalar_type() == at::kInt &&
+                    lens.dim() == 1 && lens.size(0) == table.size(0),
+                "lens must be an int32 tensor [rows] on the same CUDA device as table");
+    TORCH_CHECK(page_size > 0, "page_size must be positive, got ", page_size);
+    TORCH_CHECK(tokens >= 0, "tokens must not be negative, got ", tokens);
+    c10::OptionalDeviceGuard guard(table.device());
+    lens = lens.contiguous();
+    call.a.lens = lens.data_ptr<int32_t>();
+    at::Tensor from;
+    if (parents) {
+        TORCH_CHECK(parents->is_cuda() && parents->get_device() == table.get_device() &&
+                        parents->scalar_type() == at::kInt && parents->dim() == 1,
+                    "parents must be an int32 tensor [new rows] on the same CUDA device as table");
+        from = parents->contiguous();
+        call.a.parents = from.data_ptr<int32_t>();
+        call.a.rows = from.size(0);
+    }
+    at::Tensor out_lens = at::empty({call.a.rows}, lens.options());
+    call.a.out_lens = out_lens.data_ptr<int32_t>();
+    call.a.page_size = page_size;
+    call.a.grow = tokens;
+    call.launch(spline_hip_fork_pages_workspace_bytes, launch_fork_pages);
+    return {call.out, out_lens, call.count};
+}
+
+std::vector<at::Tensor> compact_pages(std::vector<at::Tensor> caches, at::Tensor table) {
+    PageCall call(caches, table);
+    c10::OptionalDeviceGuard guard(table.device());
+    call.launch(spline_hip_compact_pages_workspace_bytes, launch_compact_pages);
+    return {call.out, call.count};
+}
+
 // Largest dS workspace the attention backward allocates: the environment's
 // SPLINE_ATTN_DS_MAX_BYTES (bytes, 0 turns the dS-keeping backward off),
 // 8 GiB by default.
@@ -1959,6 +2168,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "Attention of new tokens [B,T,Hq,D] over a prefix [P,Hkv,D] that the batch shares and each sequence's "
           "own cache [B,L,Hkv,D] -> [out [B,T,Hq,D], lse [B,Hq,T] FP32]; mode 0 softmax, 3 softcap, "
           "4 D4 softcap (BF16)");
+
+    // a serving cache in pages of 4-bit numbers
+    m.def("paged_fp4_store", &paged_fp4_store, py::arg("cache"), py::arg("k"), py::arg("v"), py::arg("table"),
+          py::arg("lens"),
+          "Stores new keys and values [B,T,Hkv,D] as E2M1 numbers in blocks of 32 into the pages that table [B,entries] "
+          "names, at positions lens - T ..");
+    m.def("paged_fp4_load", &paged_fp4_load, py::arg("cache"), py::arg("table"), py::arg("lens"), py::arg("tokens"),
+          py::arg("head_dim"), py::arg("dtype"), "The last tokens of each sequence in the cache -> [k, v] [B,T,Hkv,D]");
+    m.def("paged_fp4_attn_fwd", &paged_fp4_attn_fwd, py::arg("q"), py::arg("cache"), py::arg("table"), py::arg("lens"),
+          py::arg("mode"), py::arg("softmax_scale"), py::arg("softcap") = 0.0,
+          "Attention of new tokens [B,T,Hq,D] over the pages of their sequences -> [out [B,T,Hq,D], lse [B,Hq,T] FP32]; "
+          "mode 0 softmax, 3 softcap, 4 D4 softcap (BF16)");
+    m.def("fork_pages", &fork_pages, py::arg("caches"), py::arg("table"), py::arg("lens"), py::arg("parents"),
+          py::arg("tokens"), py::arg("page_size"),
+          "New rows of a page table that continue old ones, with copies of the pages that they will write -> "
+          "[table, lens, short]");
+    m.def("compact_pages", &compact_pages, py::arg("caches"), py::arg("table"),
+          "Moves the pages in use to the caches' front -> [table, used]");
 
     // RoPE reference evaluator (sfu_repro.rope.polynomial_sincos on the device)
     m.def("polynomial_sincos_f32", &polynomial_sincos_f32, py::arg("angles"),

@@ -1,0 +1,671 @@
+// paged_attn.hip -- attention of new tokens over a cache in pages of 4-bit numbers
+// (fp4.hpp), for gfx950.
+//
+//   out[b, t] = softmax(s) V over keys 0 .. lens[b] - T + t of sequence b,
+//   s = q.k scale, or cap tanh(q.k scale / cap)
+//
+// The T g rows of a sequence and KV head (g query heads to a KV head) are cut into
+// tiles of 16 or 32; a tile, its keys and a KV head are a unit.  The keys of
+// all units, laid end to end in steps of 128, are divided evenly among a fixed number of
+// blocks, whatever the lengths are: a block takes its stretch of this line, which
+// may begin inside a unit and reach over several.  A unit within one block leaves
+// as its result; the pieces of one that is cut leave O, maximum and sum in FP32,
+// two pieces a block at most, and a second launch joins them:
+// O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  So neither time nor workspace goes
+// by what the table could hold.
+//
+// Of a step's 128 keys each of a block's four waves has 32, and none waits for
+// another.  Products are S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32, a
+// lane keeping one row (query).  K needs no LDS: the sum over the head dimension may take
+// its elements in any order, so a lane loads 16 bytes of a key, 32 elements of one
+// block, and turns each word into a fragment of K (v_cvt_scalef32_pk_bf16_fp4, exact);
+// Q's fragments follow that order.  V has to be turned by keys: BF16 rows in the
+// wave's own LDS, read back transposed (ds_read_b64_tr_b16).
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "fp4.hpp"
+
+namespace pt {
+
+constexpr int kStep = 128;       // keys of a block's step
+constexpr int kWaveKeys = 32;    // of which a wave has 32
+constexpr float kEmptyMax = -__FLT_MAX__;  // log2 units: below any score, and no infinity
+// From this maximum on (log2 units) scores lose the maximum in a step of its own: an FMA
+// keeps the product's rounding, half a step of the maximum, which passes the exponents'
+// range beyond 2^30, and is 2^-4 here.
+constexpr float kFarMax = 0x1p20f;
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+struct PagedParams {
+    const uint16_t* q;
+    Fp4Pages c;
+    AttnStrides qs;
+    float* part_o;    // [2 blocks][ROWS][HD]
+    float2* part_ml;  // [2 blocks][ROWS]
+    int4* cut;        // [blocks] the unit that leaves a block unfinished: batch and tile, head, last block
+    void* out;
+    float* lse;
+    int hq, group, tokens, rows, tiles, capacity;
+    int64_t places;  // batch * tiles
+    float scale, cap;
+};
+
+__device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// x of lane l ^ 16 and of l ^ 32 combined with this lane's.
+__device__ __forceinline__ float row_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+    return half_max(__builtin_fmaxf(as_f32(r[0]), as_f32(r[1])));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+    return half_sum(as_f32(r[0]) + as_f32(r[1]));
+}
+
+// ---- the line of all units ------------------------------------------------------
+
+// Keys that a row tile of a sequence sees, in steps (one at least: a tile without
+// keys leaves zeros).
+template <int ROWS>
+struct Place {
+    int64_t b;
+    int r0, nrows;  // rows of the sequence
+    int seen;       // keys that token 0 sees (token t: t more), not held to the table
+    int visible;    // keys that the tile's last row sees
+
+    __device__ __forceinline__ Place(const PagedParams& p, int64_t place) {
+        b = place / p.tiles;
+        r0 = (int)(place - b * p.tiles) * ROWS;
+        nrows = p.rows - r0 < ROWS ? p.rows - r0 : ROWS;
+        seen = p.c.len(b) - p.tokens + 1;
+        visible = keys_of(p, (r0 + nrows - 1) / p.group);
+    }
+    // Keys that a token sees.
+    __device__ __forceinline__ int keys_of(const PagedParams& p, int token) const {
+        const int64_t n = (int64_t)seen + token;
+        return n < 0 ? 0 : n < p.capacity ? (int)n : p.capacity;
+    }
+    __device__ __forceinline__ int steps() const { return visible <= kStep ? 1 : (visible + kStep - 1) / kStep; }
+};
+
+// Sums over a block of 256: of the threads ahead, and of all.
+__device__ __forceinline__ int64_t scan256(int64_t x, int64_t& total, int64_t* sums) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t inc = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int64_t y = __shfl_up(inc, d);
+        inc += lane >= d ? y : 0;
+    }
+    if (lane == 63) sums[wave] = inc;
+    __syncthreads();
+    int64_t ahead = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        ahead += w < wave ? sums[w] : 0;
+        total += sums[w];
+    }
+    return ahead + inc - x;
+}
+
+// ---- scores -----------------------------------------------------------------------
+
+// The capped scores of a softcap mode (softmax_exponents for any even number).
+template <int MODE, int N>
+__device__ __forceinline__ void cap_scores(float (&x)[N], const ScoreConsts& k) {
+    if constexpr (MODE == kAttnSoftcapD4) {
+#pragma unroll
+        for (int r = 0; r < N; r += 2) {
+            const uint32_t u = pack_bf(rbf(x[r] * k.scale) * k.inv_cap, rbf(x[r + 1] * k.scale) * k.inv_cap);
+            float t0, t1;
+            SoftcapConsts::T::eval2(u, k.tanh, t0, t1);
+            x[r] = rbf(t0 * k.cap);
+            x[r + 1] = rbf(t1 * k.cap);
+        }
+    } else if constexpr (MODE == kAttnSoftcapNative) {
+#pragma unroll
+        for (int r = 0; r < N; ++r) x[r] = k.cap * native_lane<kTanh, kFwd>(x[r] * k.scale * k.inv_cap);
+    }
+}
+
+__device__ __forceinline__ bf16x8_t prob_frag(const float (&s)[8]) {
+    bf16x8_t f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (__bf16)s[e];
+    return f;
+}
+// What that rounding left, as a second operand.
+__device__ __forceinline__ bf16x8_t prob_rest(const float (&s)[8], bf16x8_t hi) {
+    bf16x8_t f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (__bf16)(s[e] - (float)hi[e]);
+    return f;
+}
+
+// FP32 rows of O in LDS, 16 bytes between them: 16 rows' chunks fall on different columns.
+template <int HD>
+__device__ __forceinline__ constexpr uint32_t o_at(int row, int chunk) {
+    return (uint32_t)(row * (HD * 4 + 16) + chunk * 16);
+}
+
+// Elements 4 chunk .. of a row of a place, divided by their sum, to the result.
+template <int HD, bool BF>
+__device__ __forceinline__ void write_row(const PagedParams& p, int64_t b, int row, int kvh, int chunk, f32x4_t o,
+                                          float2 ml) {
+    const float inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;  // a row that sees no key is zero
+    const int t = row / p.group, head = kvh * p.group + (row - t * p.group);
+    const int64_t bt = b * p.tokens + t;
+    uint2 w;
+    if constexpr (BF) {
+        w = make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
+    } else {
+        w = make_uint2(as_u32((h2_t){(_Float16)(o[0] * inv), (_Float16)(o[1] * inv)}),
+                       as_u32((h2_t){(_Float16)(o[2] * inv), (_Float16)(o[3] * inv)}));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (bt * p.hq + head) * HD + chunk * 4) = w;
+    if (chunk == 0 && p.lse != nullptr)
+        p.lse[(b * p.hq + head) * p.tokens + t] =
+            ml.y == 0.0f ? -__builtin_inff() : (ml.x + __builtin_log2f(ml.y)) * kLn2;
+}
+
+// ---- a wave's tile of 32 keys -------------------------------------------------------
+
+// A wave's rows of V in BF16, 32 bytes between them and 16 more between groups of eight:
+// 16 rows' writes of one chunk, and the 8 rows by 32 bytes of half a transposing read,
+// fall on different columns of the 256 bytes that LDS serves at once.
+template <int HD>
+__device__ __forceinline__ constexpr uint32_t v_at(int row, int chunk) {
+    return (uint32_t)(row * (HD * 2 + 32) + (row >> 3) * 16 + chunk * 16);
+}
+
+// The codes of 16 keys that a lane holds: HD / 4 elements of key lane % 16, from
+// (lane / 16) HD / 4 on, and their block's byte.
+template <int HD>
+struct Codes {
+    uint32_t w[HD / 32];
+    uint32_t byte;
+
+    __device__ __forceinline__ void load(const uint8_t* head, uint32_t code, uint32_t at) {
+        if constexpr (HD == 128) {
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(head + code);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = a[i];
+        } else {
+            const u32x2_t a = *reinterpret_cast<const u32x2_t*>(head + code);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[i] = a[i];
+        }
+        byte = head[at];
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) w[i] = 0;
+        byte = 127;
+    }
+};
+
+// The rows that a lane's query has seen so far.
+template <int HD>
+struct PagedState {
+    f32x4_t o[HD / 16];  // O^T: o[dt][r] = element 16 dt + 4 (lane / 16) + r of row lane % 16
+    float m, l;          // log2 units; l of this lane's quarter of the keys
+
+    __device__ __forceinline__ PagedState() : m(kEmptyMax), l(0.0f) {
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) o[dt] = (f32x4_t){};
+    }
+};
+
+// A block's stretch of the line, and what its waves need throughout.
+template <int MODE, int HD, int NR, bool BF>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? (HD == 64 ? 4 : 3) : BF || HD == 64 ? 2 : 1))) paged_fp4_kernel(PagedParams p) {
+    constexpr int ROWS = 16 * NR, kC = HD / 32, kD = HD / 16;
+    constexpr int kVTile = v_at<HD>(kWaveKeys, 0), kSpill = o_at<HD>(16, 0);
+    constexpr int kRegion = kVTile > kSpill ? kVTile : kSpill;
+    __shared__ __align__(1024) unsigned char smem[4 * kRegion];
+    __shared__ float2 sml[4][16];
+    __shared__ int64_t sums[4];
+    __shared__ int64_t start[2];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int c16 = lane & 15, quarter = lane >> 4;
+
+    // ---- where the block's stretch begins
+    const int64_t each = (p.places + 255) / 256;
+    const int64_t from = tid * each, to = from + each < p.places ? from + each : p.places;
+    int64_t mine = 0;
+    for (int64_t i = from; i < to; ++i) mine += Place<ROWS>(p, i).steps();
+    int64_t plane;  // steps of a KV head
+    int64_t ahead = scan256(mine, plane, sums);
+    const int64_t all = plane * p.c.hkv;
+    const int64_t blocks = all < gridDim.x ? all : gridDim.x;  // with a step at least
+    if (blockIdx.x >= blocks) {
+        if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, -1);
+        return;
+    }
+    const int64_t x1 = (int64_t)(blockIdx.x + 1) * all / blocks;
+    int64_t x = (int64_t)blockIdx.x * all / blocks;
+    int kvh = (int)(x / plane);
+    const int64_t in = x - kvh * plane;
+    if (in >= ahead && in < ahead + mine)
+        for (int64_t i = from; i < to; ++i) {
+            const int n = Place<ROWS>(p, i).steps();
+            if (in < ahead + n) {
+                start[0] = i;
+                start[1] = in - ahead;
+                break;
+            }
+            ahead += n;
+        }
+    __syncthreads();
+    int64_t place = start[0];
+    int step0 = (int)start[1];
+
+    ScoreConsts consts;
+    consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
+    consts.scale = p.scale;
+    consts.cap = p.cap;
+    consts.inv_cap = 1.0f / p.cap;
+    if constexpr (MODE == kAttnSoftcapD4)
+#pragma unroll
+        for (int i = 1; i <= SoftcapConsts::T::P.deg; ++i) consts.tanh[i] = bf16_value(SoftcapConsts::T::P.c[i]);
+
+    unsigned char* vt = smem + wave * kRegion;
+    bool first_piece = true;
+    for (; x < x1;) {
+        const Place<ROWS> at(p, place);
+        const int steps = at.steps();
+        const int n = x1 - x < steps - step0 ? (int)(x1 - x) : steps - step0;
+        // ---- Q^T fragments: elements (HD / 4) quarter + 8 c .. of row c16
+        bf16x8_t qf[NR][kC], ql[BF ? 1 : NR][kC];
+        int klast[NR];  // the last key that the lane's row sees
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            const int row = nr * 16 + c16;
+            const bool rin = row < at.nrows;
+            const int t = (at.r0 + (rin ? row : 0)) / p.group;
+            klast[nr] = (rin ? at.keys_of(p, t) : at.visible) - 1;
+            const uint16_t* src = p.q + at.b * p.qs.b + t * p.qs.s +
+                                  (kvh * p.group + (at.r0 + (rin ? row : 0) - t * p.group)) * p.qs.h + quarter * (HD / 4);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                bf16x8_t f = {};
+                if (rin) f = *reinterpret_cast<const bf16x8_t*>(src + 8 * c);
+                if constexpr (!BF) {
+                    const f16x8_t hf = __builtin_bit_cast(f16x8_t, f);
+                    bf16x8_t hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = (float)hf[e];
+                        hi[e] = (__bf16)v;
+                        const float left = v - (float)hi[e];
+                        lo[e] = (__bf16)(left - left == 0.0f ? left : 0.0f);  // none of an infinity
+                    }
+                    qf[nr][c] = hi;
+                    ql[nr][c] = lo;
+                } else {
+                    qf[nr][c] = f;
+                }
+            }
+        }
+        PagedState<HD> st[NR];
+        const int kfull = at.keys_of(p, at.r0 / p.group) - 1;  // every row sees the keys up to it
+
+        // ---- the wave's tiles of 32 keys, one a step.  Lane 2 i + g knows where group g
+        // of step i lies, 32 steps at a time.  Codes of the next tile fly from where this
+        // one's are used on.
+        int my_page = -1, my_row = 0;
+        auto look_up = [&](int i0) __attribute__((always_inline)) {
+            const int key = (step0 + i0 + (lane >> 1)) * kStep + wave * kWaveKeys + (lane & 1) * 16;
+            const int entry = key / p.c.page_size;
+            my_page = i0 + (lane >> 1) < n && key < at.visible ? p.c.page_of(at.b, entry) : -1;
+            my_row = key - entry * p.c.page_size;
+        };
+        const uint32_t lane_code = (uint32_t)(c16 * (HD / 2) + quarter * (HD / 8));
+        const uint32_t lane_byte = (uint32_t)(p.c.page_size * (HD / 2) + c16 * (HD / kFp4Block) + quarter * (HD / 4) / kFp4Block);
+        auto load = [&](Codes<HD>& codes, int kv, int i, int g) __attribute__((always_inline)) {
+            const int l = 2 * (i & 31) + g;
+            const int page = __builtin_amdgcn_readlane(my_page, l), row = __builtin_amdgcn_readlane(my_row, l);
+            if (page < 0) codes.clear();
+            else codes.load(p.c.head(page, kv, kvh), (uint32_t)row * (HD / 2) + lane_code, (uint32_t)row * (HD / kFp4Block) + lane_byte);
+        };
+        unsigned char* const v_write = vt + v_at<HD>(c16, quarter * kC);
+        const unsigned char* const v_read = vt + v_at<HD>(4 * quarter + (c16 >> 2), (c16 & 3) >> 1) + (c16 & 1) * 8;
+        // columns 16 dt + c16 of rows 4 quarter .. + 3 and 16 + 4 quarter .. + 3
+        auto value_frag = [&](int dt) __attribute__((always_inline)) {
+            const uint16_t* src = reinterpret_cast<const uint16_t*>(v_read + dt * 32);
+            const u32x2_t lo = __builtin_bit_cast(u32x2_t, lds_read_tr16(src));
+            const u32x2_t hi = __builtin_bit_cast(u32x2_t, lds_read_tr16(src + v_at<HD>(16, 0) / 2));
+            return __builtin_bit_cast(bf16x8_t, (u32x4_t){lo.x, lo.y, hi.x, hi.y});
+        };
+        Codes<HD> k[2], v[2];
+        for (int i = 0; i < n; ++i) {
+            if ((i & 31) == 0) {
+                look_up(i);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) load(k[g], 0, i, g);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) load(v[g], 1, i, g);
+            }
+            const bool more = i + 1 < n && (i & 31) != 31;
+            const int key0 = (step0 + i) * kStep + wave * kWaveKeys;
+            const bool hole[2] = {__builtin_amdgcn_readlane(my_page, 2 * (i & 31)) < 0,
+                                  __builtin_amdgcn_readlane(my_page, 2 * (i & 31) + 1) < 0};
+            const bool masked = key0 + kWaveKeys - 1 > kfull || hole[0] || hole[1];
+            f32x4_t s[2][NR];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const float scale = fp4_scale(k[g].byte);
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) s[g][nr] = (f32x4_t){};
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    const bf16x8_t kf = fp4_to_bf16(k[g].w[c], scale);
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr) {
+                        s[g][nr] = mfma16(kf, qf[nr][c], s[g][nr]);
+                        if constexpr (!BF) s[g][nr] = mfma16(kf, ql[nr][c], s[g][nr]);
+                    }
+                }
+                if (more) load(k[g], 0, i + 1, g);
+            }
+            // V to LDS; in a tile with keys that some row does not see, blocks that are no
+            // numbers as zeros (0 * NaN is NaN)
+            bool bad[2] = {false, false};
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                if (masked) {
+                    bad[g] = v[g].byte > (uint32_t)kFp4Most;
+                    if (bad[g]) v[g].clear();
+                }
+                const float scale = fp4_scale(v[g].byte);
+#pragma unroll
+                for (int c = 0; c < kC; ++c)
+                    *reinterpret_cast<bf16x8_t*>(v_write + v_at<HD>(16 * g, c)) = fp4_to_bf16(v[g].w[c], scale);
+                if (more) load(v[g], 1, i + 1, g);
+            }
+            // probabilities of keys 4 quarter + r of the first group, then of the second
+            bf16x8_t pf[NR], pr[NR];
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][nr][e & 3];
+                cap_scores<MODE>(y, consts);
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (hole[e >> 2] || key0 + 16 * (e >> 2) + 4 * quarter + (e & 3) > klast[nr]) y[e] = -__builtin_inff();
+                }
+                float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y[0], y[1]), __builtin_fmaxf(y[2], y[3])),
+                                           __builtin_fmaxf(__builtin_fmaxf(y[4], y[5]), __builtin_fmaxf(y[6], y[7])));
+                mx = row_max(mx) * consts.sl;
+                const bool move = mx - st[nr].m > 8.0f;  // the lanes of a row decide alike
+                if (__any(move)) {
+                    const float m = move ? mx : st[nr].m;
+                    const float alpha = __builtin_amdgcn_exp2f(st[nr].m - m);
+                    st[nr].m = m;
+                    st[nr].l *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < kD; ++dt) st[nr].o[dt] *= alpha;
+                }
+                float mul = consts.sl;
+                const bool far = __builtin_fabsf(st[nr].m) >= kFarMax;
+                if (__any(far)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = far ? y[e] * mul : y[e];
+                    mul = far ? 1.0f : mul;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], mul, -st[nr].m));
+                st[nr].l += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+                pf[nr] = prob_frag(y);
+                pr[nr] = prob_rest(y, pf[nr]);
+            }
+            // O^T += V^T P^T
+#pragma unroll
+            for (int dt = 0; dt < kD; ++dt) {
+                const bf16x8_t vf = value_frag(dt);
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) {
+                    st[nr].o[dt] = mfma16(vf, pf[nr], st[nr].o[dt]);
+                    st[nr].o[dt] = mfma16(vf, pr[nr], st[nr].o[dt]);
+                }
+            }
+            if (__any(bad[0] || bad[1])) {
+                // ones in the places of NaN, times ones for the keys that a row sees
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const __bf16 one = (__bf16)(bad[g] ? 1.0f : 0.0f);
+                    const bf16x8_t marks = {one, one, one, one, one, one, one, one};
+#pragma unroll
+                    for (int c = 0; c < kC; ++c) *reinterpret_cast<bf16x8_t*>(v_write + v_at<HD>(16 * g, c)) = marks;
+                }
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) {
+                    bf16x8_t sees;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        sees[e] = (__bf16)(key0 + 16 * (e >> 2) + 4 * quarter + (e & 3) > klast[nr] ? 0.0f : 1.0f);
+#pragma unroll
+                    for (int dt = 0; dt < kD; ++dt) {
+                        const f32x4_t hit = mfma16(value_frag(dt), sees, (f32x4_t){});
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (hit[r] != 0.0f) st[nr].o[dt][r] = __builtin_nanf("");
+                    }
+                }
+            }
+        }
+
+        // ---- the waves' shares of each row
+        const bool begins = step0 == 0, ends = step0 + n == steps;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            if (nr * 16 >= at.nrows) break;
+            __syncthreads();  // the region is free
+            unsigned char* region = smem + wave * kRegion;
+#pragma unroll
+            for (int dt = 0; dt < kD; ++dt)
+                *reinterpret_cast<f32x4_t*>(region + o_at<HD>(c16, 4 * dt + quarter)) = st[nr].o[dt];
+            const float l = row_sum(st[nr].l);
+            if (quarter == 0) sml[wave][c16] = make_float2(st[nr].m, l);
+            __syncthreads();
+            constexpr int kChunks = HD / 4;
+            for (int i = tid; i < 16 * kChunks; i += 256) {
+                const int row = i / kChunks, chunk = i % kChunks;
+                if (nr * 16 + row >= at.nrows) continue;
+                float2 ml = make_float2(kEmptyMax, 0.0f);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) ml.x = __builtin_fmaxf(ml.x, sml[w][row].x);
+                f32x4_t o = {};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float2 y = sml[w][row];
+                    const float a = __builtin_amdgcn_exp2f(y.x - ml.x);
+                    o += *reinterpret_cast<const f32x4_t*>(smem + w * kRegion + o_at<HD>(row, chunk)) * a;
+                    ml.y = __builtin_fmaf(y.y, a, ml.y);
+                }
+                if (begins && ends) {
+                    write_row<HD, BF>(p, at.b, at.r0 + nr * 16 + row, kvh, chunk, o, ml);
+                } else {
+                    *reinterpret_cast<f32x4_t*>(p.part_o + (slot * ROWS + nr * 16 + row) * HD + chunk * 4) = o;
+                    if (chunk == 0) p.part_ml[slot * ROWS + nr * 16 + row] = ml;
+                }
+            }
+        }
+        __syncthreads();
+        if (tid == 0 && x + n == x1) {
+            int4 cut = make_int4(0, 0, 0, -1);
+            if (begins && !ends) {
+                // the block with the unit's last step: the first whose stretch ends behind it
+                const int64_t end = x + steps;
+                cut = make_int4((int)place, (int)(place >> 32), kvh, (int)((end * blocks + all - 1) / all - 1));
+            }
+            p.cut[blockIdx.x] = cut;
+        }
+        x += n;
+        step0 = 0;
+        if (ends && ++place == p.places) {
+            place = 0;
+            ++kvh;
+        }
+    }
+}
+
+// Joins the pieces of the unit that leaves block blockIdx.x unfinished.  HD / 4 lanes
+// hold a row, and the groups of them beyond the rows take the pieces in turn.
+template <int HD, int NR, bool BF>
+__global__ void __launch_bounds__(1024) paged_join_kernel(PagedParams p) {
+    constexpr int ROWS = 16 * NR, kChunks = HD / 4, kSlots = 1024 / kChunks;
+    const int4 cut = p.cut[blockIdx.x];
+    if (cut.w < 0) return;
+    const int64_t place = ((int64_t)cut.y << 32) | (uint32_t)cut.x;
+    const Place<ROWS> at(p, place);
+    const int pieces = cut.w - (int)blockIdx.x + 1;
+    int span = 1;  // row slots: a power of two that holds the rows
+    while (span < at.nrows) span *= 2;
+    static_assert(ROWS <= kSlots, "a slot for every row");
+    const int shares = kSlots / span;
+    const int chunk = threadIdx.x % kChunks, s = threadIdx.x / kChunks;
+    const int row = s % span, share = s / span;
+    float m = kEmptyMax, l = 0.0f;
+    f32x4_t o = (f32x4_t){};
+    auto add = [&](float m2, float l2, f32x4_t o2) {
+        const float top = __builtin_fmaxf(m, m2);
+        const float a = __builtin_amdgcn_exp2f(m - top), a2 = __builtin_amdgcn_exp2f(m2 - top);
+        l = __builtin_fmaf(l, a, l2 * a2);
+        o = o * a + o2 * a2;
+        m = top;
+    };
+    if (row < at.nrows) {
+        for (int i = share; i < pieces; i += 4 * shares) {
+            float2 ml[4];
+            f32x4_t part[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = i + u * shares < pieces ? i + u * shares : i;
+                const int64_t slot = 2 * (int64_t)(blockIdx.x + j) + (j == 0 ? 1 : 0);
+                ml[u] = p.part_ml[slot * ROWS + row];
+                part[u] = *reinterpret_cast<const f32x4_t*>(p.part_o + (slot * ROWS + row) * HD + chunk * 4);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * shares < pieces) add(ml[u].x, ml[u].y, part[u]);
+        }
+    }
+    __shared__ f32x4_t so[1024];
+    __shared__ float2 sml[kSlots];
+    if (shares > 1) {
+        so[threadIdx.x] = o;
+        if (chunk == 0) sml[s] = make_float2(m, l);
+        __syncthreads();
+        if (share == 0)
+            for (int u = 1; u < shares; ++u) {
+                const float2 ml = sml[s + u * span];
+                add(ml.x, ml.y, so[threadIdx.x + u * span * kChunks]);
+            }
+    }
+    if (share == 0 && row < at.nrows) write_row<HD, BF>(p, at.b, at.r0 + row, cut.z, chunk, o, make_float2(m, l));
+}
+
+// ---- host side -----------------------------------------------------------------
+
+namespace {
+
+constexpr int64_t kMaxBlocks = 0xffffffffll / 256;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct PagedPlan {
+    int nr;          // row tiles of 16
+    int64_t blocks;  // a fixed number: the device divides the keys among them
+    int64_t bytes;   // of the workspace
+};
+
+bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, PagedPlan& p) {
+    if (!a || !fp4_sizes_ok(c, a->tokens) || a->q_heads <= 0 || a->q_heads > 65536 || a->q_heads % c->kv_heads != 0)
+        return false;
+    const int64_t rows = a->tokens * (a->q_heads / c->kv_heads);
+    p.nr = rows <= 16 ? 1 : 2;
+    p.blocks = device_shape().cus * 2;
+    const int64_t tiles = ceil_div(rows, 16 * p.nr);
+    if (c->batch > (int64_t(1) << 31) / (tiles ? tiles : 1)) return false;
+    p.bytes = p.blocks * (16 + 2 * 16 * p.nr * (c->head_dim + 2) * 4);
+    return true;
+}
+
+template <int MODE, int HD, int NR, bool BF>
+void go(const PagedParams& p, int64_t blocks, hipStream_t st) {
+    hipLaunchKernelGGL((paged_fp4_kernel<MODE, HD, NR, BF>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((paged_join_kernel<HD, NR, BF>), dim3((unsigned)blocks), dim3(1024), 0, st, p);
+}
+
+template <bool BF>
+int run(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, void* stream) {
+    PagedPlan plan_{};
+    if (!plan(c, a, plan_) || !(a->scale > 0.0f && a->scale <= __FLT_MAX__)) return hipErrorInvalidValue;
+    if (a->mode != kAttnSoftmaxNative && a->mode != kAttnSoftcapNative && !(BF && a->mode == kAttnSoftcapD4))
+        return hipErrorInvalidValue;
+    if (a->mode != kAttnSoftmaxNative && !(a->cap > 0.0f && a->cap <= __FLT_MAX__)) return hipErrorInvalidValue;
+    if (c->batch == 0 || a->tokens == 0) return hipSuccess;
+    bool ok = fp4_pointers_ok(c) && a->q && aligned16(a->q) && a->out && aligned16(a->out) &&
+              ((uintptr_t)a->lse & 3) == 0 && a->workspace && aligned16(a->workspace);
+    for (int i = 0; i < 3; ++i) ok = ok && a->q_strides[i] >= 0 && a->q_strides[i] % 8 == 0;
+    if (!ok) return hipErrorInvalidValue;
+    PagedParams p{};
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.c = fp4_pages(c);
+    p.qs = {a->q_strides[0], a->q_strides[2], a->q_strides[1]};
+    const int64_t rows = plan_.blocks * 2 * 16 * plan_.nr;
+    p.part_o = static_cast<float*>(a->workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * c->head_dim);
+    p.cut = reinterpret_cast<int4*>(p.part_ml + rows);
+    p.out = a->out;
+    p.lse = a->lse;
+    p.hq = (int)a->q_heads;
+    p.group = (int)(a->q_heads / c->kv_heads);
+    p.tokens = (int)a->tokens;
+    p.rows = p.tokens * p.group;
+    p.tiles = (int)ceil_div(p.rows, 16 * plan_.nr);
+    p.capacity = p.c.entries * p.c.page_size;
+    p.places = c->batch * p.tiles;
+    p.scale = a->scale;
+    p.cap = a->cap;
+    const hipStream_t st = hs(stream);
+    auto shape = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        if (c->head_dim == 128) plan_.nr == 1 ? go<MODE, 128, 1, BF>(p, plan_.blocks, st) : go<MODE, 128, 2, BF>(p, plan_.blocks, st);
+        else plan_.nr == 1 ? go<MODE, 64, 1, BF>(p, plan_.blocks, st) : go<MODE, 64, 2, BF>(p, plan_.blocks, st);
+    };
+    if (a->mode == kAttnSoftmaxNative) shape(std::integral_constant<int, kAttnSoftmaxNative>{});
+    else if (a->mode == kAttnSoftcapNative) shape(std::integral_constant<int, kAttnSoftcapNative>{});
+    else if constexpr (BF) shape(std::integral_constant<int, kAttnSoftcapD4>{});
+    return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace pt
+
+using namespace pt;
+
+extern "C" int64_t spline_hip_paged_fp4_workspace_bytes(const spline_hip_fp4_cache* cache,
+                                                        const spline_hip_fp4_attention* args) {
+    PagedPlan p{};
+    if (!plan(cache, args, p)) return -1;
+    return cache->batch == 0 || args->tokens == 0 ? 0 : p.bytes;
+}
+extern "C" int launch_paged_fp4_attention_fp16(const spline_hip_fp4_cache* cache, const spline_hip_fp4_attention* args,
+                                               void* stream) {
+    return run<false>(cache, args, stream);
+}
+extern "C" int launch_paged_fp4_attention_bf16(const spline_hip_fp4_cache* cache, const spline_hip_fp4_attention* args,
+                                               void* stream) {
+    return run<true>(cache, args, stream);
+}

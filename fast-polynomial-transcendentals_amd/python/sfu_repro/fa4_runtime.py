@@ -391,6 +391,20 @@ def flash_attn_bwd(q, k, v, out, dout, lse, softmax_scale=None, causal=False, so
                                             scale, cap, bias))
 
 
+def _serving_program(what, q, keys, softmax_scale, softcap, program):
+    """(mode, cap, scale) of a serving attention, whose score programs are the softmax ones."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
+    if not program:
+        return (MODE_SOFTCAP_NATIVE, float(softcap), scale) if softcap and softcap > 0 else (MODE_SOFTMAX_NATIVE, 1.0, scale)
+    mode, _, cap, _ = select_forward(seqlen=max(1, keys), softcap=softcap, **program)
+    if mode not in (MODE_SOFTMAX_NATIVE, MODE_SOFTCAP_NATIVE, MODE_SOFTCAP_D4):
+        raise NotImplementedError(
+            f"{what} is built with the hardware softmax, the hardware softcap and the D4 softcap")
+    if mode == MODE_SOFTCAP_D4 and q.dtype != torch.bfloat16:
+        raise TypeError(f"the D4 softcap is a bfloat16 program, got {q.dtype}")
+    return mode, cap, scale
+
+
 def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, softmax_scale=None,
                              softcap=0.0, **program):
     """Attention of a batch whose sequences share a prefix, for serving: returns
@@ -413,17 +427,33 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
     hardware softcap (``softcap``) and, for bfloat16, the D4 softcap (``score_mod``).
     There is no backward: operands that require gradients are refused.
     """
-    scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
-    if program:
-        mode, _, cap, _ = select_forward(seqlen=max(1, prefix_k.shape[0]), softcap=softcap, **program)
-        if mode not in (MODE_SOFTMAX_NATIVE, MODE_SOFTCAP_NATIVE, MODE_SOFTCAP_D4):
-            raise NotImplementedError(
-                "the shared-prefix attention is built with the hardware softmax, the hardware softcap and the D4 softcap")
-        if mode == MODE_SOFTCAP_D4 and q.dtype != torch.bfloat16:
-            raise TypeError(f"the D4 softcap is a bfloat16 program, got {q.dtype}")
-    else:
-        mode, cap = (MODE_SOFTCAP_NATIVE, float(softcap)) if softcap and softcap > 0 else (MODE_SOFTMAX_NATIVE, 1.0)
+    mode, cap, scale = _serving_program("the shared-prefix attention", q, prefix_k.shape[0], softmax_scale, softcap,
+                                        program)
     return tuple(_ops().shared_prefix_attn_fwd(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, mode, scale, cap))
+
+
+def flash_attn_paged_fp4(q, cache, table, lens, softmax_scale=None, softcap=0.0, **program):
+    """Attention of new tokens over a cache in pages of 4-bit numbers, for serving:
+    returns (out [B, T, Hq, D], lse [B, Hq, T]).
+
+    ``q [B, T, Hq, D]`` holds the T new tokens of each sequence (1 when decoding),
+    ``cache`` its keys and values, those of the new tokens stored
+    (:mod:`sfu_repro.paged_cache`), ``table`` int32 ``[B, entries]`` each sequence's pages
+    and ``lens`` int32 ``[B]`` its keys, the new ones among them, both on the device.  Token
+    t sees the keys at positions 0 .. ``lens[b] - T + t``; keys past them, and past the
+    table's end, may hold anything, and those of an entry that names no page (-1) are not
+    there.  A token that sees no key, or none with a score above -inf, gets zeros and an lse
+    of -inf.
+
+    float16 or bfloat16; head_dim 64 or 128; Hq a multiple of the cache's KV heads; any
+    strides (operands that 16-byte loads cannot take are copied).  Keys and values enter
+    the products as the cache holds them, without a rounding.  Time and workspace go by
+    the keys in use, not by the table's width.  The score program is that of
+    :func:`flash_attn_shared_prefix`.  There is no backward: queries that require
+    gradients are refused.
+    """
+    mode, cap, scale = _serving_program("the attention over 4-bit pages", q, 1, softmax_scale, softcap, program)
+    return tuple(_ops().paged_fp4_attn_fwd(q, cache, table, lens, mode, scale, cap))
 
 
 def runtime() -> dict:

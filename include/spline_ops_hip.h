@@ -778,6 +778,107 @@ int64_t spline_hip_shared_prefix_workspace_bytes(const spline_hip_shared_prefix*
 int launch_shared_prefix_attention_fp16(const spline_hip_shared_prefix* args, void* stream);
 int launch_shared_prefix_attention_bf16(const spline_hip_shared_prefix* args, void* stream);
 
+/* ---- a serving cache in pages of 4-bit numbers ------------------------------
+ * No counterpart in the reference.  cache: [pages][2 (keys, values)][kv_heads]
+ * [page_size * (D / 2 + D / 32)] bytes, contiguous and 16-byte aligned.  A head's
+ * bytes are page_size rows of D / 2 bytes of codes (two a byte, the even element in
+ * the low half), then page_size rows of D / 32 bytes.  Code c stands for {0, .5, 1,
+ * 1.5, 2, 3, 4, 6}[c & 7], negative with bit 3 (E2M1), times 2^(byte - 127) of its
+ * block of 32 elements; a byte above 252 makes its block NaN.
+ * table: [batch][entries] page numbers, table_stride (elements) between rows; the key
+ * at position x of sequence b is row x % page_size of page table[b][x / page_size].
+ * An entry that names no page (outside 0 .. pages - 1) holds no keys: nothing is
+ * stored there and nobody sees it.  lens: [batch] valid keys (negative: none), the
+ * new tokens among them: of T new tokens of a call, token t is at position lens[b] -
+ * T + t, and has none where that is negative or past the table (left-padded batches).
+ * D 64 or 128, page_size a multiple of 16 up to 65536, at most 2^30 keys a table row,
+ * 2^14 tokens. */
+typedef struct spline_hip_fp4_cache {
+    void* cache;
+    const int32_t *table, *lens;
+    int64_t pages, page_size, kv_heads, head_dim, batch, entries, table_stride;
+} spline_hip_fp4_cache;
+
+/* Stores k and v [B, T, Hkv, D], 16-bit, strides (batch, token, head) in elements,
+ * multiples of 8, head dimension contiguous, 16-byte aligned.  A block's power of two
+ * 2^e is the one that puts its largest magnitude into [3.5, 7) 2^e, -100 <= e <= 125; values
+ * are rounded to nearest, ties to the even code, held to 6 2^e.  A block with an
+ * infinity or NaN is stored as NaN.  Pages that are written belong to one sequence:
+ * two tokens of one call at one place leave either's bytes. */
+int launch_paged_fp4_store_fp16(const spline_hip_fp4_cache* cache, const void* k, const void* v,
+                                const int64_t* k_strides, const int64_t* v_strides, int64_t tokens, void* stream);
+int launch_paged_fp4_store_bf16(const spline_hip_fp4_cache* cache, const void* k, const void* v,
+                                const int64_t* k_strides, const int64_t* v_strides, int64_t tokens, void* stream);
+/* The last T keys and values of each sequence, k and v [B, T, Hkv, D] contiguous and
+ * 16-byte aligned: exact in BF16, rounded and held to 65504 in FP16; zeros where a
+ * token has no place. */
+int launch_paged_fp4_load_fp16(const spline_hip_fp4_cache* cache, void* k, void* v, int64_t tokens, void* stream);
+int launch_paged_fp4_load_bf16(const spline_hip_fp4_cache* cache, void* k, void* v, int64_t tokens, void* stream);
+
+/* Attention of the T new tokens of each sequence, q [B, T, Hq, D] (strides batch,
+ * token, head), over the cache: token t sees the keys at 0 .. lens[b] - T + t.
+ * out [B, T, Hq, D] contiguous; lse, float [B, Hq, T] or null, as in
+ * launch_shared_prefix_attention_bf16, and so are rows without a key (zeros, -inf),
+ * the score programs (mode 0, 3, and 4 with BF16 operands) and scale.  Keys and
+ * values enter the products exactly, FP16 queries as two BF16 terms;
+ * sums are FP32; ahead of P V probabilities are BF16 in two terms.  A NaN block in a
+ * key that a token sees makes its row NaN, in a value its elements; what nobody sees
+ * may hold anything.  Time and workspace go by the keys in use, not by the table's
+ * width.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the same
+ * device (-1: sizes that are refused), 16-byte aligned; calls that may overlap need
+ * workspaces of their own. */
+typedef struct spline_hip_fp4_attention {
+    void* out;
+    float* lse;
+    const void* q;
+    void* workspace;
+    int64_t tokens, q_heads;
+    int64_t q_strides[3];
+    int32_t mode;
+    float scale, cap;
+} spline_hip_fp4_attention;
+int64_t spline_hip_paged_fp4_workspace_bytes(const spline_hip_fp4_cache* cache, const spline_hip_fp4_attention* args);
+int launch_paged_fp4_attention_fp16(const spline_hip_fp4_cache* cache, const spline_hip_fp4_attention* args,
+                                    void* stream);
+int launch_paged_fp4_attention_bf16(const spline_hip_fp4_cache* cache, const spline_hip_fp4_attention* args,
+                                    void* stream);
+
+/* The pages of several sequences.  table: [old_rows][entries] page numbers,
+ * table_stride between rows; a page is in use where a row names it.  caches: num_caches
+ * pointers (host array) to [pages][cache_page_bytes[i]] bytes each, 16-byte aligned,
+ * page bytes multiples of 16: one a layer, of any kind, all with the same pages.
+ *
+ * launch_fork_pages: new row i of [rows][entries] continues row parents[i] (null: row
+ * i, rows = old_rows or 0; outside 0 .. old_rows - 1: an empty row) with its lens keys, held
+ * to 0 .. entries * page_size, which out_lens repeats.  Full pages are shared.  A last
+ * page that is not full stays with the first new row that has it as its last, if no
+ * row has it as a full one; the others get copies.  Rows get pages for `grow` more
+ * keys.  New pages are the lowest that no new row has kept, in the order of rows and entries;
+ * other entries are -1, and so are ones that named no page.  Pages of rows that nobody
+ * continues are free behind the call.  out_count[0]: pages that were wanted and not
+ * there (entries past the table, and last pages that an old row lacks, among them), whose entries are -1; a
+ * row whose copy was not to be had has -1 there.
+ *
+ * launch_compact_pages (rows = old_rows): of the n pages in use those with numbers from n on
+ * move to the free ones below n, both in ascending order; out_table renames them,
+ * out_count[0] = n.
+ *
+ * out_table [rows][entries], out_lens [rows] and out_count [1] are not the inputs'
+ * memory.  workspace: as the size helpers say (-1: refused), 16-byte aligned, one for
+ * each call that may overlap.  At most 2^24 rows and entries, 2^32 cells. */
+typedef struct spline_hip_pages {
+    int32_t *out_table, *out_lens, *out_count;
+    const int32_t *table, *lens, *parents;
+    void* const* caches;
+    const int64_t* cache_page_bytes;
+    void* workspace;
+    int64_t num_caches, old_rows, rows, entries, table_stride, pages, page_size, grow;
+} spline_hip_pages;
+int64_t spline_hip_fork_pages_workspace_bytes(const spline_hip_pages* args);
+int64_t spline_hip_compact_pages_workspace_bytes(const spline_hip_pages* args);
+int launch_fork_pages(const spline_hip_pages* args, void* stream);
+int launch_compact_pages(const spline_hip_pages* args, void* stream);
+
 /* ---- device/launch introspection --------------------------------------- */
 /* Number of compute units of the current device and the grid the
  * elementwise launchers use for `size` 16-bit elements and `streams` tensors
