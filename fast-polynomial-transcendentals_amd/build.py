@@ -32,7 +32,7 @@ ARCH = os.environ.get("PT_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_SOURCES = ["launch.hip", "activations.hip", "swiglu.hip", "attention.hip", "exp2_probes.hip", "experiments.hip", "sincos.hip", "rope.hip", "qk_rope.hip", "flash_attn.hip", "flash_attn_bwd.hip", "shared_prefix.hip", "paged_cache.hip", "paged_attn.hip"]
-HIP_HEADERS = ["elementwise.hpp", "ops.hpp", "programs.hpp", "trig.hpp", "score_programs.hpp", "flash_attn.hpp", "fp4.hpp"]
+HIP_HEADERS = ["elementwise.hpp", "ops.hpp", "programs.hpp", "trig.hpp", "score_programs.hpp", "flash_attn.hpp", "fp4.hpp", "row_state.hpp"]
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -26,18 +26,13 @@
 #include <type_traits>
 
 #include "fp4.hpp"
+#include "row_state.hpp"
 
 namespace pt {
 
-constexpr int kStep = 128;       // keys of a block's step
-constexpr int kWaveKeys = 32;    // of which a wave has 32
-constexpr float kEmptyMax = -__FLT_MAX__;  // log2 units: below any score, and no infinity
-// From this maximum on (log2 units) scores lose the maximum in a step of its own: an FMA
-// keeps the product's rounding, half a step of the maximum, which passes the exponents'
-// range beyond 2^30, and is 2^-4 here.
-constexpr float kFarMax = 0x1p20f;
-
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+constexpr int kNarrowStep = 128;  // keys of a narrow block's step
+constexpr int kWaveKeys = 32;     // of which a wave has 32
+constexpr int kWideStep = 64;
 
 struct PagedParams {
     const uint16_t* q;
@@ -45,7 +40,7 @@ struct PagedParams {
     AttnStrides qs;
     float* part_o;    // [2 blocks][ROWS][HD]
     float2* part_ml;  // [2 blocks][ROWS]
-    int4* cut;        // [blocks] the unit that leaves a block unfinished: batch and tile, head, last block
+    int4* cut;        // [blocks] the unit that leaves a block unfinished: place, head, last block
     void* out;
     float* lse;
     int hq, group, tokens, rows, tiles, capacity;
@@ -69,9 +64,8 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // ---- the line of all units ------------------------------------------------------
 
-// Keys that a row tile of a sequence sees, in steps (one at least: a tile without
-// keys leaves zeros).
-template <int ROWS>
+// A row tile of a sequence.
+template <int ROWS, int STEP>
 struct Place {
     int64_t b;
     int r0, nrows;  // rows of the sequence
@@ -90,29 +84,85 @@ struct Place {
         const int64_t n = (int64_t)seen + token;
         return n < 0 ? 0 : n < p.capacity ? (int)n : p.capacity;
     }
-    __device__ __forceinline__ int steps() const { return visible <= kStep ? 1 : (visible + kStep - 1) / kStep; }
+    // One at least: a tile without keys leaves zeros.
+    __device__ __forceinline__ int steps() const { return visible <= STEP ? 1 : (visible + STEP - 1) / STEP; }
 };
 
-// Sums over a block of 256: of the threads ahead, and of all.
-__device__ __forceinline__ int64_t scan256(int64_t x, int64_t& total, int64_t* sums) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t inc = x;
+// A block's stretch of the line: from step0 of a place and KV head on, x of all steps, to x1.
+template <int ROWS, int STEP>
+struct Stretch {
+    using At = Place<ROWS, STEP>;
+    int64_t all, blocks, x, x1, place;
+    int kvh, step0;
+
+    // False: none (and the block's cut says so).  block: its number on the line.
+    __device__ __forceinline__ bool find(const PagedParams& p, int64_t block) {
+        __shared__ int64_t sums[4], start[2];
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const int64_t each = (p.places + 255) / 256;
+        const int64_t from = tid * each, to = from + each < p.places ? from + each : p.places;
+        int64_t mine = 0, plane = 0, ahead = 0;  // steps of the thread's places, of a KV head, ahead
+        for (int64_t i = from; i < to; ++i) mine += At(p, i).steps();
+        int64_t inc = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int64_t y = __shfl_up(inc, d);
-        inc += lane >= d ? y : 0;
-    }
-    if (lane == 63) sums[wave] = inc;
-    __syncthreads();
-    int64_t ahead = 0;
-    total = 0;
+        for (int d = 1; d < 64; d *= 2) {
+            const int64_t y = __shfl_up(inc, d);
+            inc += lane >= d ? y : 0;
+        }
+        if (lane == 63) sums[wave] = inc;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        ahead += w < wave ? sums[w] : 0;
-        total += sums[w];
+        for (int w = 0; w < 4; ++w) {
+            ahead += w < wave ? sums[w] : 0;
+            plane += sums[w];
+        }
+        ahead += inc - mine;
+        all = plane * p.c.hkv;
+        blocks = all < gridDim.x ? all : gridDim.x;  // with a step at least
+        if (block >= blocks) {
+            if (tid == 0) p.cut[block] = make_int4(0, 0, 0, -1);
+            return false;
+        }
+        x = block * all / blocks;
+        x1 = (block + 1) * all / blocks;
+        kvh = (int)(x / plane);
+        const int64_t in = x - kvh * plane;
+        if (in >= ahead && in < ahead + mine)
+            for (int64_t i = from; i < to; ++i) {
+                const int n = At(p, i).steps();
+                if (in < ahead + n) {
+                    start[0] = i;
+                    start[1] = in - ahead;
+                    break;
+                }
+                ahead += n;
+            }
+        __syncthreads();
+        place = start[0];
+        step0 = (int)start[1];
+        return true;
     }
-    return ahead + inc - x;
-}
+    // What a block leaves unfinished behind n more steps of a unit.
+    __device__ __forceinline__ void write_cut(const PagedParams& p, int64_t block, int n, int steps) const {
+        if (threadIdx.x != 0 || x + n != x1) return;
+        int4 cut = make_int4(0, 0, 0, -1);
+        if (step0 == 0 && n < steps) {
+            // the block with the unit's last step: the first whose stretch ends behind it
+            const int64_t end = x + steps;
+            cut = make_int4((int)place, (int)(place >> 32), kvh, (int)((end * blocks + all - 1) / all - 1));
+        }
+        p.cut[block] = cut;
+    }
+    __device__ __forceinline__ void advance(const PagedParams& p, int n, int steps) {
+        const bool ends = step0 + n == steps;
+        x += n;
+        step0 = 0;
+        if (ends && ++place == p.places) {
+            place = 0;
+            ++kvh;
+        }
+    }
+};
 
 // ---- scores -----------------------------------------------------------------------
 
@@ -134,18 +184,30 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], const ScoreConsts& k) 
     }
 }
 
-__device__ __forceinline__ bf16x8_t prob_frag(const float (&s)[8]) {
+__device__ __forceinline__ bf16x8_t row_probs(const float (&s)[8]) {
     bf16x8_t f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = (__bf16)s[e];
     return f;
 }
 // What that rounding left, as a second operand.
-__device__ __forceinline__ bf16x8_t prob_rest(const float (&s)[8], bf16x8_t hi) {
+__device__ __forceinline__ bf16x8_t row_rests(const float (&s)[8], bf16x8_t hi) {
     bf16x8_t f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = (__bf16)(s[e] - (float)hi[e]);
     return f;
+}
+
+// Eight FP16 numbers as the sum of two BF16 ones, which is exact.
+__device__ __forceinline__ void split_fp16(bf16x8_t bits, bf16x8_t& hi, bf16x8_t& lo) {
+    const f16x8_t x = __builtin_bit_cast(f16x8_t, bits);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = (float)x[e];
+        hi[e] = (__bf16)v;
+        const float left = v - (float)hi[e];
+        lo[e] = (__bf16)(left - left == 0.0f ? left : 0.0f);  // none of an infinity
+    }
 }
 
 // FP32 rows of O in LDS, 16 bytes between them: 16 rows' chunks fall on different columns.
@@ -224,47 +286,16 @@ struct PagedState {
 
 // A block's stretch of the line, and what its waves need throughout.
 template <int MODE, int HD, int NR, bool BF>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? (HD == 64 ? 4 : 3) : BF || HD == 64 ? 2 : 1))) paged_fp4_kernel(PagedParams p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? (HD == 64 ? 4 : 3) : BF || HD == 64 ? 2 : 1))) paged_narrow_kernel(PagedParams p) {
     constexpr int ROWS = 16 * NR, kC = HD / 32, kD = HD / 16;
     constexpr int kVTile = v_at<HD>(kWaveKeys, 0), kSpill = o_at<HD>(16, 0);
     constexpr int kRegion = kVTile > kSpill ? kVTile : kSpill;
     __shared__ __align__(1024) unsigned char smem[4 * kRegion];
     __shared__ float2 sml[4][16];
-    __shared__ int64_t sums[4];
-    __shared__ int64_t start[2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c16 = lane & 15, quarter = lane >> 4;
-
-    // ---- where the block's stretch begins
-    const int64_t each = (p.places + 255) / 256;
-    const int64_t from = tid * each, to = from + each < p.places ? from + each : p.places;
-    int64_t mine = 0;
-    for (int64_t i = from; i < to; ++i) mine += Place<ROWS>(p, i).steps();
-    int64_t plane;  // steps of a KV head
-    int64_t ahead = scan256(mine, plane, sums);
-    const int64_t all = plane * p.c.hkv;
-    const int64_t blocks = all < gridDim.x ? all : gridDim.x;  // with a step at least
-    if (blockIdx.x >= blocks) {
-        if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, -1);
-        return;
-    }
-    const int64_t x1 = (int64_t)(blockIdx.x + 1) * all / blocks;
-    int64_t x = (int64_t)blockIdx.x * all / blocks;
-    int kvh = (int)(x / plane);
-    const int64_t in = x - kvh * plane;
-    if (in >= ahead && in < ahead + mine)
-        for (int64_t i = from; i < to; ++i) {
-            const int n = Place<ROWS>(p, i).steps();
-            if (in < ahead + n) {
-                start[0] = i;
-                start[1] = in - ahead;
-                break;
-            }
-            ahead += n;
-        }
-    __syncthreads();
-    int64_t place = start[0];
-    int step0 = (int)start[1];
+    Stretch<ROWS, kNarrowStep> line;
+    if (!line.find(p, blockIdx.x)) return;
 
     ScoreConsts consts;
     consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
@@ -276,11 +307,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         for (int i = 1; i <= SoftcapConsts::T::P.deg; ++i) consts.tanh[i] = bf16_value(SoftcapConsts::T::P.c[i]);
 
     unsigned char* vt = smem + wave * kRegion;
-    bool first_piece = true;
-    for (; x < x1;) {
-        const Place<ROWS> at(p, place);
-        const int steps = at.steps();
-        const int n = x1 - x < steps - step0 ? (int)(x1 - x) : steps - step0;
+    while (line.x < line.x1) {
+        const Place<ROWS, kNarrowStep> at(p, line.place);
+        const int steps = at.steps(), step0 = line.step0, kvh = line.kvh;
+        const int n = line.x1 - line.x < steps - step0 ? (int)(line.x1 - line.x) : steps - step0;
         // ---- Q^T fragments: elements (HD / 4) quarter + 8 c .. of row c16
         bf16x8_t qf[NR][kC], ql[BF ? 1 : NR][kC];
         int klast[NR];  // the last key that the lane's row sees
@@ -296,21 +326,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             for (int c = 0; c < kC; ++c) {
                 bf16x8_t f = {};
                 if (rin) f = *reinterpret_cast<const bf16x8_t*>(src + 8 * c);
-                if constexpr (!BF) {
-                    const f16x8_t hf = __builtin_bit_cast(f16x8_t, f);
-                    bf16x8_t hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = (float)hf[e];
-                        hi[e] = (__bf16)v;
-                        const float left = v - (float)hi[e];
-                        lo[e] = (__bf16)(left - left == 0.0f ? left : 0.0f);  // none of an infinity
-                    }
-                    qf[nr][c] = hi;
-                    ql[nr][c] = lo;
-                } else {
-                    qf[nr][c] = f;
-                }
+                if constexpr (!BF) split_fp16(f, qf[nr][c], ql[nr][c]);
+                else qf[nr][c] = f;
             }
         }
         PagedState<HD> st[NR];
@@ -321,7 +338,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         // one's are used on.
         int my_page = -1, my_row = 0;
         auto look_up = [&](int i0) __attribute__((always_inline)) {
-            const int key = (step0 + i0 + (lane >> 1)) * kStep + wave * kWaveKeys + (lane & 1) * 16;
+            const int key = (step0 + i0 + (lane >> 1)) * kNarrowStep + wave * kWaveKeys + (lane & 1) * 16;
             const int entry = key / p.c.page_size;
             my_page = i0 + (lane >> 1) < n && key < at.visible ? p.c.page_of(at.b, entry) : -1;
             my_row = key - entry * p.c.page_size;
@@ -353,7 +370,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 for (int g = 0; g < 2; ++g) load(v[g], 1, i, g);
             }
             const bool more = i + 1 < n && (i & 31) != 31;
-            const int key0 = (step0 + i) * kStep + wave * kWaveKeys;
+            const int key0 = (step0 + i) * kNarrowStep + wave * kWaveKeys;
             const bool hole[2] = {__builtin_amdgcn_readlane(my_page, 2 * (i & 31)) < 0,
                                   __builtin_amdgcn_readlane(my_page, 2 * (i & 31) + 1) < 0};
             const bool masked = key0 + kWaveKeys - 1 > kfull || hole[0] || hole[1];
@@ -424,8 +441,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], mul, -st[nr].m));
                 st[nr].l += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-                pf[nr] = prob_frag(y);
-                pr[nr] = prob_rest(y, pf[nr]);
+                pf[nr] = row_probs(y);
+                pr[nr] = row_rests(y, pf[nr]);
             }
             // O^T += V^T P^T
 #pragma unroll
@@ -437,30 +454,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                     st[nr].o[dt] = mfma16(vf, pr[nr], st[nr].o[dt]);
                 }
             }
-            if (__any(bad[0] || bad[1])) {
-                // ones in the places of NaN, times ones for the keys that a row sees
+            // what is NaN in V reaches the rows that see it
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const __bf16 one = (__bf16)(bad[g] ? 1.0f : 0.0f);
-                    const bf16x8_t marks = {one, one, one, one, one, one, one, one};
+            for (int g = 0; g < 2; ++g)
+                for (uint64_t m = __ballot(bad[g]); m != 0; m &= m - 1) {
+                    const int l = __builtin_ctzll(m), key = key0 + 16 * g + (l & 15), part = l >> 4;  // of the head, in four
 #pragma unroll
-                    for (int c = 0; c < kC; ++c) *reinterpret_cast<bf16x8_t*>(v_write + v_at<HD>(16 * g, c)) = marks;
+                    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                        for (int dt = 0; dt < kD; ++dt)
+                            if (key <= klast[nr] && dt / (kD / 4) == part)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) st[nr].o[dt][r] = __builtin_nanf("");
                 }
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr) {
-                    bf16x8_t sees;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        sees[e] = (__bf16)(key0 + 16 * (e >> 2) + 4 * quarter + (e & 3) > klast[nr] ? 0.0f : 1.0f);
-#pragma unroll
-                    for (int dt = 0; dt < kD; ++dt) {
-                        const f32x4_t hit = mfma16(value_frag(dt), sees, (f32x4_t){});
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (hit[r] != 0.0f) st[nr].o[dt][r] = __builtin_nanf("");
-                    }
-                }
-            }
         }
 
         // ---- the waves' shares of each row
@@ -501,40 +507,283 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             }
         }
         __syncthreads();
-        if (tid == 0 && x + n == x1) {
-            int4 cut = make_int4(0, 0, 0, -1);
-            if (begins && !ends) {
-                // the block with the unit's last step: the first whose stretch ends behind it
-                const int64_t end = x + steps;
-                cut = make_int4((int)place, (int)(place >> 32), kvh, (int)((end * blocks + all - 1) / all - 1));
+        line.write_cut(p, blockIdx.x, n, steps);
+        line.advance(p, n, steps);
+    }
+}
+
+// ---- many rows ----------------------------------------------------------------------
+//
+// A block has 128 rows, each wave 32 of them (or 64 rows, two waves sharing a row
+// and halving each tile's keys), on v_mfma_f32_32x32x16 (row_state.hpp).  All waves share
+// tiles of 64 keys, which they turn into BF16 rows in LDS, each wave 16 keys, a tile
+// ahead; the codes of the tile behind that are in flight meanwhile.
+
+// Rows of K are read 16 rows at a time, 16 bytes of each, rows of V transposed, four rows by
+// 64 bytes: 16 bytes lie between rows of K, 64 between those of V and 16 more between
+// groups of four, so that the reads and the writes (16 rows of one chunk) fall on different
+// columns of 256 bytes.
+template <int MODE, int HD, int ROWS, bool BF>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_wide_kernel(PagedParams p) {
+    constexpr int kC = HD / 16, kD = HD / 32, kW = HD / 32;      // kW: words of codes of a lane
+    constexpr int NT = ROWS == 128 ? 2 : 1;                      // 32-key accumulators of a wave
+    constexpr uint32_t kRowK = HD * 2 + 16, kRowV = HD * 2 + 64;
+    constexpr uint32_t kTileK = kWideStep * kRowK, kTileV = kWideStep * kRowV + kWideStep / 4 * 16;
+    constexpr uint32_t kSlot = kTileK + kTileV, kRegion = 32 * (HD * 4 + 16);
+    constexpr uint32_t kLds = 2 * kSlot > 4 * kRegion ? 2 * kSlot : 4 * kRegion;
+    __shared__ __align__(1024) unsigned char smem[kLds];
+    __shared__ float2 sml[4][32];
+    __shared__ uint8_t marks[2][kWideStep];  // blocks of V that are NaN, where some row does not see all keys
+    __shared__ int marked[2];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int h = lane >> 5, c32 = lane & 31, c16 = lane & 15, quarter = lane >> 4;
+    // neighbours on the line share keys: they go to one XCD, whose L2 holds them
+    const int64_t each_xcd = gridDim.x / 8;
+    const int64_t block = gridDim.x % 8 == 0 ? blockIdx.x % 8 * each_xcd + blockIdx.x / 8 : blockIdx.x;
+    Stretch<ROWS, kWideStep> line;
+    if (!line.find(p, block)) return;
+
+    ScoreConsts consts;
+    consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
+    consts.scale = p.scale;
+    consts.cap = p.cap;
+    consts.inv_cap = 1.0f / p.cap;
+    if constexpr (MODE == kAttnSoftcapD4)
+#pragma unroll
+        for (int i = 1; i <= SoftcapConsts::T::P.deg; ++i) consts.tanh[i] = bf16_value(SoftcapConsts::T::P.c[i]);
+
+    const int rbase = ROWS == 128 ? wave * 32 : (wave & 1) * 32;  // the wave's rows in the block
+    const int koff = ROWS == 128 ? 0 : (wave >> 1) * 32;          // and keys in a tile
+    while (line.x < line.x1) {
+        const Place<ROWS, kWideStep> at(p, line.place);
+        const int steps = at.steps(), step0 = line.step0, kvh = line.kvh;
+        const int n = line.x1 - line.x < steps - step0 ? (int)(line.x1 - line.x) : steps - step0;
+
+        // ---- staging: the wave's 16 keys of a tile.  Lane 4 i + g knows the page of group g
+        // of step i, 16 steps at a time.
+        int my_page = -1, my_row = 0;
+        uint32_t ahead_holes = 0;  // of the tile whose codes are in flight
+        Codes<HD> ck, cv;
+        const uint32_t lane_code = (uint32_t)(c16 * (HD / 2) + quarter * (HD / 8));
+        const uint32_t lane_byte = (uint32_t)(p.c.page_size * (HD / 2) + c16 * (HD / kFp4Block) + quarter * (HD / 4) / kFp4Block);
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            if ((i & 15) == 0) {
+                const int key = (step0 + i + (lane >> 2)) * kWideStep + (lane & 3) * 16;
+                const int entry = key / p.c.page_size;
+                my_page = i + (lane >> 2) < n && key < at.visible ? p.c.page_of(at.b, entry) : -1;
+                my_row = key - entry * p.c.page_size;
             }
-            p.cut[blockIdx.x] = cut;
+            ahead_holes = (uint32_t)(__ballot(my_page < 0) >> (4 * (i & 15))) & 15;
+            const int l = 4 * (i & 15) + wave;
+            const int page = __builtin_amdgcn_readlane(my_page, l), row = __builtin_amdgcn_readlane(my_row, l);
+            if (page < 0) {
+                ck.clear();
+                cv.clear();
+            } else {
+                const uint32_t code = (uint32_t)row * (HD / 2) + lane_code, byte = (uint32_t)row * (HD / kFp4Block) + lane_byte;
+                ck.load(p.c.head(page, 0, kvh), code, byte);
+                cv.load(p.c.head(page, 1, kvh), code, byte);
+            }
+        };
+        const int kfull = at.keys_of(p, at.r0 / p.group) - 1;  // every row sees the keys up to it
+        const int key16 = wave * 16 + c16;
+        // the tile in flight to slot i % 2
+        auto stage = [&](int i) __attribute__((always_inline)) {
+            unsigned char* slot = smem + (i & 1) * kSlot;
+            const bool masked = (step0 + i + 1) * kWideStep - 1 > kfull || ahead_holes != 0;
+            if (masked) {  // blocks of V that are NaN are zeros (0 * NaN is NaN), and marked
+                const bool bad = cv.byte > (uint32_t)kFp4Most;
+                const uint64_t any = __ballot(bad);
+                if (bad) cv.clear();
+                if (any != 0) {
+                    if (quarter == 0) {
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) m |= (uint32_t)(any >> (16 * q + c16) & 1) << (q * kD / 4);
+                        marks[i & 1][key16] = (uint8_t)m;
+                    }
+                    if (lane == 0) marked[i & 1] = 1;
+                } else if (quarter == 0) marks[i & 1][key16] = 0;
+            }
+            const float sk = fp4_scale(ck.byte), sv = fp4_scale(cv.byte);
+            unsigned char* k = slot + key16 * kRowK + quarter * kW * 16;
+            unsigned char* v = slot + kTileK + key16 * kRowV + (key16 >> 2) * 16 + quarter * kW * 16;
+#pragma unroll
+            for (int c = 0; c < kW; ++c) *reinterpret_cast<bf16x8_t*>(k + c * 16) = fp4_to_bf16(ck.w[c], sk);
+#pragma unroll
+            for (int c = 0; c < kW; ++c) *reinterpret_cast<bf16x8_t*>(v + c * 16) = fp4_to_bf16(cv.w[c], sv);
+        };
+        fetch(0);
+
+        // ---- Q^T fragments: columns 16 c + 8 h .. of row c32
+        const int row = rbase + c32;
+        const bool rin = row < at.nrows;
+        const int t = (at.r0 + (rin ? row : 0)) / p.group;
+        const int klast = (rin ? at.keys_of(p, t) : at.visible) - 1;  // the last key that the lane's row sees
+        const uint16_t* src = p.q + at.b * p.qs.b + t * p.qs.s + (kvh * p.group + (at.r0 + (rin ? row : 0) - t * p.group)) * p.qs.h;
+        bf16x8_t qf[kC], ql[BF ? 1 : kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            bf16x8_t f = {};
+            if (rin) f = *reinterpret_cast<const bf16x8_t*>(src + 16 * c + 8 * h);
+            if constexpr (!BF) split_fp16(f, qf[c], ql[c]);
+            else qf[c] = f;
         }
-        x += n;
-        step0 = 0;
-        if (ends && ++place == p.places) {
-            place = 0;
-            ++kvh;
+        RowState<HD> st;
+        __syncthreads();  // the tiles and marks of the unit before are read
+        if (tid < 2) marked[tid] = 0;
+        __syncthreads();
+        uint32_t holes = ahead_holes;
+        stage(0);
+        if (n > 1) fetch(1);
+        __syncthreads();
+        for (int i = 0; i < n; ++i) {
+            const unsigned char* ks = smem + (i & 1) * kSlot + (koff + c32) * kRowK + h * 16;
+            // transposing reads: row 4 h + (l % 16) / 4, columns 16 ((l / 16) % 2) + 4 (l % 4)
+            const int tr = koff + 4 * h + (c16 >> 2);
+            const unsigned char* vs = smem + (i & 1) * kSlot + kTileK + tr * kRowV + (tr >> 2) * 16 + (quarter & 1) * 32 + (lane & 3) * 8;
+            const int key0 = (step0 + i) * kWideStep;
+            const bool masked = key0 + kWideStep - 1 > kfull || holes != 0;
+            constexpr int kTerms = BF ? 1 : 2;  // products a fragment of K or V
+            f32x16_t s[NT];
+            // fragments of K are read six ahead of their products
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt) {
+                    const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(ks + kt * 32 * kRowK + c * 32);
+                    s[kt] = mfma32(kf, qf[c], s[kt]);
+                    if constexpr (!BF) s[kt] = mfma32(kf, ql[c], s[kt]);
+                }
+            constexpr int kReads = NT * kC, kAhead = kReads < 6 ? kReads : 6;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+            for (int g = 0; g < kReads - kAhead; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x008, kTerms, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kTerms, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!attn_is_plain_softmax(MODE)) {
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt) {
+                    float x[16];
+                    softmax_exponents<MODE>(s[kt], consts, x);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kt][r] = x[r];
+                }
+            }
+            if (masked) {  // keys of accumulator kt: 32 kt + 8 (r / 4) + 4 h + r % 4
+                const int diag = key0 + koff + 4 * h - klast;
+#pragma unroll
+                for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (diag + kt * 32 + 8 * (r >> 2) + (r & 3) > 0 || (holes >> (koff / 16 + 2 * kt + (r >> 3)) & 1))
+                            s[kt][r] = -__builtin_inff();
+            }
+            const float mul = score_state<kAttnSoftmaxNative, HD, true, NT, false>(s, st, consts, 0);
+            score_exps<HD, NT>(s, st, mul);
+            // fragments of V (two reads each) three ahead
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < 2 * NT; ++g) {
+                const bf16x8_t pf = prob_frag<true>(s[g >> 1], g & 1);
+                bf16x8_t rest;
+                if constexpr (!BF) rest = prob_rest<true>(s[g >> 1], g & 1, pf);
+#pragma unroll
+                for (int dt = 0; dt < kD; ++dt) {
+                    const uint16_t* vp = reinterpret_cast<const uint16_t*>(vs + g * (16 * kRowV + 64) + dt * 64);
+                    const u32x2_t lo = __builtin_bit_cast(u32x2_t, lds_read_tr16(vp));
+                    const u32x2_t hi = __builtin_bit_cast(u32x2_t, lds_read_tr16(vp + (8 * kRowV + 32) / 2));
+                    const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, (u32x4_t){lo.x, lo.y, hi.x, hi.y});
+                    st.o[dt] = mfma32(vf, pf, st.o[dt]);
+                    if constexpr (!BF) st.o[dt] = mfma32(vf, rest, st.o[dt]);
+                }
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+            for (int g = 0; g < 2 * NT * kD - 3; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x008, kTerms, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 3 * kTerms, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (masked && marked[i & 1] != 0)
+                for (int key = koff; key < koff + 32 * NT; ++key) {
+                    const uint32_t m = marks[i & 1][key];
+#pragma unroll
+                    for (int dt = 0; dt < kD; ++dt)
+                        if ((m >> dt & 1) && key0 + key <= klast)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) st.o[dt][r] = __builtin_nanf("");
+                }
+            if (i + 1 < n) {
+                holes = ahead_holes;
+                stage(i + 1);
+                if (i + 2 < n) fetch(i + 2);
+            }
+            __syncthreads();
         }
+
+        // ---- the rows: whole ones through LDS
+        unsigned char* region = smem + wave * kRegion;
+#pragma unroll
+        for (int dt = 0; dt < kD; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4_t*>(region + o_at<HD>(c32, dt * 8 + 2 * g + h)) =
+                    (f32x4_t){st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]};
+        const float l = half_sum(st.l);
+        if (h == 0) sml[wave][c32] = make_float2(st.m, l);
+        __syncthreads();
+        const bool begins = step0 == 0, ends = step0 + n == steps;
+        const int64_t slot = 2 * block + (begins ? 1 : 0);
+        constexpr int kChunks = HD / 4;
+        for (int i = tid; i < at.nrows * kChunks; i += 256) {
+            const int orow = i / kChunks, chunk = i % kChunks, w = orow >> 5, r = orow & 31;
+            float2 ml = sml[w][r];
+            f32x4_t o = *reinterpret_cast<const f32x4_t*>(smem + w * kRegion + o_at<HD>(r, chunk));
+            if constexpr (ROWS == 64) {
+                const float2 y = sml[w + 2][r];
+                const float top = __builtin_fmaxf(ml.x, y.x);
+                const float a = __builtin_amdgcn_exp2f(ml.x - top), a2 = __builtin_amdgcn_exp2f(y.x - top);
+                o = o * a + *reinterpret_cast<const f32x4_t*>(smem + (w + 2) * kRegion + o_at<HD>(r, chunk)) * a2;
+                ml = make_float2(top, __builtin_fmaf(ml.y, a, y.y * a2));
+            }
+            if (begins && ends) {
+                write_row<HD, BF>(p, at.b, at.r0 + orow, kvh, chunk, o, ml);
+            } else {
+                *reinterpret_cast<f32x4_t*>(p.part_o + (slot * ROWS + orow) * HD + chunk * 4) = o;
+                if (chunk == 0) p.part_ml[slot * ROWS + orow] = ml;
+            }
+        }
+        line.write_cut(p, block, n, steps);
+        line.advance(p, n, steps);
     }
 }
 
 // Joins the pieces of the unit that leaves block blockIdx.x unfinished.  HD / 4 lanes
 // hold a row, and the groups of them beyond the rows take the pieces in turn.
-template <int HD, int NR, bool BF>
+template <int HD, int ROWS, int STEP, bool BF>
 __global__ void __launch_bounds__(1024) paged_join_kernel(PagedParams p) {
-    constexpr int ROWS = 16 * NR, kChunks = HD / 4, kSlots = 1024 / kChunks;
+    constexpr int kChunks = HD / 4, kSlots = 1024 / kChunks;
     const int4 cut = p.cut[blockIdx.x];
     if (cut.w < 0) return;
     const int64_t place = ((int64_t)cut.y << 32) | (uint32_t)cut.x;
-    const Place<ROWS> at(p, place);
+    const Place<ROWS, STEP> at(p, place);
     const int pieces = cut.w - (int)blockIdx.x + 1;
+    // blocks of y have kSlots rows each
+    const int row_base = (int)blockIdx.y * kSlots, rows = at.nrows - row_base < kSlots ? at.nrows - row_base : kSlots;
+    if (rows <= 0) return;
     int span = 1;  // row slots: a power of two that holds the rows
-    while (span < at.nrows) span *= 2;
-    static_assert(ROWS <= kSlots, "a slot for every row");
+    while (span < rows) span *= 2;
     const int shares = kSlots / span;
     const int chunk = threadIdx.x % kChunks, s = threadIdx.x / kChunks;
-    const int row = s % span, share = s / span;
+    const int share = s / span, row = s % span < rows ? row_base + s % span : at.nrows;
     float m = kEmptyMax, l = 0.0f;
     f32x4_t o = (f32x4_t){};
     auto add = [&](float m2, float l2, f32x4_t o2) {
@@ -584,7 +833,7 @@ constexpr int64_t kMaxBlocks = 0xffffffffll / 256;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct PagedPlan {
-    int nr;          // row tiles of 16
+    int rows;        // of a tile
     int64_t blocks;  // a fixed number: the device divides the keys among them
     int64_t bytes;   // of the workspace
 };
@@ -593,18 +842,28 @@ bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, Page
     if (!a || !fp4_sizes_ok(c, a->tokens) || a->q_heads <= 0 || a->q_heads > 65536 || a->q_heads % c->kv_heads != 0)
         return false;
     const int64_t rows = a->tokens * (a->q_heads / c->kv_heads);
-    p.nr = rows <= 16 ? 1 : 2;
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.blocks = device_shape().cus * 2;
-    const int64_t tiles = ceil_div(rows, 16 * p.nr);
+    const int64_t tiles = ceil_div(rows, p.rows);
     if (c->batch > (int64_t(1) << 31) / (tiles ? tiles : 1)) return false;
-    p.bytes = p.blocks * (16 + 2 * 16 * p.nr * (c->head_dim + 2) * 4);
+    p.bytes = p.blocks * (16 + 2 * p.rows * (c->head_dim + 2) * 4);
     return true;
 }
 
-template <int MODE, int HD, int NR, bool BF>
+template <int MODE, int HD, int ROWS, bool BF>
 void go(const PagedParams& p, int64_t blocks, hipStream_t st) {
-    hipLaunchKernelGGL((paged_fp4_kernel<MODE, HD, NR, BF>), dim3((unsigned)blocks), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((paged_join_kernel<HD, NR, BF>), dim3((unsigned)blocks), dim3(1024), 0, st, p);
+    constexpr int STEP = ROWS <= 32 ? kNarrowStep : kWideStep;
+    const dim3 grid((unsigned)blocks), join((unsigned)blocks, (unsigned)ceil_div(ROWS, 1024 / (HD / 4)));
+    if constexpr (ROWS <= 32) hipLaunchKernelGGL((paged_narrow_kernel<MODE, HD, ROWS / 16, BF>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_wide_kernel<MODE, HD, ROWS, BF>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((paged_join_kernel<HD, ROWS, STEP, BF>), join, dim3(1024), 0, st, p);
+}
+template <int MODE, int HD, bool BF>
+void go(const PagedParams& p, const PagedPlan& plan, hipStream_t st) {
+    if (plan.rows == 16) go<MODE, HD, 16, BF>(p, plan.blocks, st);
+    else if (plan.rows == 32) go<MODE, HD, 32, BF>(p, plan.blocks, st);
+    else if (plan.rows == 64) go<MODE, HD, 64, BF>(p, plan.blocks, st);
+    else go<MODE, HD, 128, BF>(p, plan.blocks, st);
 }
 
 template <bool BF>
@@ -623,7 +882,7 @@ int run(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, void* 
     p.q = static_cast<const uint16_t*>(a->q);
     p.c = fp4_pages(c);
     p.qs = {a->q_strides[0], a->q_strides[2], a->q_strides[1]};
-    const int64_t rows = plan_.blocks * 2 * 16 * plan_.nr;
+    const int64_t rows = plan_.blocks * 2 * plan_.rows;
     p.part_o = static_cast<float*>(a->workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * c->head_dim);
     p.cut = reinterpret_cast<int4*>(p.part_ml + rows);
@@ -633,7 +892,7 @@ int run(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, void* 
     p.group = (int)(a->q_heads / c->kv_heads);
     p.tokens = (int)a->tokens;
     p.rows = p.tokens * p.group;
-    p.tiles = (int)ceil_div(p.rows, 16 * plan_.nr);
+    p.tiles = (int)ceil_div(p.rows, plan_.rows);
     p.capacity = p.c.entries * p.c.page_size;
     p.places = c->batch * p.tiles;
     p.scale = a->scale;
@@ -641,8 +900,8 @@ int run(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, void* 
     const hipStream_t st = hs(stream);
     auto shape = [&](auto mode) {
         constexpr int MODE = decltype(mode)::value;
-        if (c->head_dim == 128) plan_.nr == 1 ? go<MODE, 128, 1, BF>(p, plan_.blocks, st) : go<MODE, 128, 2, BF>(p, plan_.blocks, st);
-        else plan_.nr == 1 ? go<MODE, 64, 1, BF>(p, plan_.blocks, st) : go<MODE, 64, 2, BF>(p, plan_.blocks, st);
+        if (c->head_dim == 128) go<MODE, 128, BF>(p, plan_, st);
+        else go<MODE, 64, BF>(p, plan_, st);
     };
     if (a->mode == kAttnSoftmaxNative) shape(std::integral_constant<int, kAttnSoftmaxNative>{});
     else if (a->mode == kAttnSoftcapNative) shape(std::integral_constant<int, kAttnSoftcapNative>{});

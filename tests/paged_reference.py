@@ -66,15 +66,17 @@ def attention(q, cache, table, lens, scale, cap=0.0):
     Keys and values are exact in the products, as are queries.  A score is a sum of D products in
     FP32 (2 D for FP16 queries, which are two terms): off by at most 2 D 2^-24 sum |q k| scale, with a
     softcap 4e-7 cap more (its tanh is within 2^-21 of 1); 1e-5 covers the exponent's rounding and
-    its instruction: d in all.  A probability in two BF16 terms is off by 2^-16 of itself, and the sums
-    over n keys by n 2^-23, twice that with the join of parts.  So an output is off by (2^-16 + 2 d + n 2^-22)
-    sum p |v| and half a step of its type, lse by d + n 2^-22 + 1e-6 |lse|."""
+    its instruction: d in all.  A probability in two BF16 terms is off by r = 2^-8 2^-8 of itself; BF16
+    queries with more than 32 rows to a KV head (T Hq / Hkv) have one term, r = 2^-8, half a step.  The
+    sums over n keys are off by n 2^-23, twice that with the join of parts.  So an output is off by
+    (r + 2 d + n 2^-22) sum p |v| and half a step of its type, lse by d + n 2^-22 + 1e-6 |lse|."""
     b, t, hq, d = q.shape
     u = torch.finfo(q.dtype).eps / 2
     least = torch.finfo(q.dtype).smallest_normal * u  # half a step of what is not normal
     out, tol_o = (torch.zeros(b, t, hq, d, dtype=torch.float64) for _ in range(2))
     lse, tol_l = torch.full((b, hq, t), -math.inf, dtype=torch.float64), torch.zeros(b, hq, t, dtype=torch.float64)
     group = hq // cache.shape[2]
+    r = 2.0 ** -8 if q.dtype == torch.bfloat16 and t * group > 32 else 2.0 ** -16
     for i in range(b):
         k, v, there = sequence(cache, d, table[i].tolist(), lens[i])
         for j in range(t):
@@ -93,7 +95,7 @@ def attention(q, cache, table, lens, scale, cap=0.0):
             out[i, j] = (p[..., None] * vv).sum(0)
             lse[i, :, j] = z
             size = (p[..., None] * vv.abs()).sum(0)
-            tol_o[i, j] = (2.0 ** -16 + 2 * err + c * 2.0 ** -22)[:, None] * size + out[i, j].abs() * u * 1.01 + least
+            tol_o[i, j] = (r + 2 * err + c * 2.0 ** -22)[:, None] * size + out[i, j].abs() * u * 1.01 + least
             tol_l[i, :, j] = err + c * 2.0 ** -22 + 1e-6 * z.abs()
     return out, lse, tol_o, tol_l
 
