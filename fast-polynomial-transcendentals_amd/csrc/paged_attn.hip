@@ -33,6 +33,8 @@ namespace pt {
 constexpr int kNarrowStep = 128;  // keys of a narrow block's step
 constexpr int kWaveKeys = 32;     // of which a wave has 32
 constexpr int kWideStep = 64;
+// A unit's first keys and its result cost as much as so many steps more.
+constexpr int unit_steps(int step) { return step == kWideStep ? 4 : 2; }
 
 struct PagedParams {
     const uint16_t* q;
@@ -40,11 +42,11 @@ struct PagedParams {
     AttnStrides qs;
     float* part_o;    // [2 blocks][ROWS][HD]
     float2* part_ml;  // [2 blocks][ROWS]
-    int4* cut;        // [blocks] the unit that leaves a block unfinished: place, head, last block
+    int4* cut;        // [blocks] the unit that leaves a block unfinished: place, head, pieces (0: none), first row
     void* out;
     float* lse;
     int hq, group, tokens, rows, tiles, capacity;
-    int64_t places;  // batch * tiles
+    int places;  // batch * tiles
     float scale, cap;
 };
 
@@ -52,10 +54,17 @@ __device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// x of lane l ^ 16 and of l ^ 32 combined with this lane's.
-__device__ __forceinline__ float row_max(float x) {
+// Over the lanes of a row (l ^ 16 and l ^ 32): the largest of eight scores, NaN if one is
+// (v_maximum3_f32: no instructions that quiet its operands), and a sum.
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float row_max(const float (&y)[8]) {
+    float x = maximum(maximum(maximum(y[0], y[1]), y[2]), y[3]);
+    x = maximum(maximum(x, y[4]), y[5]);
+    x = maximum(maximum(x, y[6]), y[7]);
     const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
-    return half_max(__builtin_fmaxf(as_f32(r[0]), as_f32(r[1])));
+    x = maximum(as_f32(r[0]), as_f32(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+    return maximum(as_f32(t[0]), as_f32(t[1]));
 }
 __device__ __forceinline__ float row_sum(float x) {
     const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
@@ -67,14 +76,14 @@ __device__ __forceinline__ float row_sum(float x) {
 // A row tile of a sequence.
 template <int ROWS, int STEP>
 struct Place {
-    int64_t b;
+    int b;
     int r0, nrows;  // rows of the sequence
     int seen;       // keys that token 0 sees (token t: t more), not held to the table
     int visible;    // keys that the tile's last row sees
 
-    __device__ __forceinline__ Place(const PagedParams& p, int64_t place) {
+    __device__ __forceinline__ Place(const PagedParams& p, int place) {
         b = place / p.tiles;
-        r0 = (int)(place - b * p.tiles) * ROWS;
+        r0 = (place - b * p.tiles) * ROWS;
         nrows = p.rows - r0 < ROWS ? p.rows - r0 : ROWS;
         seen = p.c.len(b) - p.tokens + 1;
         visible = keys_of(p, (r0 + nrows - 1) / p.group);
@@ -86,27 +95,31 @@ struct Place {
     }
     // One at least: a tile without keys leaves zeros.
     __device__ __forceinline__ int steps() const { return visible <= STEP ? 1 : (visible + STEP - 1) / STEP; }
+    // On the line.
+    __device__ __forceinline__ int length() const { return steps() + unit_steps(STEP); }
 };
 
-// A block's stretch of the line: from step0 of a place and KV head on, x of all steps, to x1.
+// A block's stretch of the line: x to x1 of all steps (fewer than 2^31), from `in` of a
+// place and KV head on.  The first `longer` blocks have each + 1 steps, the others each.
 template <int ROWS, int STEP>
 struct Stretch {
     using At = Place<ROWS, STEP>;
-    int64_t all, blocks, x, x1, place;
-    int kvh, step0;
+    static constexpr int kUnit = unit_steps(STEP);
+    int each, longer, x, x1, place, kvh, in;
 
     // False: none (and the block's cut says so).  block: its number on the line.
-    __device__ __forceinline__ bool find(const PagedParams& p, int64_t block) {
-        __shared__ int64_t sums[4], start[2];
+    __device__ __forceinline__ bool find(const PagedParams& p, int block) {
+        __shared__ int sums[4], start[2];
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-        const int64_t each = (p.places + 255) / 256;
-        const int64_t from = tid * each, to = from + each < p.places ? from + each : p.places;
-        int64_t mine = 0, plane = 0, ahead = 0;  // steps of the thread's places, of a KV head, ahead
-        for (int64_t i = from; i < to; ++i) mine += At(p, i).steps();
-        int64_t inc = mine;
+        const int per = (p.places + 255) / 256;
+        const int64_t first = (int64_t)tid * per;
+        const int from = first < p.places ? (int)first : p.places, to = p.places - from < per ? p.places : from + per;
+        int mine = 0, plane = 0, ahead = 0;  // steps of the thread's places, of a KV head, ahead
+        for (int i = from; i < to; ++i) mine += At(p, i).length();
+        int inc = mine;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const int64_t y = __shfl_up(inc, d);
+            const int y = __shfl_up(inc, d);
             inc += lane >= d ? y : 0;
         }
         if (lane == 63) sums[wave] = inc;
@@ -117,47 +130,54 @@ struct Stretch {
             plane += sums[w];
         }
         ahead += inc - mine;
-        all = plane * p.c.hkv;
-        blocks = all < gridDim.x ? all : gridDim.x;  // with a step at least
-        if (block >= blocks) {
-            if (tid == 0) p.cut[block] = make_int4(0, 0, 0, -1);
+        const int all = plane * p.c.hkv;
+        each = all / (int)gridDim.x;
+        longer = all - each * (int)gridDim.x;
+        x = block * each + (block < longer ? block : longer);
+        x1 = x + each + (block < longer ? 1 : 0);
+        if (x == x1) {
+            if (tid == 0) p.cut[block] = make_int4(0, 0, 0, 0);
             return false;
         }
-        x = block * all / blocks;
-        x1 = (block + 1) * all / blocks;
-        kvh = (int)(x / plane);
-        const int64_t in = x - kvh * plane;
-        if (in >= ahead && in < ahead + mine)
-            for (int64_t i = from; i < to; ++i) {
-                const int n = At(p, i).steps();
-                if (in < ahead + n) {
+        kvh = x / plane;
+        const int at = x - kvh * plane;
+        if (at >= ahead && at < ahead + mine)
+            for (int i = from; i < to; ++i) {
+                const int n = At(p, i).length();
+                if (at < ahead + n) {
                     start[0] = i;
-                    start[1] = in - ahead;
+                    start[1] = at - ahead;
                     break;
                 }
                 ahead += n;
             }
         __syncthreads();
         place = start[0];
-        step0 = (int)start[1];
+        in = start[1];
         return true;
     }
-    // What a block leaves unfinished behind n more steps of a unit.
-    __device__ __forceinline__ void write_cut(const PagedParams& p, int64_t block, int n, int steps) const {
-        if (threadIdx.x != 0 || x + n != x1) return;
-        int4 cut = make_int4(0, 0, 0, -1);
-        if (step0 == 0 && n < steps) {
-            // the block with the unit's last step: the first whose stretch ends behind it
-            const int64_t end = x + steps;
-            cut = make_int4((int)place, (int)(place >> 32), kvh, (int)((end * blocks + all - 1) / all - 1));
-        }
-        p.cut[block] = cut;
+    // The block's steps of the unit that it is at: the first, and behind the last.
+    __device__ __forceinline__ int first() const { return in > kUnit ? in - kUnit : 0; }
+    __device__ __forceinline__ int last(int steps) const {
+        const int end = in + (x1 - x) - kUnit;
+        return end < 0 ? 0 : end < steps ? end : steps;
     }
-    __device__ __forceinline__ void advance(const PagedParams& p, int n, int steps) {
-        const bool ends = step0 + n == steps;
-        x += n;
-        step0 = 0;
-        if (ends && ++place == p.places) {
+    // Goes on behind a unit.  What the block leaves unfinished is its cut.
+    __device__ __forceinline__ void advance(const PagedParams& p, int block, const At& at) {
+        const int steps = at.steps(), end = x - in + steps + kUnit;  // of the unit
+        if (threadIdx.x == 0 && end >= x1) {
+            int4 cut = make_int4(0, 0, 0, 0);
+            if (first() == 0 && last(steps) > 0 && last(steps) < steps) {
+                // the block with the unit's last step
+                const int to = end - 1, many = longer * (each + 1);
+                const int stop = to < many ? to / (each + 1) : longer + (to - many) / each;
+                cut = make_int4(at.b, kvh, stop - block + 1, at.r0);
+            }
+            p.cut[block] = cut;
+        }
+        x = end;
+        in = 0;
+        if (++place == p.places) {
             place = 0;
             ++kvh;
         }
@@ -218,11 +238,11 @@ __device__ __forceinline__ constexpr uint32_t o_at(int row, int chunk) {
 
 // Elements 4 chunk .. of a row of a place, divided by their sum, to the result.
 template <int HD, bool BF>
-__device__ __forceinline__ void write_row(const PagedParams& p, int64_t b, int row, int kvh, int chunk, f32x4_t o,
+__device__ __forceinline__ void write_row(const PagedParams& p, int b, int row, int kvh, int chunk, f32x4_t o,
                                           float2 ml) {
     const float inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;  // a row that sees no key is zero
     const int t = row / p.group, head = kvh * p.group + (row - t * p.group);
-    const int64_t bt = b * p.tokens + t;
+    const int64_t bt = (int64_t)b * p.tokens + t;
     uint2 w;
     if constexpr (BF) {
         w = make_uint2(pack_bf(o[0] * inv, o[1] * inv), pack_bf(o[2] * inv, o[3] * inv));
@@ -232,7 +252,7 @@ __device__ __forceinline__ void write_row(const PagedParams& p, int64_t b, int r
     }
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (bt * p.hq + head) * HD + chunk * 4) = w;
     if (chunk == 0 && p.lse != nullptr)
-        p.lse[(b * p.hq + head) * p.tokens + t] =
+        p.lse[((int64_t)b * p.hq + head) * p.tokens + t] =
             ml.y == 0.0f ? -__builtin_inff() : (ml.x + __builtin_log2f(ml.y)) * kLn2;
 }
 
@@ -253,22 +273,27 @@ struct Codes {
     uint32_t w[HD / 32];
     uint32_t byte;
 
+    template <bool ONCE>
     __device__ __forceinline__ void load(const uint8_t* head, uint32_t code, uint32_t at) {
-        if constexpr (HD == 128) {
-            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(head + code);
+        typedef typename std::conditional<HD == 128, u32x4_t, u32x2_t>::type Words;
+        const Words* src = reinterpret_cast<const Words*>(head + code);
+        const Words a = ONCE ? __builtin_nontemporal_load(src) : *src;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = a[i];
-        } else {
-            const u32x2_t a = *reinterpret_cast<const u32x2_t*>(head + code);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) w[i] = a[i];
-        }
-        byte = head[at];
+        for (int i = 0; i < HD / 32; ++i) w[i] = a[i];
+        byte = ONCE ? __builtin_nontemporal_load(head + at) : head[at];
+    }
+    // Of page 0 where there is none (its keys are masked, its values cleared): a branch would
+    // have every wait for a load wait for all of them.
+    // ONCE: nobody else reads them.
+    template <bool ONCE>
+    __device__ __forceinline__ void load(const Fp4Pages& c, int page, int row, int kv, int h, uint32_t lane_code,
+                                         uint32_t lane_byte) {
+        load<ONCE>(c.head(page < 0 ? 0 : page, kv, h), (uint32_t)row * (HD / 2) + lane_code, (uint32_t)row * (HD / kFp4Block) + lane_byte);
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) w[i] = 0;
-        byte = 127;
+        byte = 0;
     }
 };
 
@@ -286,7 +311,7 @@ struct PagedState {
 
 // A block's stretch of the line, and what its waves need throughout.
 template <int MODE, int HD, int NR, bool BF>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? (HD == 64 ? 4 : 3) : BF || HD == 64 ? 2 : 1))) paged_narrow_kernel(PagedParams p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? (HD == 64 ? 4 : 3) : 2))) paged_narrow_kernel(PagedParams p) {
     constexpr int ROWS = 16 * NR, kC = HD / 32, kD = HD / 16;
     constexpr int kVTile = v_at<HD>(kWaveKeys, 0), kSpill = o_at<HD>(16, 0);
     constexpr int kRegion = kVTile > kSpill ? kVTile : kSpill;
@@ -309,8 +334,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
     unsigned char* vt = smem + wave * kRegion;
     while (line.x < line.x1) {
         const Place<ROWS, kNarrowStep> at(p, line.place);
-        const int steps = at.steps(), step0 = line.step0, kvh = line.kvh;
-        const int n = line.x1 - line.x < steps - step0 ? (int)(line.x1 - line.x) : steps - step0;
+        const int steps = at.steps(), step0 = line.first(), n = line.last(steps) - step0, kvh = line.kvh;
+        if (n == 0) {
+            line.advance(p, blockIdx.x, at);
+            break;
+        }
         // ---- Q^T fragments: elements (HD / 4) quarter + 8 c .. of row c16
         bf16x8_t qf[NR][kC], ql[BF ? 1 : NR][kC];
         int klast[NR];  // the last key that the lane's row sees
@@ -347,9 +375,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         const uint32_t lane_byte = (uint32_t)(p.c.page_size * (HD / 2) + c16 * (HD / kFp4Block) + quarter * (HD / 4) / kFp4Block);
         auto load = [&](Codes<HD>& codes, int kv, int i, int g) __attribute__((always_inline)) {
             const int l = 2 * (i & 31) + g;
-            const int page = __builtin_amdgcn_readlane(my_page, l), row = __builtin_amdgcn_readlane(my_row, l);
-            if (page < 0) codes.clear();
-            else codes.load(p.c.head(page, kv, kvh), (uint32_t)row * (HD / 2) + lane_code, (uint32_t)row * (HD / kFp4Block) + lane_byte);
+            codes.template load<true>(p.c, __builtin_amdgcn_readlane(my_page, l), __builtin_amdgcn_readlane(my_row, l), kv, kvh,
+                                      lane_code, lane_byte);
         };
         unsigned char* const v_write = vt + v_at<HD>(c16, quarter * kC);
         const unsigned char* const v_read = vt + v_at<HD>(4 * quarter + (c16 >> 2), (c16 & 3) >> 1) + (c16 & 1) * 8;
@@ -361,51 +388,56 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             return __builtin_bit_cast(bf16x8_t, (u32x4_t){lo.x, lo.y, hi.x, hi.y});
         };
         Codes<HD> k[2], v[2];
-        for (int i = 0; i < n; ++i) {
-            if ((i & 31) == 0) {
-                look_up(i);
+        const int tiles = p.c.pages > 0 ? n : 0;
+        if (tiles > 0) {
+            look_up(0);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) load(k[g], 0, i, g);
+            for (int g = 0; g < 2; ++g) load(k[g], 0, 0, g);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) load(v[g], 1, i, g);
-            }
-            const bool more = i + 1 < n && (i & 31) != 31;
+            for (int g = 0; g < 2; ++g) load(v[g], 1, 0, g);
+        }
+        for (int i = 0; i < tiles; ++i) {
             const int key0 = (step0 + i) * kNarrowStep + wave * kWaveKeys;
             const bool hole[2] = {__builtin_amdgcn_readlane(my_page, 2 * (i & 31)) < 0,
                                   __builtin_amdgcn_readlane(my_page, 2 * (i & 31) + 1) < 0};
             const bool masked = key0 + kWaveKeys - 1 > kfull || hole[0] || hole[1];
+            if ((i & 31) == 31) look_up(i + 1);  // no page behind the last tile
             f32x4_t s[2][NR];
+            const float scale[2] = {fp4_scale(k[0].byte), fp4_scale(k[1].byte)};
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const float scale = fp4_scale(k[g].byte);
+            for (int nr = 0; nr < NR; ++nr) s[0][nr] = s[1][nr] = (f32x4_t){};
 #pragma unroll
-                for (int nr = 0; nr < NR; ++nr) s[g][nr] = (f32x4_t){};
+            for (int c = 0; c < kC; ++c)
 #pragma unroll
-                for (int c = 0; c < kC; ++c) {
-                    const bf16x8_t kf = fp4_to_bf16(k[g].w[c], scale);
+                for (int g = 0; g < 2; ++g) {
+                    const bf16x8_t kf = fp4_to_bf16(k[g].w[c], scale[g]);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
                         s[g][nr] = mfma16(kf, qf[nr][c], s[g][nr]);
                         if constexpr (!BF) s[g][nr] = mfma16(kf, ql[nr][c], s[g][nr]);
                     }
                 }
-                if (more) load(k[g], 0, i + 1, g);
-            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) load(k[g], 0, i + 1, g);
             // V to LDS; in a tile with keys that some row does not see, blocks that are no
             // numbers as zeros (0 * NaN is NaN)
             bool bad[2] = {false, false};
+            if (masked)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    bad[g] = v[g].byte > (uint32_t)kFp4Most && !hole[g];
+                    if (bad[g] || hole[g]) v[g].clear();
+                }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                if (masked) {
-                    bad[g] = v[g].byte > (uint32_t)kFp4Most;
-                    if (bad[g]) v[g].clear();
-                }
                 const float scale = fp4_scale(v[g].byte);
 #pragma unroll
                 for (int c = 0; c < kC; ++c)
                     *reinterpret_cast<bf16x8_t*>(v_write + v_at<HD>(16 * g, c)) = fp4_to_bf16(v[g].w[c], scale);
-                if (more) load(v[g], 1, i + 1, g);
             }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) load(v[g], 1, i + 1, g);
+            __builtin_amdgcn_sched_barrier(0);
             // probabilities of keys 4 quarter + r of the first group, then of the second
             bf16x8_t pf[NR], pr[NR];
 #pragma unroll
@@ -419,9 +451,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                     for (int e = 0; e < 8; ++e)
                         if (hole[e >> 2] || key0 + 16 * (e >> 2) + 4 * quarter + (e & 3) > klast[nr]) y[e] = -__builtin_inff();
                 }
-                float mx = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y[0], y[1]), __builtin_fmaxf(y[2], y[3])),
-                                           __builtin_fmaxf(__builtin_fmaxf(y[4], y[5]), __builtin_fmaxf(y[6], y[7])));
-                mx = row_max(mx) * consts.sl;
+                const float mx = row_max(y) * consts.sl;
                 const bool move = mx - st[nr].m > 8.0f;  // the lanes of a row decide alike
                 if (__any(move)) {
                     const float m = move ? mx : st[nr].m;
@@ -444,15 +474,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 pf[nr] = row_probs(y);
                 pr[nr] = row_rests(y, pf[nr]);
             }
-            // O^T += V^T P^T
+            // O^T += V^T P^T, fragments of V three ahead
+            __builtin_amdgcn_sched_barrier(0);
+            bf16x8_t vf[kD];
+#pragma unroll
+            for (int dt = 0; dt < kD && dt < 3; ++dt) vf[dt] = value_frag(dt);
 #pragma unroll
             for (int dt = 0; dt < kD; ++dt) {
-                const bf16x8_t vf = value_frag(dt);
+                if (dt + 3 < kD) vf[dt + 3] = value_frag(dt + 3);
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
-                    st[nr].o[dt] = mfma16(vf, pf[nr], st[nr].o[dt]);
-                    st[nr].o[dt] = mfma16(vf, pr[nr], st[nr].o[dt]);
+                    st[nr].o[dt] = mfma16(vf[dt], pf[nr], st[nr].o[dt]);
+                    st[nr].o[dt] = mfma16(vf[dt], pr[nr], st[nr].o[dt]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             // what is NaN in V reaches the rows that see it
 #pragma unroll
@@ -471,7 +506,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 
         // ---- the waves' shares of each row
         const bool begins = step0 == 0, ends = step0 + n == steps;
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
+        const int slot = 2 * (int)blockIdx.x + (begins ? 1 : 0);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
             if (nr * 16 >= at.nrows) break;
@@ -501,14 +536,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 if (begins && ends) {
                     write_row<HD, BF>(p, at.b, at.r0 + nr * 16 + row, kvh, chunk, o, ml);
                 } else {
-                    *reinterpret_cast<f32x4_t*>(p.part_o + (slot * ROWS + nr * 16 + row) * HD + chunk * 4) = o;
+                    *reinterpret_cast<f32x4_t*>(p.part_o + (int64_t)(slot * ROWS + nr * 16 + row) * HD + chunk * 4) = o;
                     if (chunk == 0) p.part_ml[slot * ROWS + nr * 16 + row] = ml;
                 }
             }
         }
         __syncthreads();
-        line.write_cut(p, blockIdx.x, n, steps);
-        line.advance(p, n, steps);
+        line.advance(p, blockIdx.x, at);
     }
 }
 
@@ -538,13 +572,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int h = lane >> 5, c32 = lane & 31, c16 = lane & 15, quarter = lane >> 4;
     // neighbours on the line share keys: they go to one XCD, whose L2 holds them
-    const int64_t each_xcd = gridDim.x / 8;
-    const int64_t block = gridDim.x % 8 == 0 ? blockIdx.x % 8 * each_xcd + blockIdx.x / 8 : blockIdx.x;
+    const int block = (int)(gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x);
     Stretch<ROWS, kWideStep> line;
     if (!line.find(p, block)) return;
 
     ScoreConsts consts;
-    consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
+    consts.sl = vgpr(attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e);
     consts.scale = p.scale;
     consts.cap = p.cap;
     consts.inv_cap = 1.0f / p.cap;
@@ -556,8 +589,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     const int koff = ROWS == 128 ? 0 : (wave >> 1) * 32;          // and keys in a tile
     while (line.x < line.x1) {
         const Place<ROWS, kWideStep> at(p, line.place);
-        const int steps = at.steps(), step0 = line.step0, kvh = line.kvh;
-        const int n = line.x1 - line.x < steps - step0 ? (int)(line.x1 - line.x) : steps - step0;
+        const int steps = at.steps(), step0 = line.first(), n = line.last(steps) - step0, kvh = line.kvh;
+        if (n == 0) {
+            line.advance(p, block, at);
+            break;
+        }
 
         // ---- staging: the wave's 16 keys of a tile.  Lane 4 i + g knows the page of group g
         // of step i, 16 steps at a time.
@@ -576,14 +612,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             ahead_holes = (uint32_t)(__ballot(my_page < 0) >> (4 * (i & 15))) & 15;
             const int l = 4 * (i & 15) + wave;
             const int page = __builtin_amdgcn_readlane(my_page, l), row = __builtin_amdgcn_readlane(my_row, l);
-            if (page < 0) {
-                ck.clear();
-                cv.clear();
-            } else {
-                const uint32_t code = (uint32_t)row * (HD / 2) + lane_code, byte = (uint32_t)row * (HD / kFp4Block) + lane_byte;
-                ck.load(p.c.head(page, 0, kvh), code, byte);
-                cv.load(p.c.head(page, 1, kvh), code, byte);
-            }
+            ck.template load<false>(p.c, page, row, 0, kvh, lane_code, lane_byte);
+            cv.template load<false>(p.c, page, row, 1, kvh, lane_code, lane_byte);
         };
         const int kfull = at.keys_of(p, at.r0 / p.group) - 1;  // every row sees the keys up to it
         const int key16 = wave * 16 + c16;
@@ -592,9 +622,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             unsigned char* slot = smem + (i & 1) * kSlot;
             const bool masked = (step0 + i + 1) * kWideStep - 1 > kfull || ahead_holes != 0;
             if (masked) {  // blocks of V that are NaN are zeros (0 * NaN is NaN), and marked
-                const bool bad = cv.byte > (uint32_t)kFp4Most;
+                const bool hole = ahead_holes >> wave & 1, bad = cv.byte > (uint32_t)kFp4Most && !hole;
                 const uint64_t any = __ballot(bad);
-                if (bad) cv.clear();
+                if (bad || hole) cv.clear();
                 if (any != 0) {
                     if (quarter == 0) {
                         uint32_t m = 0;
@@ -613,7 +643,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
             for (int c = 0; c < kW; ++c) *reinterpret_cast<bf16x8_t*>(v + c * 16) = fp4_to_bf16(cv.w[c], sv);
         };
-        fetch(0);
+        const int tiles = p.c.pages > 0 ? n : 0;
+        if (tiles > 0) fetch(0);
 
         // ---- Q^T fragments: columns 16 c + 8 h .. of row c32
         const int row = rbase + c32;
@@ -634,10 +665,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         if (tid < 2) marked[tid] = 0;
         __syncthreads();
         uint32_t holes = ahead_holes;
-        stage(0);
-        if (n > 1) fetch(1);
+        if (tiles > 0) stage(0);
+        if (tiles > 1) fetch(1);
         __syncthreads();
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < tiles; ++i) {
             const unsigned char* ks = smem + (i & 1) * kSlot + (koff + c32) * kRowK + h * 16;
             // transposing reads: row 4 h + (l % 16) / 4, columns 16 ((l / 16) % 2) + 4 (l % 4)
             const int tr = koff + 4 * h + (c16 >> 2);
@@ -648,6 +679,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             f32x16_t s[NT];
             // fragments of K are read six ahead of their products
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kt = 0; kt < NT; ++kt) s[kt] = (f32x16_t){};
 #pragma unroll
@@ -667,6 +699,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             }
             __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kTerms, 0);
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             if constexpr (!attn_is_plain_softmax(MODE)) {
 #pragma unroll
                 for (int kt = 0; kt < NT; ++kt) {
@@ -689,6 +722,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             score_exps<HD, NT>(s, st, mul);
             // fragments of V (two reads each) three ahead
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int g = 0; g < 2 * NT; ++g) {
                 const bf16x8_t pf = prob_frag<true>(s[g >> 1], g & 1);
@@ -712,6 +746,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             }
             __builtin_amdgcn_sched_group_barrier(0x008, 3 * kTerms, 0);
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             if (masked && marked[i & 1] != 0)
                 for (int key = koff; key < koff + 32 * NT; ++key) {
                     const uint32_t m = marks[i & 1][key];
@@ -721,10 +756,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
                             for (int r = 0; r < 16; ++r) st.o[dt][r] = __builtin_nanf("");
                 }
-            if (i + 1 < n) {
+            if (i + 1 < tiles) {
                 holes = ahead_holes;
                 stage(i + 1);
-                if (i + 2 < n) fetch(i + 2);
+                if (i + 2 < tiles) fetch(i + 2);
             }
             __syncthreads();
         }
@@ -741,7 +776,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         if (h == 0) sml[wave][c32] = make_float2(st.m, l);
         __syncthreads();
         const bool begins = step0 == 0, ends = step0 + n == steps;
-        const int64_t slot = 2 * block + (begins ? 1 : 0);
+        const int slot = 2 * block + (begins ? 1 : 0);
         constexpr int kChunks = HD / 4;
         for (int i = tid; i < at.nrows * kChunks; i += 256) {
             const int orow = i / kChunks, chunk = i % kChunks, w = orow >> 5, r = orow & 31;
@@ -757,71 +792,73 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             if (begins && ends) {
                 write_row<HD, BF>(p, at.b, at.r0 + orow, kvh, chunk, o, ml);
             } else {
-                *reinterpret_cast<f32x4_t*>(p.part_o + (slot * ROWS + orow) * HD + chunk * 4) = o;
+                *reinterpret_cast<f32x4_t*>(p.part_o + (int64_t)(slot * ROWS + orow) * HD + chunk * 4) = o;
                 if (chunk == 0) p.part_ml[slot * ROWS + orow] = ml;
             }
         }
-        line.write_cut(p, block, n, steps);
-        line.advance(p, n, steps);
+        line.advance(p, block, at);
     }
 }
 
 // Joins the pieces of the unit that leaves block blockIdx.x unfinished.  HD / 4 lanes
 // hold a row, and the groups of them beyond the rows take the pieces in turn.
-template <int HD, int ROWS, int STEP, bool BF>
-__global__ void __launch_bounds__(1024) paged_join_kernel(PagedParams p) {
-    constexpr int kChunks = HD / 4, kSlots = 1024 / kChunks;
+template <int HD, int ROWS, bool BF>
+__global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
+    constexpr int kChunks = HD / 4, kSlots = 512 / kChunks;  // row slots
     const int4 cut = p.cut[blockIdx.x];
-    if (cut.w < 0) return;
-    const int64_t place = ((int64_t)cut.y << 32) | (uint32_t)cut.x;
-    const Place<ROWS, STEP> at(p, place);
-    const int pieces = cut.w - (int)blockIdx.x + 1;
-    // blocks of y have kSlots rows each
-    const int row_base = (int)blockIdx.y * kSlots, rows = at.nrows - row_base < kSlots ? at.nrows - row_base : kSlots;
-    if (rows <= 0) return;
-    int span = 1;  // row slots: a power of two that holds the rows
-    while (span < rows) span *= 2;
+    const int pieces = cut.z;
+    if (pieces == 0) return;
+    const int nrows = p.rows - cut.w < ROWS ? p.rows - cut.w : ROWS;
+    int span = 1;  // a power of two that holds the rows
+    while (span < nrows && span < kSlots) span *= 2;
     const int shares = kSlots / span;
-    const int chunk = threadIdx.x % kChunks, s = threadIdx.x / kChunks;
-    const int share = s / span, row = s % span < rows ? row_base + s % span : at.nrows;
-    float m = kEmptyMax, l = 0.0f;
-    f32x4_t o = (f32x4_t){};
-    auto add = [&](float m2, float l2, f32x4_t o2) {
-        const float top = __builtin_fmaxf(m, m2);
-        const float a = __builtin_amdgcn_exp2f(m - top), a2 = __builtin_amdgcn_exp2f(m2 - top);
-        l = __builtin_fmaf(l, a, l2 * a2);
-        o = o * a + o2 * a2;
-        m = top;
-    };
-    if (row < at.nrows) {
+    const int chunk = threadIdx.x % kChunks, s = threadIdx.x / kChunks, share = s / span;
+    __shared__ f32x4_t so[512];
+    __shared__ float2 sml[kSlots];
+    for (int row = s % span; row < nrows; row += kSlots) {  // more than once where all slots have a row
+        float m = kEmptyMax, l = 0.0f;
+        f32x4_t o = (f32x4_t){};
+        auto add = [&](float m2, float l2, f32x4_t o2) {
+            const float top = __builtin_fmaxf(m, m2);
+            const float a = __builtin_amdgcn_exp2f(m - top), a2 = __builtin_amdgcn_exp2f(m2 - top);
+            l = __builtin_fmaf(l, a, l2 * a2);
+            o = o * a + o2 * a2;
+            m = top;
+        };
         for (int i = share; i < pieces; i += 4 * shares) {
             float2 ml[4];
             f32x4_t part[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int j = i + u * shares < pieces ? i + u * shares : i;
-                const int64_t slot = 2 * (int64_t)(blockIdx.x + j) + (j == 0 ? 1 : 0);
+                const int slot = 2 * ((int)blockIdx.x + j) + (j == 0 ? 1 : 0);
                 ml[u] = p.part_ml[slot * ROWS + row];
-                part[u] = *reinterpret_cast<const f32x4_t*>(p.part_o + (slot * ROWS + row) * HD + chunk * 4);
+                part[u] = *reinterpret_cast<const f32x4_t*>(p.part_o + (int64_t)(slot * ROWS + row) * HD + chunk * 4);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (i + u * shares < pieces) add(ml[u].x, ml[u].y, part[u]);
         }
+        if (shares > 1) {
+            so[threadIdx.x] = o;
+            if (chunk == 0) sml[s] = make_float2(m, l);
+        }
+        if (shares == 1) write_row<HD, BF>(p, cut.x, cut.w + row, cut.y, chunk, o, make_float2(m, l));
     }
-    __shared__ f32x4_t so[1024];
-    __shared__ float2 sml[kSlots];
-    if (shares > 1) {
-        so[threadIdx.x] = o;
-        if (chunk == 0) sml[s] = make_float2(m, l);
-        __syncthreads();
-        if (share == 0)
-            for (int u = 1; u < shares; ++u) {
-                const float2 ml = sml[s + u * span];
-                add(ml.x, ml.y, so[threadIdx.x + u * span * kChunks]);
-            }
+    if (shares == 1) return;
+    __syncthreads();
+    const int row = s % span;
+    if (share != 0 || row >= nrows) return;
+    float top = kEmptyMax, l = 0.0f;
+    for (int u = 0; u < shares; ++u) top = __builtin_fmaxf(top, sml[s + u * span].x);
+    f32x4_t o = (f32x4_t){};
+    for (int u = 0; u < shares; ++u) {
+        const float2 ml = sml[s + u * span];
+        const float a = __builtin_amdgcn_exp2f(ml.x - top);
+        o += so[threadIdx.x + u * span * kChunks] * a;
+        l = __builtin_fmaf(ml.y, a, l);
     }
-    if (share == 0 && row < at.nrows) write_row<HD, BF>(p, at.b, at.r0 + row, cut.z, chunk, o, make_float2(m, l));
+    write_row<HD, BF>(p, cut.x, cut.w + row, cut.y, chunk, o, make_float2(top, l));
 }
 
 // ---- host side -----------------------------------------------------------------
@@ -843,20 +880,23 @@ bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, Page
         return false;
     const int64_t rows = a->tokens * (a->q_heads / c->kv_heads);
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    p.blocks = device_shape().cus * 2;
+    p.blocks = device_shape().cus * (rows <= 16 ? 3 : 2);
     const int64_t tiles = ceil_div(rows, p.rows);
-    if (c->batch > (int64_t(1) << 31) / (tiles ? tiles : 1)) return false;
+    // places, and the steps of the line, are counted in 32 bits
+    if (c->batch > 0x7fffffff / (tiles ? tiles : 1)) return false;
+    const int step = p.rows <= 32 ? kNarrowStep : kWideStep;
+    const int64_t steps = ceil_div(c->entries * c->page_size, step) + 1 + unit_steps(step);
+    if (c->batch * tiles > 0x7fffffff / (steps * c->kv_heads)) return false;
     p.bytes = p.blocks * (16 + 2 * p.rows * (c->head_dim + 2) * 4);
     return true;
 }
 
 template <int MODE, int HD, int ROWS, bool BF>
 void go(const PagedParams& p, int64_t blocks, hipStream_t st) {
-    constexpr int STEP = ROWS <= 32 ? kNarrowStep : kWideStep;
-    const dim3 grid((unsigned)blocks), join((unsigned)blocks, (unsigned)ceil_div(ROWS, 1024 / (HD / 4)));
+    const dim3 grid((unsigned)blocks);
     if constexpr (ROWS <= 32) hipLaunchKernelGGL((paged_narrow_kernel<MODE, HD, ROWS / 16, BF>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((paged_wide_kernel<MODE, HD, ROWS, BF>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((paged_join_kernel<HD, ROWS, STEP, BF>), join, dim3(1024), 0, st, p);
+    hipLaunchKernelGGL((paged_join_kernel<HD, ROWS, BF>), grid, dim3(512), 0, st, p);
 }
 template <int MODE, int HD, bool BF>
 void go(const PagedParams& p, const PagedPlan& plan, hipStream_t st) {
@@ -894,7 +934,7 @@ int run(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, void* 
     p.rows = p.tokens * p.group;
     p.tiles = (int)ceil_div(p.rows, plan_.rows);
     p.capacity = p.c.entries * p.c.page_size;
-    p.places = c->batch * p.tiles;
+    p.places = (int)c->batch * p.tiles;
     p.scale = a->scale;
     p.cap = a->cap;
     const hipStream_t st = hs(stream);
