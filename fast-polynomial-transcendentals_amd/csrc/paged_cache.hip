@@ -14,12 +14,24 @@
 
 namespace pt {
 
+// n / d for n below 2^31: the high half of n m, shifted, with m = 2^(31 + s) / d rounded up
+// and 2^s >= d, which is off by less than 1 / d.
+struct Divisor {
+    uint32_t d, m, s;
+
+    Divisor() = default;
+    explicit Divisor(uint32_t d_) : d(d_), s(0) {
+        while ((uint64_t(1) << s) < d) ++s;
+        m = (uint32_t)((uint64_t(1) << (31 + s)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t divide(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> (s - 1); }
+};
+
 struct Fp4Rows {
     const uint16_t *k, *v;
     AttnStrides ks, vs;
-    int tokens;
-    uint32_t threads;  // 2 hkv HD / 8 a token
-    uint32_t per;
+    uint32_t threads;
+    Divisor per, tokens, page;  // threads of a token (hkv HD / 8), tokens, page size
 };
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
@@ -80,45 +92,37 @@ __device__ __forceinline__ u32x4_t fp4_elements(uint32_t codes, float scale) {
     return r;
 }
 
-// A thread's eight elements: key or value, head, position and the row in the cache.
+// A thread's eight elements of a key and of its value: token, head and the row in the
+// cache.
 template <int HD>
 struct Fp4Place {
-    uint32_t bt, kv, h, chunk;
+    uint32_t bt, b, t, h, chunk;
     int page, row;
 
     __device__ __forceinline__ Fp4Place(const Fp4Pages& p, const Fp4Rows& r, uint32_t i) {
         constexpr uint32_t kChunks = HD / 8;
-        bt = i / r.per;
-        const uint32_t rest = i - bt * r.per;
+        bt = r.per.divide(i);
+        const uint32_t rest = i - bt * r.per.d;
         chunk = rest % kChunks;
-        const uint32_t head = rest / kChunks;
-        kv = head >= (uint32_t)p.hkv;
-        h = head - kv * (uint32_t)p.hkv;
-        const uint32_t b = bt / (uint32_t)r.tokens;
-        const int pos = p.len(b) - r.tokens + (int)(bt - b * (uint32_t)r.tokens);
-        const int entry = pos / p.page_size;
-        page = pos < 0 ? -1 : p.page_of(b, entry);
+        h = rest / kChunks;
+        b = r.tokens.divide(bt);
+        t = bt - b * r.tokens.d;
+        const int pos = p.len(b) - (int)r.tokens.d + (int)t;
+        const int entry = pos < 0 ? -1 : (int)r.page.divide((uint32_t)pos);
+        page = p.page_of(b, entry);
         row = pos - entry * p.page_size;
     }
-    __device__ __forceinline__ uint8_t* codes(const Fp4Pages& p) const {
-        return const_cast<uint8_t*>(p.head(page, (int)kv, (int)h)) + row * (HD / 2) + chunk * 4;
+    __device__ __forceinline__ uint8_t* head(const Fp4Pages& p, int kv) const {
+        return const_cast<uint8_t*>(p.head(page, kv, (int)h));
     }
-    __device__ __forceinline__ uint8_t* byte(const Fp4Pages& p) const {
-        return const_cast<uint8_t*>(p.head(page, (int)kv, (int)h)) + p.page_size * (HD / 2) + row * (HD / kFp4Block) +
-               chunk / 4;
+    __device__ __forceinline__ uint32_t codes() const { return (uint32_t)row * (HD / 2) + chunk * 4; }
+    __device__ __forceinline__ uint32_t byte(const Fp4Pages& p) const {
+        return (uint32_t)(p.page_size * (HD / 2) + row * (HD / kFp4Block)) + chunk / 4;
     }
 };
 
-template <int HD, bool BF>
-__global__ void __launch_bounds__(256) fp4_store_kernel(Fp4Pages p, Fp4Rows r) {
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= r.threads) return;
-    const Fp4Place<HD> at(p, r, i);
-    if (at.page < 0) return;
-    const uint32_t b = at.bt / (uint32_t)r.tokens, t = at.bt - b * (uint32_t)r.tokens;
-    const AttnStrides& s = at.kv ? r.vs : r.ks;
-    const u32x4_t x =
-        *reinterpret_cast<const u32x4_t*>((at.kv ? r.v : r.k) + b * s.b + t * s.s + at.h * s.h + at.chunk * 8);
+template <bool BF>
+__device__ __forceinline__ uint32_t largest(u32x4_t x) {
     uint32_t top = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -126,9 +130,26 @@ __global__ void __launch_bounds__(256) fp4_store_kernel(Fp4Pages p, Fp4Rows r) {
         top = lo > top ? lo : top;
         top = hi > top ? hi : top;
     }
-    const uint32_t byte = fp4_byte<BF>(quad_max(top));
-    *reinterpret_cast<uint32_t*>(at.codes(p)) = byte == 255 ? 0 : fp4_codes<BF>(x, as_f32(byte << 23));
-    if ((at.chunk & 3) == 0) *at.byte(p) = (uint8_t)byte;
+    return fp4_byte<BF>(quad_max(top));
+}
+
+template <int HD, bool BF>
+__global__ void __launch_bounds__(256) fp4_store_kernel(Fp4Pages p, Fp4Rows r) {
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= r.threads) return;
+    const Fp4Place<HD> at(p, r, i);
+    if (at.page < 0) return;
+    const u32x4_t k = *reinterpret_cast<const u32x4_t*>(r.k + at.b * r.ks.b + at.t * r.ks.s + at.h * r.ks.h + at.chunk * 8);
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(r.v + at.b * r.vs.b + at.t * r.vs.s + at.h * r.vs.h + at.chunk * 8);
+    const uint32_t kb = largest<BF>(k), vb = largest<BF>(v);
+    uint8_t *kh = at.head(p, 0), *vh = at.head(p, 1);
+    const uint32_t codes = at.codes();
+    *reinterpret_cast<uint32_t*>(kh + codes) = kb == 255 ? 0 : fp4_codes<BF>(k, as_f32(kb << 23));
+    *reinterpret_cast<uint32_t*>(vh + codes) = vb == 255 ? 0 : fp4_codes<BF>(v, as_f32(vb << 23));
+    if ((at.chunk & 3) == 0) {
+        kh[at.byte(p)] = (uint8_t)kb;
+        vh[at.byte(p)] = (uint8_t)vb;
+    }
 }
 
 template <int HD, bool BF>
@@ -136,10 +157,16 @@ __global__ void __launch_bounds__(256) fp4_load_kernel(Fp4Pages p, Fp4Rows r, ui
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     if (i >= r.threads) return;
     const Fp4Place<HD> at(p, r, i);
-    u32x4_t x = {0, 0, 0, 0};
-    if (at.page >= 0)
-        x = fp4_elements<BF>(*reinterpret_cast<const uint32_t*>(at.codes(p)), fp4_scale(*at.byte(p)));
-    *reinterpret_cast<u32x4_t*>((at.kv ? v : k) + ((int64_t)at.bt * p.hkv + at.h) * HD + at.chunk * 8) = x;
+    u32x4_t kx = {0, 0, 0, 0}, vx = kx;
+    if (at.page >= 0) {
+        const uint8_t *kh = at.head(p, 0), *vh = at.head(p, 1);
+        const uint32_t codes = at.codes(), byte = at.byte(p);
+        kx = fp4_elements<BF>(*reinterpret_cast<const uint32_t*>(kh + codes), fp4_scale(kh[byte]));
+        vx = fp4_elements<BF>(*reinterpret_cast<const uint32_t*>(vh + codes), fp4_scale(vh[byte]));
+    }
+    const int64_t out = (int64_t)i * 8;
+    *reinterpret_cast<u32x4_t*>(k + out) = kx;
+    *reinterpret_cast<u32x4_t*>(v + out) = vx;
 }
 
 // ---- pages of several sequences ------------------------------------------------
@@ -159,7 +186,9 @@ __global__ void __launch_bounds__(256) fp4_load_kernel(Fp4Pages p, Fp4Rows r, ui
 //
 // Four launches: the marks are cleared, every entry marks its page, one block counts
 // (a bitmap of the pages, 32 to a thread and step, and the rows' wishes), and the last
-// writes the table and copies the pages, which is what takes the time.
+// writes the table and copies the pages, which is what takes the time.  With few pages and
+// entries one block does all but the copies, its marks in LDS: 16 rows of 25
+// entries 12.4 us, 17 in four launches.
 
 constexpr int kNoRow = 0x7fffffff;
 constexpr int kScan = 1024;
@@ -181,8 +210,7 @@ struct PagePlan {
 
 __device__ __forceinline__ int words_of(int pages) { return (pages + 31) / 32; }
 
-__global__ void __launch_bounds__(256) clear_marks_kernel(PagePlan p, bool fork) {
-    const int i = (int)(blockIdx.x * 256u + threadIdx.x);
+__device__ __forceinline__ void clear_marks(const PagePlan& p, bool fork, int i) {
     if (i < words_of(p.pages)) {
         p.used[i] = 0;
         if (fork) p.full[i] = 0;
@@ -215,9 +243,7 @@ struct ForkRow {
     }
 };
 
-__global__ void __launch_bounds__(256) fork_mark_kernel(PagePlan p) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.rows * p.entries) return;
+__device__ __forceinline__ void fork_mark(const PagePlan& p, int64_t i) {
     const int row = (int)(i / p.entries), entry = (int)(i - (int64_t)row * p.entries);
     const ForkRow r(p, row);
     if (entry >= r.held) return;
@@ -227,12 +253,21 @@ __global__ void __launch_bounds__(256) fork_mark_kernel(PagePlan p) {
     if (entry < r.full) atomicOr(&p.full[id >> 5], 1u << (id & 31));
     else atomicMin(&p.first[id], row);
 }
-__global__ void __launch_bounds__(256) compact_mark_kernel(PagePlan p) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.rows * p.entries) return;
+__device__ __forceinline__ void compact_mark(const PagePlan& p, int64_t i) {
     const int64_t row = i / p.entries;
     const int id = p.table[row * p.table_stride + (i - row * p.entries)];
     if ((unsigned)id < (unsigned)p.pages) atomicOr(&p.used[id >> 5], 1u << (id & 31));
+}
+template <bool FORK>
+__global__ void __launch_bounds__(256) clear_marks_kernel(PagePlan p) {
+    clear_marks(p, FORK, (int)(blockIdx.x * 256u + threadIdx.x));
+}
+template <bool FORK>
+__global__ void __launch_bounds__(256) mark_kernel(PagePlan p) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)p.rows * p.entries) return;
+    if constexpr (FORK) fork_mark(p, i);
+    else compact_mark(p, i);
 }
 
 // The sum of the threads ahead, and of all.
@@ -273,7 +308,7 @@ __device__ __forceinline__ uint32_t valid_bits(const PagePlan& p, int word) {
     return left >= 32 ? ~0u : (1u << left) - 1;
 }
 
-__global__ void __launch_bounds__(kScan) fork_plan_kernel(PagePlan p) {
+__device__ __forceinline__ void fork_plan(const PagePlan& p) {
     const int words = words_of(p.pages);
     const WordRange w(words);
     int n = 0, free = 0;
@@ -318,7 +353,7 @@ __global__ void __launch_bounds__(kScan) fork_plan_kernel(PagePlan p) {
     }
 }
 
-__global__ void __launch_bounds__(kScan) compact_plan_kernel(PagePlan p) {
+__device__ __forceinline__ void compact_plan(const PagePlan& p) {
     const int words = words_of(p.pages);
     const WordRange w(words);
     int n = 0, used = 0, holes = 0, moves = 0;
@@ -347,53 +382,99 @@ __global__ void __launch_bounds__(kScan) compact_plan_kernel(PagePlan p) {
     }
 }
 
+template <bool FORK>
+__global__ void __launch_bounds__(kScan) plan_kernel(PagePlan p) {
+    if constexpr (FORK) fork_plan(p);
+    else compact_plan(p);
+}
+
+// An entry of the new table.
+template <bool FORK>
+__device__ __forceinline__ void write_entry(const PagePlan& p, int64_t i) {
+    const int row = (int)(i / p.entries), entry = (int)(i - (int64_t)row * p.entries);
+    int id = -1;
+    if constexpr (FORK) {
+        const ForkRow r(p, row);
+        const int copy = r.copies(p, row);
+        const int wish = p.base[row] + (entry == r.full && copy ? 0 : copy + entry - r.held);
+        if (entry < r.held && !(entry == r.full && copy)) id = r.page(p, entry);
+        else if (entry < r.end) id = wish < p.count[1] ? p.ids[wish] : -1;
+    } else {
+        id = p.table[row * p.table_stride + entry];
+        if ((unsigned)id >= (unsigned)p.pages) id = -1;
+        else if (id >= p.out_count[0]) id = p.ids[p.place[id]];
+    }
+    p.out[i] = id;
+}
+
+constexpr int kSmallPages = 8192, kSmallCells = 4096;
+
+template <bool FORK>
+__global__ void __launch_bounds__(kScan) small_plan_kernel(PagePlan p) {
+    __shared__ uint32_t used[kSmallPages / 32], full[FORK ? kSmallPages / 32 : 1];
+    __shared__ int32_t ids[kSmallPages], other[kSmallPages];  // first or place
+    p.used = used;
+    p.full = full;
+    (FORK ? p.first : p.place) = other;
+    int32_t* const holes = p.ids;  // what the copies look up
+    p.ids = ids;
+    for (int i = threadIdx.x; i < p.pages; i += kScan) clear_marks(p, FORK, i);
+    __syncthreads();
+    const int cells = p.rows * p.entries;
+    for (int i = threadIdx.x; i < cells; i += kScan) {
+        if constexpr (FORK) fork_mark(p, i);
+        else compact_mark(p, i);
+    }
+    __syncthreads();
+    if constexpr (FORK) fork_plan(p);
+    else compact_plan(p);
+    __syncthreads();
+    for (int i = threadIdx.x; i < cells; i += kScan) write_entry<FORK>(p, i);
+    if constexpr (!FORK)
+        for (int i = threadIdx.x; i < p.count[0]; i += kScan) holes[i] = ids[i];
+}
+
 struct PageCaches {
     unsigned char* at[kMostCaches];
     int64_t bytes[kMostCaches];  // of a page
 };
 
-// Blocks of y = the last write the table, those of the others copy their cache's
-// pages, 16 KB a block and step.
-template <bool FORK>
-__global__ void __launch_bounds__(256) move_pages_kernel(PagePlan p, PageCaches c, int caches, bool table) {
+// Blocks of y = the last write the table (small plans have), those of the others copy
+// their cache's pages, 8 KB a block and step.  ONCE: more than the caches hold, past which
+// the copies go (1024 pages of 557 KB, 1.14 GB read and written: 203 us, 5.6 TB/s; 239 us through the
+// caches; 213 with 8192 blocks, 222 in steps of 16 KB).
+template <bool FORK, bool ONCE>
+__global__ void __launch_bounds__(256) move_pages_kernel(PagePlan p, PageCaches c, int caches) {
     if ((int)blockIdx.y == caches) {
-        if (!table) return;
         const int64_t n = (int64_t)p.rows * p.entries;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-            const int row = (int)(i / p.entries), entry = (int)(i - (int64_t)row * p.entries);
-            int id = -1;
-            if constexpr (FORK) {
-                const ForkRow r(p, row);
-                const int copy = r.copies(p, row);
-                const int wish = p.base[row] + (entry == r.full && copy ? 0 : copy + entry - r.held);
-                if (entry < r.held && !(entry == r.full && copy)) id = r.page(p, entry);
-                else if (entry < r.end) id = wish < p.count[1] ? p.ids[wish] : -1;
-            } else {
-                id = p.table[row * p.table_stride + entry];
-                if ((unsigned)id >= (unsigned)p.pages) id = -1;
-                else if (id >= p.out_count[0]) id = p.ids[p.place[id]];
-            }
-            p.out[i] = id;
-        }
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) write_entry<FORK>(p, i);
         return;
     }
     unsigned char* cache = c.at[blockIdx.y];
     const int64_t bytes = c.bytes[blockIdx.y];
-    const uint32_t steps = (uint32_t)((bytes + 16383) / 16384);
+    // parts of 8 KB
+    const uint32_t steps = (uint32_t)((bytes + 8191) / 8192);
     const uint64_t all = (uint64_t)p.count[0] * steps;
     for (uint64_t i = blockIdx.x; i < all; i += gridDim.x) {
         const uint32_t k = (uint32_t)(i / steps), step = (uint32_t)(i - (uint64_t)k * steps);
         const int2 m = FORK ? p.moves[k] : make_int2(p.moves[k].x, p.ids[k]);
-        const int64_t off = (int64_t)step * 16384 + threadIdx.x * 16;
+        const int64_t off = (int64_t)step * 8192 + threadIdx.x * 16;
         const unsigned char* src = cache + m.x * bytes + off;
         unsigned char* dst = cache + m.y * bytes + off;
-        u32x4_t v[4];
+        u32x4_t v[2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (off + u * 4096 < bytes) v[u] = *reinterpret_cast<const u32x4_t*>(src + u * 4096);
+        for (int u = 0; u < 2; ++u)
+            if (off + u * 4096 < bytes) {
+                const u32x4_t* x = reinterpret_cast<const u32x4_t*>(src + u * 4096);
+                v[u] = ONCE ? __builtin_nontemporal_load(x) : *x;
+            }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (off + u * 4096 < bytes) *reinterpret_cast<u32x4_t*>(dst + u * 4096) = v[u];
+        for (int u = 0; u < 2; ++u)
+            if (off + u * 4096 < bytes) {
+                u32x4_t* x = reinterpret_cast<u32x4_t*>(dst + u * 4096);
+                if constexpr (ONCE) __builtin_nontemporal_store(v[u], x);
+                else *x = v[u];
+            }
     }
 }
 
@@ -416,10 +497,11 @@ int64_t blocks_of(const spline_hip_fp4_cache* c, int64_t tokens, Fp4Rows& r) {
     if (!fp4_sizes_ok(c, tokens)) return -1;
     if (c->batch == 0 || tokens == 0) return 0;
     if (!fp4_pointers_ok(c)) return -1;
-    const int64_t per = 2 * c->kv_heads * c->head_dim / 8;
-    if (c->batch * tokens > 0xffffff00ll / per) return -1;
-    r.tokens = (int)tokens;
-    r.per = (uint32_t)per;
+    const int64_t per = c->kv_heads * c->head_dim / 8;
+    if (c->batch * tokens > 0x7fffff00ll / per) return -1;
+    r.per = Divisor((uint32_t)per);
+    r.tokens = Divisor((uint32_t)tokens);
+    r.page = Divisor((uint32_t)c->page_size);
     r.threads = (uint32_t)(c->batch * tokens * per);
     return ceil_div(r.threads, 256);
 }
@@ -488,6 +570,49 @@ int64_t lay_out(const spline_hip_pages* a, bool fork, PagePlan& p, char* ws) {
     return bytes;
 }
 
+template <bool FORK>
+void move(const spline_hip_pages* a, const PagePlan& p, hipStream_t st) {
+    const dim3 block(256);
+    const int64_t cells = ceil_div(a->rows * a->entries, 256);
+    const bool small = a->pages <= kSmallPages && a->rows * a->entries <= kSmallCells;
+    if (small) {
+        hipLaunchKernelGGL((small_plan_kernel<FORK>), dim3(1), dim3(kScan), 0, st, p);
+    } else {
+        const int64_t marks = ceil_div(FORK ? a->pages : ceil_div(a->pages, 32), 256);
+        if (marks > 0) hipLaunchKernelGGL((clear_marks_kernel<FORK>), dim3((unsigned)marks), block, 0, st, p);
+        if (cells > 0) hipLaunchKernelGGL((mark_kernel<FORK>), dim3((unsigned)cells), block, 0, st, p);
+        hipLaunchKernelGGL((plan_kernel<FORK>), dim3(1), dim3(kScan), 0, st, p);
+    }
+    // A page goes to one place.  A fork seldom copies as many pages as it has rows, and
+    // blocks without one cost their launch.
+    const int64_t most_moves = FORK ? (a->rows < a->pages ? a->rows : a->pages) : a->pages / 2;
+    double bytes = 0;
+    for (int64_t i = 0; i < a->num_caches; ++i) bytes += (double)a->cache_page_bytes[i] * most_moves;
+    const bool once = bytes >= kMallBytes;
+    int64_t at = 0;
+    do {
+        const int n = (int)(a->num_caches - at < kMostCaches ? a->num_caches - at : kMostCaches);
+        const bool table = at == 0 && !small;
+        PageCaches c{};
+        int64_t steps = 0;
+        for (int i = 0; i < n; ++i) {
+            c.at[i] = static_cast<unsigned char*>(a->caches[at + i]);
+            c.bytes[i] = a->cache_page_bytes[at + i];
+            steps = c.bytes[i] > steps ? c.bytes[i] : steps;
+        }
+        steps = ceil_div(steps, 8192) * most_moves;
+        int64_t x = ceil_div(FORK ? 8192 : 32768, n + 1);
+        const int64_t need = table && cells > steps ? cells : steps;
+        x = x < need ? x : need;
+        if (x > 0 && n + table > 0) {
+            const dim3 grid((unsigned)x, (unsigned)(n + table));
+            if (once) hipLaunchKernelGGL((move_pages_kernel<FORK, true>), grid, block, 0, st, p, c, n);
+            else hipLaunchKernelGGL((move_pages_kernel<FORK, false>), grid, block, 0, st, p, c, n);
+        }
+        at += n;
+    } while (at < a->num_caches);
+}
+
 int rearrange(const spline_hip_pages* a, bool fork, void* stream) {
     PagePlan p{};
     if (lay_out(a, fork, p, static_cast<char*>(a ? a->workspace : nullptr)) < 0) return hipErrorInvalidValue;
@@ -517,39 +642,7 @@ int rearrange(const spline_hip_pages* a, bool fork, void* stream) {
     p.pages = (int)a->pages;
     p.page_size = (int)a->page_size;
     p.grow = (int)a->grow;
-    const hipStream_t st = hs(stream);
-    const dim3 block(256);
-    const int64_t marks = ceil_div(fork ? a->pages : ceil_div(a->pages, 32), 256), cells = ceil_div(a->rows * a->entries, 256);
-    if (marks > 0) hipLaunchKernelGGL(clear_marks_kernel, dim3((unsigned)marks), block, 0, st, p, fork);
-    if (cells > 0) {
-        if (fork) hipLaunchKernelGGL(fork_mark_kernel, dim3((unsigned)cells), block, 0, st, p);
-        else hipLaunchKernelGGL(compact_mark_kernel, dim3((unsigned)cells), block, 0, st, p);
-    }
-    if (fork) hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kScan), 0, st, p);
-    else hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kScan), 0, st, p);
-    // a page goes to one place, and 4096 blocks keep enough loads in flight
-    const int64_t most_moves = fork ? a->rows : a->pages / 2;
-    int64_t at = 0;
-    do {
-        const int n = (int)(a->num_caches - at < kMostCaches ? a->num_caches - at : kMostCaches);
-        PageCaches c{};
-        int64_t steps = 0;
-        for (int i = 0; i < n; ++i) {
-            c.at[i] = static_cast<unsigned char*>(a->caches[at + i]);
-            c.bytes[i] = a->cache_page_bytes[at + i];
-            steps = c.bytes[i] > steps ? c.bytes[i] : steps;
-        }
-        steps = ceil_div(steps, 16384) * most_moves;
-        int64_t x = ceil_div(4096, n + 1);
-        const int64_t need = at == 0 && cells > steps ? cells : steps;
-        x = x < need ? x : need;
-        if (x > 0) {
-            const dim3 grid((unsigned)x, (unsigned)(n + 1));
-            if (fork) hipLaunchKernelGGL((move_pages_kernel<true>), grid, block, 0, st, p, c, n, at == 0);
-            else hipLaunchKernelGGL((move_pages_kernel<false>), grid, block, 0, st, p, c, n, at == 0);
-        }
-        at += n;
-    } while (at < a->num_caches);
+    fork ? move<true>(a, p, hs(stream)) : move<false>(a, p, hs(stream));
     return hipGetLastError();
 }
 

@@ -317,10 +317,9 @@ def test_graph_of_a_decoding_step(cuda):
     assert state[1].tolist() == [34, 50, 21]
     every = torch.cat([x for x, _ in queries], 1)
     whole, lse = fa4_runtime.flash_attn_paged_fp4(every, caches[0], *state)
-    for i, (_, o) in enumerate(queries):
-        ref_out = ref.attention(queries[i][0].cpu(), caches[0].cpu(), state[0].cpu(), state[1].cpu() - 19 + i, 1 / math.sqrt(dim))
-        ref.check(o[:2], ref_out)
-        ref.check((whole[:, i:i + 1], lse[..., i:i + 1]), ref_out)
+    for i, (step_q, o) in enumerate(queries):
+        ref.check(o[:2], ref.attention(step_q.cpu(), caches[0].cpu(), state[0].cpu(), state[1].cpu() - 19 + i, 1 / math.sqrt(dim)))
+    ref.check((whole, lse), ref.attention(every.cpu(), caches[0].cpu(), state[0].cpu(), state[1].cpu(), 1 / math.sqrt(dim)))
 
 
 def test_beams_share_their_prompt(cuda):
