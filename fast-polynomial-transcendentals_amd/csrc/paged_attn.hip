@@ -33,8 +33,9 @@ namespace pt {
 constexpr int kNarrowStep = 128;  // keys of a narrow block's step
 constexpr int kWaveKeys = 32;     // of which a wave has 32
 constexpr int kWideStep = 64;
+constexpr int kDecodeStep = 256;  // each wave 64 of them
 // A unit's first keys and its result cost as much as so many steps more.
-constexpr int unit_steps(int step) { return step == kWideStep ? 4 : 2; }
+constexpr int unit_steps(int step) { return step == kWideStep ? 4 : step == kDecodeStep ? 2 : 2; }
 
 struct PagedParams {
     const uint16_t* q;
@@ -54,13 +55,19 @@ __device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Over the lanes of a row (l ^ 16 and l ^ 32): the largest of eight scores, NaN if one is
+// Has the compiler wait for a fragment's load here: where it is first used inside a loop,
+// the wait there would be for every load issued since, in every turn.
+__device__ __forceinline__ void loaded(bf16x8_t& f) { asm volatile("" : "+v"(f)); }
+
+// Over the lanes of a row (l ^ 16 and l ^ 32): the largest of N scores, NaN if one is
 // (v_maximum3_f32: no instructions that quiet its operands), and a sum.
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-__device__ __forceinline__ float row_max(const float (&y)[8]) {
-    float x = maximum(maximum(maximum(y[0], y[1]), y[2]), y[3]);
-    x = maximum(maximum(x, y[4]), y[5]);
-    x = maximum(maximum(x, y[6]), y[7]);
+template <int N>
+__device__ __forceinline__ float row_max(const float (&y)[N]) {
+    float x = maximum(maximum(y[0], y[1]), y[2]);
+#pragma unroll
+    for (int e = 3; e + 1 < N; e += 2) x = maximum(maximum(x, y[e]), y[e + 1]);
+    x = maximum(x, y[N - 1]);
     const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
     x = maximum(as_f32(r[0]), as_f32(r[1]));
     const auto t = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
@@ -258,20 +265,42 @@ __device__ __forceinline__ void write_row(const PagedParams& p, int b, int row, 
 
 // ---- a wave's tile of 32 keys -------------------------------------------------------
 
-// A wave's rows of V in BF16, 32 bytes between them and 16 more between groups of eight:
-// 16 rows' writes of one chunk, and the 8 rows by 32 bytes of half a transposing read,
-// fall on different columns of the 256 bytes that LDS serves at once.
+// A wave's rows of V in BF16, 32 bytes between them and 16 more between groups of eight.
+// A transposing read takes 256 bytes at once, eight rows by 32 bytes, which fall on
+// different columns; a write 128 bytes, 16 of eight lanes: lanes 0..7 have the rows 0..3
+// and 8..11 (v_key), and those do.
 template <int HD>
 __device__ __forceinline__ constexpr uint32_t v_at(int row, int chunk) {
     return (uint32_t)(row * (HD * 2 + 32) + (row >> 3) * 16 + chunk * 16);
 }
 
-// The codes of 16 keys that a lane holds: HD / 4 elements of key lane % 16, from
-// (lane / 16) HD / 4 on, and their block's byte.
+// The key of 16 whose values a lane holds.
+__device__ __forceinline__ int v_key(int c16) { return (c16 & 3) | (c16 & 4) << 1 | (c16 & 8) >> 1; }
+
+// Where a lane's codes of 16 keys lie: HD / 4 elements of a key (row) from quarter HD / 4
+// on, and the word with their block's byte.
+template <int HD>
+struct LaneCodes {
+    uint32_t code, word, shift;
+
+    __device__ __forceinline__ LaneCodes(const Fp4Pages& c, int row, int quarter) {
+        code = (uint32_t)(row * (HD / 2) + quarter * (HD / 8));
+        const uint32_t byte = (uint32_t)(c.page_size * (HD / 2) + row * (HD / kFp4Block) + quarter * (HD / 4) / kFp4Block);
+        word = byte & ~3u;
+        shift = (byte & 3) * 8;
+    }
+};
+
+// The codes of 16 keys that a lane holds.  The byte is loaded in its word: what the
+// compiler makes of a byte that goes round a loop waits for it too early.
 template <int HD>
 struct Codes {
     uint32_t w[HD / 32];
-    uint32_t byte;
+    uint32_t word;
+
+    __device__ __forceinline__ uint32_t byte(const LaneCodes<HD>& lane) const {
+        return __builtin_amdgcn_ubfe(word, lane.shift, 8);
+    }
 
     template <bool ONCE>
     __device__ __forceinline__ void load(const uint8_t* head, uint32_t code, uint32_t at) {
@@ -280,20 +309,21 @@ struct Codes {
         const Words a = ONCE ? __builtin_nontemporal_load(src) : *src;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) w[i] = a[i];
-        byte = ONCE ? __builtin_nontemporal_load(head + at) : head[at];
+        const uint32_t* bytes = reinterpret_cast<const uint32_t*>(head + at);
+        word = ONCE ? __builtin_nontemporal_load(bytes) : *bytes;
     }
     // Of page 0 where there is none (its keys are masked, its values cleared): a branch would
     // have every wait for a load wait for all of them.
     // ONCE: nobody else reads them.
     template <bool ONCE>
-    __device__ __forceinline__ void load(const Fp4Pages& c, int page, int row, int kv, int h, uint32_t lane_code,
-                                         uint32_t lane_byte) {
-        load<ONCE>(c.head(page < 0 ? 0 : page, kv, h), (uint32_t)row * (HD / 2) + lane_code, (uint32_t)row * (HD / kFp4Block) + lane_byte);
+    __device__ __forceinline__ void load(const Fp4Pages& c, int page, int row, int kv, int h, const LaneCodes<HD>& lane) {
+        load<ONCE>(c.head(page < 0 ? 0 : page, kv, h), (uint32_t)row * (HD / 2) + lane.code,
+                   (uint32_t)row * (HD / kFp4Block) + lane.word);
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) w[i] = 0;
-        byte = 0;
+        word = 0;
     }
 };
 
@@ -371,14 +401,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             my_page = i0 + (lane >> 1) < n && key < at.visible ? p.c.page_of(at.b, entry) : -1;
             my_row = key - entry * p.c.page_size;
         };
-        const uint32_t lane_code = (uint32_t)(c16 * (HD / 2) + quarter * (HD / 8));
-        const uint32_t lane_byte = (uint32_t)(p.c.page_size * (HD / 2) + c16 * (HD / kFp4Block) + quarter * (HD / 4) / kFp4Block);
+        const LaneCodes<HD> k_lane(p.c, c16, quarter), v_lane(p.c, v_key(c16), quarter);
+        const int vkey = v_key(c16);
+        unsigned char* const v_write = vt + v_at<HD>(vkey, quarter * kC);
         auto load = [&](Codes<HD>& codes, int kv, int i, int g) __attribute__((always_inline)) {
             const int l = 2 * (i & 31) + g;
             codes.template load<true>(p.c, __builtin_amdgcn_readlane(my_page, l), __builtin_amdgcn_readlane(my_row, l), kv, kvh,
-                                      lane_code, lane_byte);
+                                      kv ? v_lane : k_lane);
         };
-        unsigned char* const v_write = vt + v_at<HD>(c16, quarter * kC);
         const unsigned char* const v_read = vt + v_at<HD>(4 * quarter + (c16 >> 2), (c16 & 3) >> 1) + (c16 & 1) * 8;
         // columns 16 dt + c16 of rows 4 quarter .. + 3 and 16 + 4 quarter .. + 3
         auto value_frag = [&](int dt) __attribute__((always_inline)) {
@@ -396,6 +426,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 #pragma unroll
             for (int g = 0; g < 2; ++g) load(v[g], 1, 0, g);
         }
+        if constexpr (BF)
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) loaded(qf[nr][c]);
         for (int i = 0; i < tiles; ++i) {
             const int key0 = (step0 + i) * kNarrowStep + wave * kWaveKeys;
             const bool hole[2] = {__builtin_amdgcn_readlane(my_page, 2 * (i & 31)) < 0,
@@ -403,7 +438,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             const bool masked = key0 + kWaveKeys - 1 > kfull || hole[0] || hole[1];
             if ((i & 31) == 31) look_up(i + 1);  // no page behind the last tile
             f32x4_t s[2][NR];
-            const float scale[2] = {fp4_scale(k[0].byte), fp4_scale(k[1].byte)};
+            const float scale[2] = {fp4_scale(k[0].byte(k_lane)), fp4_scale(k[1].byte(k_lane))};
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) s[0][nr] = s[1][nr] = (f32x4_t){};
 #pragma unroll
@@ -425,12 +460,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             if (masked)
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
-                    bad[g] = v[g].byte > (uint32_t)kFp4Most && !hole[g];
+                    bad[g] = v[g].byte(v_lane) > (uint32_t)kFp4Most && !hole[g];
                     if (bad[g] || hole[g]) v[g].clear();
                 }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const float scale = fp4_scale(v[g].byte);
+                const float scale = fp4_scale(v[g].byte(v_lane));
 #pragma unroll
                 for (int c = 0; c < kC; ++c)
                     *reinterpret_cast<bf16x8_t*>(v_write + v_at<HD>(16 * g, c)) = fp4_to_bf16(v[g].w[c], scale);
@@ -493,7 +528,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 #pragma unroll
             for (int g = 0; g < 2; ++g)
                 for (uint64_t m = __ballot(bad[g]); m != 0; m &= m - 1) {
-                    const int l = __builtin_ctzll(m), key = key0 + 16 * g + (l & 15), part = l >> 4;  // of the head, in four
+                    const int l = __builtin_ctzll(m), key = key0 + 16 * g + v_key(l & 15), part = l >> 4;  // of the head, in four
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
@@ -546,6 +581,241 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
     }
 }
 
+// ---- one new token -------------------------------------------------------------------
+//
+// The same for the up to 8 rows of a single token, all of which see the same keys.  A
+// wave has 64 keys of a step, in groups of 16, and its 16 columns hold the rows NC =
+// 2 or 4 times, 16 / NC columns each.  All columns of a group's scores are alike, so
+// column class c takes those of group c: the maximum, the exponentials and a softcap run
+// over NC groups at once.  In P the other groups' rows of a column are zero, so that a
+// column keeps a softmax over its class's keys, and the classes of a row are joined as the
+// waves are.
+template <int MODE, int HD, int NC, bool BF>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 || BF ? 3 : 2))) paged_decode_kernel(PagedParams p) {
+    constexpr int ROWS = 16, W = 16 / NC, kA = 4 / NC;  // rows' columns; accumulators of scores
+    constexpr int kC = HD / 32, kD = HD / 16;
+    constexpr int kVTile = v_at<HD>(32, 0), kSpill = o_at<HD>(16, 0);
+    constexpr int kRegion = kVTile > kSpill ? kVTile : kSpill;
+    __shared__ __align__(1024) unsigned char smem[4 * kRegion];
+    __shared__ float2 sml[4][16];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int c16 = lane & 15, quarter = lane >> 4, cls = c16 / W;
+    Stretch<ROWS, kDecodeStep> line;
+    if (!line.find(p, blockIdx.x)) return;
+
+    ScoreConsts consts;
+    consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
+    consts.scale = p.scale;
+    consts.cap = p.cap;
+    consts.inv_cap = 1.0f / p.cap;
+    if constexpr (MODE == kAttnSoftcapD4)
+#pragma unroll
+        for (int i = 1; i <= SoftcapConsts::T::P.deg; ++i) consts.tanh[i] = bf16_value(SoftcapConsts::T::P.c[i]);
+
+    unsigned char* const vt = smem + wave * kRegion;
+    const int vkey = v_key(c16);
+    unsigned char* const v_write = vt + v_at<HD>(vkey, quarter * kC);
+    const unsigned char* const v_read = vt + v_at<HD>(4 * quarter + (c16 >> 2), (c16 & 3) >> 1) + (c16 & 1) * 8;
+    auto value_frag = [&](int dt) __attribute__((always_inline)) {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(v_read + dt * 32);
+        const u32x2_t lo = __builtin_bit_cast(u32x2_t, lds_read_tr16(src));
+        const u32x2_t hi = __builtin_bit_cast(u32x2_t, lds_read_tr16(src + v_at<HD>(16, 0) / 2));
+        return __builtin_bit_cast(bf16x8_t, (u32x4_t){lo.x, lo.y, hi.x, hi.y});
+    };
+    const LaneCodes<HD> k_lane(p.c, c16, quarter), v_lane(p.c, v_key(c16), quarter);
+
+    while (line.x < line.x1) {
+        const Place<ROWS, kDecodeStep> at(p, line.place);
+        const int steps = at.steps(), step0 = line.first(), n = line.last(steps) - step0, kvh = line.kvh;
+        if (n == 0) {
+            line.advance(p, blockIdx.x, at);
+            break;
+        }
+        // ---- Q^T fragments, the rows in every class
+        bf16x8_t qf[kC], ql[BF ? 1 : kC];
+        {
+            const int row = c16 % W;
+            const uint16_t* src = p.q + at.b * p.qs.b + (kvh * p.group + (row < p.group ? row : 0)) * p.qs.h + quarter * (HD / 4);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                bf16x8_t f = {};
+                if (row < p.group) f = *reinterpret_cast<const bf16x8_t*>(src + 8 * c);
+                if constexpr (!BF) split_fp16(f, qf[c], ql[c]);
+                else qf[c] = f;
+            }
+        }
+        // ---- pages: lane 4 i + g knows where group g of step i lies, 16 steps at a time
+        int my_page = -1, my_row = 0;
+        auto look_up = [&](int i0) __attribute__((always_inline)) {
+            const int key = (step0 + i0 + (lane >> 2)) * kDecodeStep + wave * 64 + (lane & 3) * 16;
+            const int entry = key / p.c.page_size;
+            my_page = i0 + (lane >> 2) < n && key < at.visible ? p.c.page_of(at.b, entry) : -1;
+            my_row = key - entry * p.c.page_size;
+        };
+        Codes<HD> k[4], v[4];
+        auto load = [&](Codes<HD>& codes, int kv, int i, int g) __attribute__((always_inline)) {
+            const int l = 4 * (i & 15) + g;
+            codes.template load<true>(p.c, __builtin_amdgcn_readlane(my_page, l), __builtin_amdgcn_readlane(my_row, l), kv, kvh,
+                                      kv ? v_lane : k_lane);
+        };
+        const int tiles = p.c.pages > 0 ? n : 0;
+        if (tiles > 0) {
+            look_up(0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) load(k[g], 0, 0, g);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) load(v[g], 1, 0, g);
+        }
+        if constexpr (BF)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) loaded(qf[c]);
+        PagedState<HD> st;
+        for (int i = 0; i < tiles; ++i) {
+            const int key0 = (step0 + i) * kDecodeStep + wave * 64;
+            const uint32_t holes = (uint32_t)(__ballot(my_page < 0) >> (4 * (i & 15))) & 15;
+            const bool masked = key0 + 63 >= at.visible || holes != 0;
+            if ((i & 15) == 15) look_up(i + 1);  // no page behind the last tile
+            f32x4_t s[4];
+            float scale[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                s[g] = (f32x4_t){};
+                scale[g] = fp4_scale(k[g].byte(k_lane));
+            }
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const bf16x8_t kf = fp4_to_bf16(k[g].w[c], scale[g]);
+                    s[g] = mfma16(kf, qf[c], s[g]);
+                    if constexpr (!BF) s[g] = mfma16(kf, ql[c], s[g]);
+                }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) load(k[g], 0, i + 1, g);
+            // scores of the column's groups: keys 16 (NC a + cls) + 4 quarter + r
+            float y[4 * kA];
+#pragma unroll
+            for (int a = 0; a < kA; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = s[NC * a][r];
+#pragma unroll
+                    for (int c = 1; c < NC; ++c) x = cls == c ? s[NC * a + c][r] : x;
+                    y[4 * a + r] = x;
+                }
+            cap_scores<MODE>(y, consts);
+            if (masked) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g)  // what is not seen may be no number
+                    if ((holes >> g & 1) || key0 + 16 * g + vkey >= at.visible) v[g].clear();
+#pragma unroll
+                for (int a = 0; a < kA; ++a)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int g = NC * a + cls;
+                        if ((holes >> g & 1) || key0 + 16 * g + 4 * quarter + r >= at.visible) y[4 * a + r] = -__builtin_inff();
+                    }
+            }
+            const float mx = row_max(y) * consts.sl;
+            const bool move = mx - st.m > 8.0f;  // the lanes of a column decide alike
+            if (__any(move)) {
+                const float m = move ? mx : st.m;
+                const float alpha = __builtin_amdgcn_exp2f(st.m - m);
+                st.m = m;
+                st.l *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < kD; ++dt) st.o[dt] *= alpha;
+            }
+            float mul = consts.sl;
+            const bool far = __builtin_fabsf(st.m) >= kFarMax;
+            if (__any(far)) {
+#pragma unroll
+                for (int e = 0; e < 4 * kA; ++e) y[e] = far ? y[e] * mul : y[e];
+                mul = far ? 1.0f : mul;
+            }
+            uint32_t hi[2 * kA], lo[2 * kA];  // pairs of probabilities in two BF16 terms
+#pragma unroll
+            for (int e = 0; e < 4 * kA; e += 2) {
+                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], mul, -st.m));
+                const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e + 1], mul, -st.m));
+                st.l += a + b;
+                const bf16x2_t h = {(__bf16)a, (__bf16)b};
+                const bf16x2_t rest = {(__bf16)(a - (float)h.x), (__bf16)(b - (float)h.y)};
+                hi[e / 2] = __builtin_bit_cast(uint32_t, h);
+                lo[e / 2] = __builtin_bit_cast(uint32_t, rest);
+            }
+            // O^T += V^T P^T, 32 keys at a time
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int a = 2 * t / NC, c0 = 2 * t % NC;  // the classes of its groups: c0 and c0 + 1
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const float sv = fp4_scale(v[2 * t + g].byte(v_lane));
+#pragma unroll
+                    for (int c = 0; c < kC; ++c)
+                        *reinterpret_cast<bf16x8_t*>(v_write + v_at<HD>(16 * g, c)) = fp4_to_bf16(v[2 * t + g].w[c], sv);
+                }
+#pragma unroll
+                for (int g = 0; g < 2; ++g) load(v[2 * t + g], 1, i + 1, 2 * t + g);
+                auto frag = [&](const uint32_t (&w)[2 * kA]) __attribute__((always_inline)) {
+                    const bool x = cls == c0, z = cls == c0 + 1;
+                    return __builtin_bit_cast(bf16x8_t, (u32x4_t){x ? w[2 * a] : 0, x ? w[2 * a + 1] : 0, z ? w[2 * a] : 0,
+                                                                  z ? w[2 * a + 1] : 0});
+                };
+                const bf16x8_t pf = frag(hi), pr = frag(lo);
+                __builtin_amdgcn_sched_barrier(0);
+                bf16x8_t vf[kD];
+#pragma unroll
+                for (int dt = 0; dt < 3; ++dt) vf[dt] = value_frag(dt);
+#pragma unroll
+                for (int dt = 0; dt < kD; ++dt) {
+                    if (dt + 3 < kD) vf[dt + 3] = value_frag(dt + 3);
+                    st.o[dt] = mfma16(vf[dt], pf, st.o[dt]);
+                    st.o[dt] = mfma16(vf[dt], pr, st.o[dt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+
+        // ---- the shares of each row: four waves' classes
+        const bool begins = step0 == 0, ends = step0 + n == steps;
+        const int slot = 2 * (int)blockIdx.x + (begins ? 1 : 0);
+        __syncthreads();  // the region is free
+#pragma unroll
+        for (int dt = 0; dt < kD; ++dt) *reinterpret_cast<f32x4_t*>(vt + o_at<HD>(c16, 4 * dt + quarter)) = st.o[dt];
+        const float l = row_sum(st.l);
+        if (quarter == 0) sml[wave][c16] = make_float2(st.m, l);
+        __syncthreads();
+        constexpr int kChunks = HD / 4;
+        for (int i = tid; i < at.nrows * kChunks; i += 256) {
+            const int row = i / kChunks, chunk = i % kChunks;
+            float2 ml = make_float2(kEmptyMax, 0.0f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) ml.x = __builtin_fmaxf(ml.x, sml[w][W * c + row].x);
+            f32x4_t o = {};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const float2 x = sml[w][W * c + row];
+                    const float a = __builtin_amdgcn_exp2f(x.x - ml.x);
+                    o += *reinterpret_cast<const f32x4_t*>(smem + w * kRegion + o_at<HD>(W * c + row, chunk)) * a;
+                    ml.y = __builtin_fmaf(x.y, a, ml.y);
+                }
+            if (begins && ends) {
+                write_row<HD, BF>(p, at.b, row, kvh, chunk, o, ml);
+            } else {
+                *reinterpret_cast<f32x4_t*>(p.part_o + (int64_t)(slot * ROWS + row) * HD + chunk * 4) = o;
+                if (chunk == 0) p.part_ml[slot * ROWS + row] = ml;
+            }
+        }
+        __syncthreads();
+        line.advance(p, blockIdx.x, at);
+    }
+}
+
 // ---- many rows ----------------------------------------------------------------------
 //
 // A block has 128 rows, each wave 32 of them (or 64 rows, two waves sharing a row
@@ -555,8 +825,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 
 // Rows of K are read 16 rows at a time, 16 bytes of each, rows of V transposed, four rows by
 // 64 bytes: 16 bytes lie between rows of K, 64 between those of V and 16 more between
-// groups of four, so that the reads and the writes (16 rows of one chunk) fall on different
-// columns of 256 bytes.
+// groups of four, so that the 256 bytes of a read fall on different columns, and the 128 of a
+// write: 16 of eight rows of K, or of two rows of V in each group of four.
 template <int MODE, int HD, int ROWS, bool BF>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_wide_kernel(PagedParams p) {
     constexpr int kC = HD / 16, kD = HD / 32, kW = HD / 32;      // kW: words of codes of a lane
@@ -600,8 +870,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         int my_page = -1, my_row = 0;
         uint32_t ahead_holes = 0;  // of the tile whose codes are in flight
         Codes<HD> ck, cv;
-        const uint32_t lane_code = (uint32_t)(c16 * (HD / 2) + quarter * (HD / 8));
-        const uint32_t lane_byte = (uint32_t)(p.c.page_size * (HD / 2) + c16 * (HD / kFp4Block) + quarter * (HD / 4) / kFp4Block);
+        // the wave's keys, lanes 0..7 with values of keys whose rows' writes do not meet
+        const int vkey = (c16 & 1) | (c16 & 8) >> 2 | (c16 & 6) << 1;
+        const LaneCodes<HD> k_lane(p.c, c16, quarter), v_lane(p.c, vkey, quarter);
+        const int key16 = wave * 16 + c16, val16 = wave * 16 + vkey;
         auto fetch = [&](int i) __attribute__((always_inline)) {
             if ((i & 15) == 0) {
                 const int key = (step0 + i + (lane >> 2)) * kWideStep + (lane & 3) * 16;
@@ -612,17 +884,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             ahead_holes = (uint32_t)(__ballot(my_page < 0) >> (4 * (i & 15))) & 15;
             const int l = 4 * (i & 15) + wave;
             const int page = __builtin_amdgcn_readlane(my_page, l), row = __builtin_amdgcn_readlane(my_row, l);
-            ck.template load<false>(p.c, page, row, 0, kvh, lane_code, lane_byte);
-            cv.template load<false>(p.c, page, row, 1, kvh, lane_code, lane_byte);
+            ck.template load<false>(p.c, page, row, 0, kvh, k_lane);
+            cv.template load<false>(p.c, page, row, 1, kvh, v_lane);
         };
         const int kfull = at.keys_of(p, at.r0 / p.group) - 1;  // every row sees the keys up to it
-        const int key16 = wave * 16 + c16;
         // the tile in flight to slot i % 2
         auto stage = [&](int i) __attribute__((always_inline)) {
             unsigned char* slot = smem + (i & 1) * kSlot;
             const bool masked = (step0 + i + 1) * kWideStep - 1 > kfull || ahead_holes != 0;
             if (masked) {  // blocks of V that are NaN are zeros (0 * NaN is NaN), and marked
-                const bool hole = ahead_holes >> wave & 1, bad = cv.byte > (uint32_t)kFp4Most && !hole;
+                const bool hole = ahead_holes >> wave & 1, bad = cv.byte(v_lane) > (uint32_t)kFp4Most && !hole;
                 const uint64_t any = __ballot(bad);
                 if (bad || hole) cv.clear();
                 if (any != 0) {
@@ -630,14 +901,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
                         uint32_t m = 0;
 #pragma unroll
                         for (int q = 0; q < 4; ++q) m |= (uint32_t)(any >> (16 * q + c16) & 1) << (q * kD / 4);
-                        marks[i & 1][key16] = (uint8_t)m;
+                        marks[i & 1][val16] = (uint8_t)m;
                     }
                     if (lane == 0) marked[i & 1] = 1;
-                } else if (quarter == 0) marks[i & 1][key16] = 0;
+                } else if (quarter == 0) marks[i & 1][val16] = 0;
             }
-            const float sk = fp4_scale(ck.byte), sv = fp4_scale(cv.byte);
+            const float sk = fp4_scale(ck.byte(k_lane)), sv = fp4_scale(cv.byte(v_lane));
             unsigned char* k = slot + key16 * kRowK + quarter * kW * 16;
-            unsigned char* v = slot + kTileK + key16 * kRowV + (key16 >> 2) * 16 + quarter * kW * 16;
+            unsigned char* v = slot + kTileK + val16 * kRowV + (val16 >> 2) * 16 + quarter * kW * 16;
 #pragma unroll
             for (int c = 0; c < kW; ++c) *reinterpret_cast<bf16x8_t*>(k + c * 16) = fp4_to_bf16(ck.w[c], sk);
 #pragma unroll
@@ -668,6 +939,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         if (tiles > 0) stage(0);
         if (tiles > 1) fetch(1);
         __syncthreads();
+        if constexpr (BF)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) loaded(qf[c]);
         for (int i = 0; i < tiles; ++i) {
             const unsigned char* ks = smem + (i & 1) * kSlot + (koff + c32) * kRowK + h * 16;
             // transposing reads: row 4 h + (l % 16) / 4, columns 16 ((l / 16) % 2) + 4 (l % 4)
@@ -815,7 +1089,8 @@ __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
     const int chunk = threadIdx.x % kChunks, s = threadIdx.x / kChunks, share = s / span;
     __shared__ f32x4_t so[512];
     __shared__ float2 sml[kSlots];
-    for (int row = s % span; row < nrows; row += kSlots) {  // more than once where all slots have a row
+    const int first = s % span + (int)blockIdx.y * span;
+    for (int row = first; row < nrows; row += kSlots * (int)gridDim.y) {  // more than once where all slots have a row
         float m = kEmptyMax, l = 0.0f;
         f32x4_t o = (f32x4_t){};
         auto add = [&](float m2, float l2, f32x4_t o2) {
@@ -847,8 +1122,8 @@ __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
     }
     if (shares == 1) return;
     __syncthreads();
-    const int row = s % span;
-    if (share != 0 || row >= nrows) return;
+    if (share != 0 || first >= nrows) return;
+    const int row = first;
     float top = kEmptyMax, l = 0.0f;
     for (int u = 0; u < shares; ++u) top = __builtin_fmaxf(top, sml[s + u * span].x);
     f32x4_t o = (f32x4_t){};
@@ -871,20 +1146,31 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct PagedPlan {
     int rows;        // of a tile
+    int classes;     // of columns, for one token
     int64_t blocks;  // a fixed number: the device divides the keys among them
     int64_t bytes;   // of the workspace
 };
 
-bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, PagedPlan& p) {
+// Where columns of several groups pay: 32 sequences of 8192 keys, heads of 64, 16 ungrouped
+// ones 64 us against 75, with a softcap 63 against 89, 32 / 8 heads 39 and 40, with a softcap 40
+// and 48.  Heads of 128, 32 / 8: 57 against 54, with a softcap 58 against 63; FP16 queries, whose second
+// terms take the registers of a third block, 74 against 58 and 77 against 66.
+constexpr bool has_classes(int mode, int head_dim, bool bf) {
+    return head_dim == 64 || (bf && mode != kAttnSoftmaxNative);
+}
+
+bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, bool bf, PagedPlan& p) {
     if (!a || !fp4_sizes_ok(c, a->tokens) || a->q_heads <= 0 || a->q_heads > 65536 || a->q_heads % c->kv_heads != 0)
         return false;
     const int64_t rows = a->tokens * (a->q_heads / c->kv_heads);
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    p.blocks = device_shape().cus * (rows <= 16 ? 3 : 2);
+    p.classes = 1;
+    if (a->tokens == 1 && rows <= 8 && has_classes(a->mode, (int)c->head_dim, bf)) p.classes = rows > 4 ? 2 : 4;
+    p.blocks = device_shape().cus * (rows > 16 ? 2 : 3);
     const int64_t tiles = ceil_div(rows, p.rows);
     // places, and the steps of the line, are counted in 32 bits
     if (c->batch > 0x7fffffff / (tiles ? tiles : 1)) return false;
-    const int step = p.rows <= 32 ? kNarrowStep : kWideStep;
+    const int step = p.classes > 1 ? kDecodeStep : p.rows <= 32 ? kNarrowStep : kWideStep;
     const int64_t steps = ceil_div(c->entries * c->page_size, step) + 1 + unit_steps(step);
     if (c->batch * tiles > 0x7fffffff / (steps * c->kv_heads)) return false;
     p.bytes = p.blocks * (16 + 2 * p.rows * (c->head_dim + 2) * 4);
@@ -896,10 +1182,20 @@ void go(const PagedParams& p, int64_t blocks, hipStream_t st) {
     const dim3 grid((unsigned)blocks);
     if constexpr (ROWS <= 32) hipLaunchKernelGGL((paged_narrow_kernel<MODE, HD, ROWS / 16, BF>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((paged_wide_kernel<MODE, HD, ROWS, BF>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((paged_join_kernel<HD, ROWS, BF>), grid, dim3(512), 0, st, p);
+    hipLaunchKernelGGL((paged_join_kernel<HD, ROWS, BF>), dim3((unsigned)blocks, ROWS <= 32 ? 1 : 4), dim3(512), 0, st, p);
+}
+template <int MODE, int HD, int NC, bool BF>
+void decode(const PagedParams& p, int64_t blocks, hipStream_t st) {
+    const dim3 grid((unsigned)blocks);
+    hipLaunchKernelGGL((paged_decode_kernel<MODE, HD, NC, BF>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((paged_join_kernel<HD, 16, BF>), grid, dim3(512), 0, st, p);
 }
 template <int MODE, int HD, bool BF>
 void go(const PagedParams& p, const PagedPlan& plan, hipStream_t st) {
+    if constexpr (has_classes(MODE, HD, BF)) {
+        if (plan.classes == 4) return decode<MODE, HD, 4, BF>(p, plan.blocks, st);
+        if (plan.classes == 2) return decode<MODE, HD, 2, BF>(p, plan.blocks, st);
+    }
     if (plan.rows == 16) go<MODE, HD, 16, BF>(p, plan.blocks, st);
     else if (plan.rows == 32) go<MODE, HD, 32, BF>(p, plan.blocks, st);
     else if (plan.rows == 64) go<MODE, HD, 64, BF>(p, plan.blocks, st);
@@ -909,7 +1205,7 @@ void go(const PagedParams& p, const PagedPlan& plan, hipStream_t st) {
 template <bool BF>
 int run(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, void* stream) {
     PagedPlan plan_{};
-    if (!plan(c, a, plan_) || !(a->scale > 0.0f && a->scale <= __FLT_MAX__)) return hipErrorInvalidValue;
+    if (!plan(c, a, BF, plan_) || !(a->scale > 0.0f && a->scale <= __FLT_MAX__)) return hipErrorInvalidValue;
     if (a->mode != kAttnSoftmaxNative && a->mode != kAttnSoftcapNative && !(BF && a->mode == kAttnSoftcapD4))
         return hipErrorInvalidValue;
     if (a->mode != kAttnSoftmaxNative && !(a->cap > 0.0f && a->cap <= __FLT_MAX__)) return hipErrorInvalidValue;
@@ -957,8 +1253,9 @@ using namespace pt;
 extern "C" int64_t spline_hip_paged_fp4_workspace_bytes(const spline_hip_fp4_cache* cache,
                                                         const spline_hip_fp4_attention* args) {
     PagedPlan p{};
-    if (!plan(cache, args, p)) return -1;
-    return cache->batch == 0 || args->tokens == 0 ? 0 : p.bytes;
+    PagedPlan q{};  // the types' plans differ; the larger one
+    if (!plan(cache, args, true, p) || !plan(cache, args, false, q)) return -1;
+    return cache->batch == 0 || args->tokens == 0 ? 0 : p.bytes > q.bytes ? p.bytes : q.bytes;
 }
 extern "C" int launch_paged_fp4_attention_fp16(const spline_hip_fp4_cache* cache, const spline_hip_fp4_attention* args,
                                                void* stream) {
