@@ -33,6 +33,7 @@ namespace pt {
 constexpr int kNarrowStep = 128;  // keys of a narrow block's step
 constexpr int kWaveKeys = 32;     // of which a wave has 32
 constexpr int kWideStep = 64;
+constexpr int kPieces = 48;
 constexpr int kDecodeStep = 256;  // each wave 64 of them
 // A unit's first keys and its result cost as much as so many steps more.
 constexpr int unit_steps(int step) { return step == kWideStep ? 4 : step == kDecodeStep ? 2 : 2; }
@@ -43,7 +44,7 @@ struct PagedParams {
     AttnStrides qs;
     float* part_o;    // [2 blocks][ROWS][HD]
     float2* part_ml;  // [2 blocks][ROWS]
-    int4* cut;        // [blocks] the unit that leaves a block unfinished: place, head, pieces (0: none), first row
+    int4* cut;        // [blocks] the unit that leaves a block unfinished: batch, head and block on the line, pieces (0: none), first row
     void* out;
     float* lse;
     int hq, group, tokens, rows, tiles, capacity;
@@ -112,10 +113,12 @@ template <int ROWS, int STEP>
 struct Stretch {
     using At = Place<ROWS, STEP>;
     static constexpr int kUnit = unit_steps(STEP);
-    int each, longer, x, x1, place, kvh, in;
+    int block, each, longer, x, x1, place, kvh, in;
 
-    // False: none (and the block's cut says so).  block: its number on the line.
-    __device__ __forceinline__ bool find(const PagedParams& p, int block) {
+    // False: none (and the block's cut says so).  SHARED: neighbours on the line, which read
+    // the same keys, are on one XCD, whose L2 holds them.
+    template <bool SHARED>
+    __device__ __forceinline__ bool find(const PagedParams& p) {
         __shared__ int sums[4], start[2];
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         const int per = (p.places + 255) / 256;
@@ -138,14 +141,22 @@ struct Stretch {
         }
         ahead += inc - mine;
         const int all = plane * p.c.hkv;
-        each = all / (int)gridDim.x;
-        longer = all - each * (int)gridDim.x;
-        x = block * each + (block < longer ? block : longer);
-        x1 = x + each + (block < longer ? 1 : 0);
-        if (x == x1) {
-            if (tid == 0) p.cut[block] = make_int4(0, 0, 0, 0);
+        // With a step each, and so that the block that joins a unit's pieces has not more to do
+        // than those that make them: one sequence and KV head with 8 heads of 64 over 131072 keys
+        // 22 us, 41 with a piece a block; 4 heads of 128 25 and 57.
+        const int64_t most = (int64_t)kPieces * p.places * p.c.hkv + all / 32;
+        int blocks = (int)gridDim.x < all ? (int)gridDim.x : all;
+        blocks = blocks < most ? blocks : (int)most;
+        const int id = (int)blockIdx.x, share = (blocks + 7) / 8;
+        block = SHARED ? id % 8 * share + id / 8 : id;
+        if (block >= blocks || (SHARED && id / 8 >= share)) {
+            if (tid == 0) p.cut[id] = make_int4(0, 0, 0, 0);
             return false;
         }
+        each = all / blocks;
+        longer = all - each * blocks;
+        x = block * each + (block < longer ? block : longer);
+        x1 = x + each + (block < longer ? 1 : 0);
         kvh = x / plane;
         const int at = x - kvh * plane;
         if (at >= ahead && at < ahead + mine)
@@ -170,7 +181,7 @@ struct Stretch {
         return end < 0 ? 0 : end < steps ? end : steps;
     }
     // Goes on behind a unit.  What the block leaves unfinished is its cut.
-    __device__ __forceinline__ void advance(const PagedParams& p, int block, const At& at) {
+    __device__ __forceinline__ void advance(const PagedParams& p, const At& at) {
         const int steps = at.steps(), end = x - in + steps + kUnit;  // of the unit
         if (threadIdx.x == 0 && end >= x1) {
             int4 cut = make_int4(0, 0, 0, 0);
@@ -178,9 +189,9 @@ struct Stretch {
                 // the block with the unit's last step
                 const int to = end - 1, many = longer * (each + 1);
                 const int stop = to < many ? to / (each + 1) : longer + (to - many) / each;
-                cut = make_int4(at.b, kvh, stop - block + 1, at.r0);
+                cut = make_int4(at.b, block << 16 | kvh, stop - block + 1, at.r0);
             }
-            p.cut[block] = cut;
+            p.cut[blockIdx.x] = cut;
         }
         x = end;
         in = 0;
@@ -350,7 +361,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c16 = lane & 15, quarter = lane >> 4;
     Stretch<ROWS, kNarrowStep> line;
-    if (!line.find(p, blockIdx.x)) return;
+    if (!line.template find<false>(p)) return;
 
     ScoreConsts consts;
     consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
@@ -366,7 +377,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         const Place<ROWS, kNarrowStep> at(p, line.place);
         const int steps = at.steps(), step0 = line.first(), n = line.last(steps) - step0, kvh = line.kvh;
         if (n == 0) {
-            line.advance(p, blockIdx.x, at);
+            line.advance(p, at);
             break;
         }
         // ---- Q^T fragments: elements (HD / 4) quarter + 8 c .. of row c16
@@ -541,7 +552,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 
         // ---- the waves' shares of each row
         const bool begins = step0 == 0, ends = step0 + n == steps;
-        const int slot = 2 * (int)blockIdx.x + (begins ? 1 : 0);
+        const int slot = 2 * line.block + (begins ? 1 : 0);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
             if (nr * 16 >= at.nrows) break;
@@ -577,7 +588,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             }
         }
         __syncthreads();
-        line.advance(p, blockIdx.x, at);
+        line.advance(p, at);
     }
 }
 
@@ -601,7 +612,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c16 = lane & 15, quarter = lane >> 4, cls = c16 / W;
     Stretch<ROWS, kDecodeStep> line;
-    if (!line.find(p, blockIdx.x)) return;
+    if (!line.template find<false>(p)) return;
 
     ScoreConsts consts;
     consts.sl = attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e;
@@ -628,7 +639,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
         const Place<ROWS, kDecodeStep> at(p, line.place);
         const int steps = at.steps(), step0 = line.first(), n = line.last(steps) - step0, kvh = line.kvh;
         if (n == 0) {
-            line.advance(p, blockIdx.x, at);
+            line.advance(p, at);
             break;
         }
         // ---- Q^T fragments, the rows in every class
@@ -779,7 +790,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
 
         // ---- the shares of each row: four waves' classes
         const bool begins = step0 == 0, ends = step0 + n == steps;
-        const int slot = 2 * (int)blockIdx.x + (begins ? 1 : 0);
+        const int slot = 2 * line.block + (begins ? 1 : 0);
         __syncthreads();  // the region is free
 #pragma unroll
         for (int dt = 0; dt < kD; ++dt) *reinterpret_cast<f32x4_t*>(vt + o_at<HD>(c16, 4 * dt + quarter)) = st.o[dt];
@@ -812,7 +823,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
             }
         }
         __syncthreads();
-        line.advance(p, blockIdx.x, at);
+        line.advance(p, at);
     }
 }
 
@@ -841,10 +852,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     __shared__ int marked[2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int h = lane >> 5, c32 = lane & 31, c16 = lane & 15, quarter = lane >> 4;
-    // neighbours on the line share keys: they go to one XCD, whose L2 holds them
-    const int block = (int)(gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x);
     Stretch<ROWS, kWideStep> line;
-    if (!line.find(p, block)) return;
+    if (!line.template find<true>(p)) return;
 
     ScoreConsts consts;
     consts.sl = vgpr(attn_is_plain_softmax(MODE) ? p.scale * kLog2e : kLog2e);
@@ -861,7 +870,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         const Place<ROWS, kWideStep> at(p, line.place);
         const int steps = at.steps(), step0 = line.first(), n = line.last(steps) - step0, kvh = line.kvh;
         if (n == 0) {
-            line.advance(p, block, at);
+            line.advance(p, at);
             break;
         }
 
@@ -1050,7 +1059,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         if (h == 0) sml[wave][c32] = make_float2(st.m, l);
         __syncthreads();
         const bool begins = step0 == 0, ends = step0 + n == steps;
-        const int slot = 2 * block + (begins ? 1 : 0);
+        const int slot = 2 * line.block + (begins ? 1 : 0);
         constexpr int kChunks = HD / 4;
         for (int i = tid; i < at.nrows * kChunks; i += 256) {
             const int orow = i / kChunks, chunk = i % kChunks, w = orow >> 5, r = orow & 31;
@@ -1070,17 +1079,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
                 if (chunk == 0) p.part_ml[slot * ROWS + orow] = ml;
             }
         }
-        line.advance(p, block, at);
+        line.advance(p, at);
     }
 }
 
-// Joins the pieces of the unit that leaves block blockIdx.x unfinished.  HD / 4 lanes
+// Joins the pieces of the unit of a block's cut.  HD / 4 lanes
 // hold a row, and the groups of them beyond the rows take the pieces in turn.
 template <int HD, int ROWS, bool BF>
 __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
     constexpr int kChunks = HD / 4, kSlots = 512 / kChunks;  // row slots
     const int4 cut = p.cut[blockIdx.x];
-    const int pieces = cut.z;
+    const int pieces = cut.z, block = cut.y >> 16, kvh = cut.y & 0xffff;
     if (pieces == 0) return;
     const int nrows = p.rows - cut.w < ROWS ? p.rows - cut.w : ROWS;
     int span = 1;  // a power of two that holds the rows
@@ -1106,7 +1115,7 @@ __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int j = i + u * shares < pieces ? i + u * shares : i;
-                const int slot = 2 * ((int)blockIdx.x + j) + (j == 0 ? 1 : 0);
+                const int slot = 2 * (block + j) + (j == 0 ? 1 : 0);
                 ml[u] = p.part_ml[slot * ROWS + row];
                 part[u] = *reinterpret_cast<const f32x4_t*>(p.part_o + (int64_t)(slot * ROWS + row) * HD + chunk * 4);
             }
@@ -1118,7 +1127,7 @@ __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
             so[threadIdx.x] = o;
             if (chunk == 0) sml[s] = make_float2(m, l);
         }
-        if (shares == 1) write_row<HD, BF>(p, cut.x, cut.w + row, cut.y, chunk, o, make_float2(m, l));
+        if (shares == 1) write_row<HD, BF>(p, cut.x, cut.w + row, kvh, chunk, o, make_float2(m, l));
     }
     if (shares == 1) return;
     __syncthreads();
@@ -1133,7 +1142,7 @@ __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
         o += so[threadIdx.x + u * span * kChunks] * a;
         l = __builtin_fmaf(ml.y, a, l);
     }
-    write_row<HD, BF>(p, cut.x, cut.w + row, cut.y, chunk, o, make_float2(top, l));
+    write_row<HD, BF>(p, cut.x, cut.w + row, kvh, chunk, o, make_float2(top, l));
 }
 
 // ---- host side -----------------------------------------------------------------

@@ -48,14 +48,14 @@ def same(a, b):
         pytest.fail(f"{int(bad.sum())} of {bad.numel()} differ, first at {at}: {a[at]} for {b[at]}")
 
 
-def sequence(cache, dim, table, length):
-    """Keys and values [keys, hkv, dim] of a row of the table, and which of them there are."""
-    v = numbers(cache, dim)
+def sequence(v, table, length):
+    """Keys and values [keys, hkv, dim] of a row of the table, and which of them there are, from the
+    cache's numbers."""
     size = v.shape[3]
     n = min(max(int(length), 0), len(table) * size)
     pages = [int(table[x // size]) for x in range(n)]
-    there = torch.tensor([0 <= p < cache.shape[0] for p in pages], dtype=torch.bool)
-    where = torch.tensor([p if 0 <= p < cache.shape[0] else 0 for p in pages], dtype=torch.long)
+    there = torch.tensor([0 <= p < v.shape[0] for p in pages], dtype=torch.bool)
+    where = torch.tensor([p if 0 <= p < v.shape[0] else 0 for p in pages], dtype=torch.long)
     rows = torch.arange(n) % size
     return v[where, 0, :, rows], v[where, 1, :, rows], there
 
@@ -77,8 +77,9 @@ def attention(q, cache, table, lens, scale, cap=0.0):
     lse, tol_l = torch.full((b, hq, t), -math.inf, dtype=torch.float64), torch.zeros(b, hq, t, dtype=torch.float64)
     group = hq // cache.shape[2]
     r = 2.0 ** -8 if q.dtype == torch.bfloat16 and t * group > 32 else 2.0 ** -16
+    held = numbers(cache, d)
     for i in range(b):
-        k, v, there = sequence(cache, d, table[i].tolist(), lens[i])
+        k, v, there = sequence(held, table[i].tolist(), lens[i])
         for j in range(t):
             c = max(0, min(max(int(lens[i]), 0) - t + j + 1, k.shape[0]))
             if not there[:c].any():
@@ -98,6 +99,44 @@ def attention(q, cache, table, lens, scale, cap=0.0):
             tol_o[i, j] = (r + 2 * err + c * 2.0 ** -22)[:, None] * size + out[i, j].abs() * u * 1.01 + least
             tol_l[i, :, j] = err + c * 2.0 ** -22 + 1e-6 * z.abs()
     return out, lse, tol_o, tol_l
+
+
+def attention_at_scale(q, cache, table, lens, scale, cap=0.0):
+    """The same of whole sequences whose pages are all there, on the operands' device."""
+    b, t, hq, d = q.shape
+    u, group = torch.finfo(q.dtype).eps / 2, hq // cache.shape[2]
+    least = torch.finfo(q.dtype).smallest_normal * u  # half a step of what is not normal
+    r = 2.0 ** -8 if q.dtype == torch.bfloat16 and t * group > 32 else 2.0 ** -16
+    out, tol_o = (torch.zeros(b, t, hq, d, dtype=torch.float64, device=q.device) for _ in range(2))
+    lse, tol_l = (torch.zeros(b, hq, t, dtype=torch.float64, device=q.device) for _ in range(2))
+    half, size = d // 2, cache.shape[-1] // (d // 2 + d // 32)
+    lut = torch.cat([CODES, -CODES]).to(q.device)
+    for i in range(b):
+        n = int(lens[i])
+        pages = table[i, : -(-n // size)].long()
+        hidden = torch.arange(n, device=q.device) > n - t + torch.arange(t, device=q.device)[:, None]  # [t, n]
+        for h in range(cache.shape[2]):
+            kv = []
+            for x in cache[pages, :, h].unbind(1):
+                codes = x[:, : size * half].reshape(-1, half)[:n].long()
+                scale2 = torch.exp2(x[:, size * half:].reshape(-1, d // 32)[:n].double() - 127)
+                kv.append(lut[torch.stack([codes & 15, codes >> 4], -1).flatten(1)] * scale2.repeat_interleave(32, 1))
+            k, v = kv
+            heads = slice(h * group, (h + 1) * group)
+            x = q[i, :, heads].reshape(-1, d).double()
+            s = (x @ k.t().contiguous() * scale).view(t, group, n)
+            err = (x.abs() @ k.abs().t().contiguous()).amax(1).view(t, group) * scale * 2 * d * 2.0 ** -24 + 1e-5
+            if cap:
+                s, err = cap * torch.tanh(s / cap), err + 4e-7 * cap
+            s = s.masked_fill(hidden[:, None], -math.inf)
+            z = torch.logsumexp(s, -1)
+            p = torch.exp(s - z[..., None])
+            out[i, :, heads] = (p.view(-1, n) @ v).view(t, group, d)
+            total = (p.view(-1, n) @ v.abs()).view(t, group, d)
+            lse[i, heads] = z.t()
+            tol_o[i, :, heads] = (r + 2 * err + n * 2.0 ** -22)[..., None] * total + out[i, :, heads].abs() * u * 1.01 + least
+            tol_l[i, heads] = (err + n * 2.0 ** -22 + 1e-6 * z.abs()).t()
+    return tuple(x.cpu() for x in (out, lse, tol_o, tol_l))
 
 
 def check(got, want):
