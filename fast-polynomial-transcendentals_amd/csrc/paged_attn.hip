@@ -5,8 +5,8 @@
 //   s = q.k scale, or cap tanh(q.k scale / cap)
 //
 // The T g rows of a sequence and KV head (g query heads to a KV head) are cut into
-// tiles of 16 or 32; a tile, its keys and a KV head are a unit.  The keys of
-// all units, laid end to end in steps of 128, are divided evenly among a fixed number of
+// tiles of 16, 32, 64 or 128; a tile, its keys and a KV head are a unit.  The keys of
+// all units, laid end to end in steps, are divided evenly among a fixed number of
 // blocks, whatever the lengths are: a block takes its stretch of this line, which
 // may begin inside a unit and reach over several.  A unit within one block leaves
 // as its result; the pieces of one that is cut leave O, maximum and sum in FP32,
@@ -14,13 +14,22 @@
 // O = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  So neither time nor workspace goes
 // by what the table could hold.
 //
-// Of a step's 128 keys each of a block's four waves has 32, and none waits for
-// another.  Products are S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32, a
-// lane keeping one row (query).  K needs no LDS: the sum over the head dimension may take
-// its elements in any order, so a lane loads 16 bytes of a key, 32 elements of one
-// block, and turns each word into a fragment of K (v_cvt_scalef32_pk_bf16_fp4, exact);
-// Q's fragments follow that order.  V has to be turned by keys: BF16 rows in the
-// wave's own LDS, read back transposed (ds_read_b64_tr_b16).
+// Up to 32 rows ("narrow"): of a step's 128 keys each of a block's four waves has 32, and
+// none waits for another.  Products are S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_16x16x32, a lane keeping one row (query).  K needs no LDS: the sum over the head
+// dimension may take its elements in any order, so a lane loads 16 bytes of a key, 32 elements
+// of one block, and turns each word into a fragment of K (v_cvt_scalef32_pk_bf16_fp4,
+// exact); Q's fragments follow that order.  V has to be turned by keys: BF16 rows in the
+// wave's own LDS, read back transposed (ds_read_b64_tr_b16).  One token's rows have a form
+// of their own where it pays (below), and so have more than 32 rows.
+//
+// What bounds it: with few rows the bytes of K and V (17 a block of 32 elements), whose loads
+// alone take 91 us where 64 sequences of up to 16384 keys (571 MB) take 103 to 109, 6.2 TB/s a
+// further key and 15 us a call; from about 64 rows a KV head on the matrix cores and the
+// exponentials and conversions beside them: 4 x 512 tokens over 17408 keys 591 us, 974 TFLOP/s, over up
+// to 8700 keys each 178 us, 820 TFLOP/s, where first keys and results of 512 units count.
+// Two sequences of up to 131072 keys take 39 us, 8 of up to 1200 12 us, most of it latency: lengths,
+// table, codes and the join one behind the other.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -30,13 +39,16 @@
 
 namespace pt {
 
-constexpr int kNarrowStep = 128;  // keys of a narrow block's step
-constexpr int kWaveKeys = 32;     // of which a wave has 32
+// Keys of a block's step
+constexpr int kNarrowStep = 128;  // each wave 32 of them
+constexpr int kWaveKeys = 32;
+constexpr int kDecodeStep = 256;  // each wave 64
 constexpr int kWideStep = 64;
-constexpr int kPieces = 48;
-constexpr int kDecodeStep = 256;  // each wave 64 of them
-// A unit's first keys and its result cost as much as so many steps more.
-constexpr int unit_steps(int step) { return step == kWideStep ? 4 : step == kDecodeStep ? 2 : 2; }
+constexpr int kPieces = 48;       // blocks that a unit is cut into, besides one per 32 of its steps, at most
+// A unit's first keys and its result cost as much as so many steps more: 4 x 512 tokens
+// over up to 8700 keys 262 us counting none, 222 with one, 202 with two, 188 with four, 190 with
+// eight; 64 decoding sequences 136, 131 with one or two, 135 with four.
+constexpr int unit_steps(int step) { return step == kWideStep ? 4 : 2; }
 
 struct PagedParams {
     const uint16_t* q;
@@ -44,7 +56,8 @@ struct PagedParams {
     AttnStrides qs;
     float* part_o;    // [2 blocks][ROWS][HD]
     float2* part_ml;  // [2 blocks][ROWS]
-    int4* cut;        // [blocks] the unit that leaves a block unfinished: batch, head and block on the line, pieces (0: none), first row
+    int4* cut;        // [blocks] the unit that leaves a block unfinished: batch, KV head and (from bit 16
+                      // on) the block's number on the line, pieces (0: no such unit), first row
     void* out;
     float* lse;
     int hq, group, tokens, rows, tiles, capacity;
@@ -350,7 +363,7 @@ struct PagedState {
     }
 };
 
-// A block's stretch of the line, and what its waves need throughout.
+// Up to 32 rows: NR tiles of 16, which share a wave's fragments of K and V.
 template <int MODE, int HD, int NR, bool BF>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? (HD == 64 ? 4 : 3) : 2))) paged_narrow_kernel(PagedParams p) {
     constexpr int ROWS = 16 * NR, kC = HD / 32, kD = HD / 16;
@@ -1149,8 +1162,6 @@ __global__ void __launch_bounds__(512) paged_join_kernel(PagedParams p) {
 
 namespace {
 
-constexpr int64_t kMaxBlocks = 0xffffffffll / 256;
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct PagedPlan {
@@ -1175,7 +1186,7 @@ bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, bool
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.classes = 1;
     if (a->tokens == 1 && rows <= 8 && has_classes(a->mode, (int)c->head_dim, bf)) p.classes = rows > 4 ? 2 : 4;
-    p.blocks = device_shape().cus * (rows > 16 ? 2 : 3);
+    p.blocks = ceil_div(device_shape().cus * (rows > 16 ? 2 : 3), 8) * 8;  // whole rows of XCDs
     const int64_t tiles = ceil_div(rows, p.rows);
     // places, and the steps of the line, are counted in 32 bits
     if (c->batch > 0x7fffffff / (tiles ? tiles : 1)) return false;

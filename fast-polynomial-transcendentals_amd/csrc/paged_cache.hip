@@ -482,8 +482,6 @@ __global__ void __launch_bounds__(256) move_pages_kernel(PagePlan p, PageCaches 
 
 namespace {
 
-constexpr int64_t kMaxBlocks = 0xffffffffll / 256;
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool rows_ok(const void* x, const int64_t* s) {
@@ -548,7 +546,8 @@ int64_t lay_out(const spline_hip_pages* a, bool fork, PagePlan& p, char* ws) {
                    a->grow > kFp4MostKeys / 2
              : a->rows != a->old_rows)
         return -1;
-    if (a->rows * a->entries > kMaxBlocks * 256) return -1;
+    // entries, and the pages that all rows may want, are counted in 32 bits
+    if (a->rows * (a->entries + 2 + (fork ? ceil_div(a->grow, a->page_size) : 0)) > 0x7fffffff) return -1;
     int64_t bytes = 0;
     auto take = [&](int64_t n) {
         char* at = ws + bytes;

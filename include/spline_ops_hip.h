@@ -825,7 +825,8 @@ int launch_paged_fp4_load_bf16(const spline_hip_fp4_cache* cache, void* k, void*
  * operands and more than 32 rows to a KV head (T Hq / Hkv).  A NaN block in a
  * key that a token sees makes its row NaN, in a value its elements; what nobody sees
  * may hold anything.  Time and workspace go by the keys in use, not by the table's
- * width.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the same
+ * width.  Refused are more than 2^31 steps of 64 keys, over the tables' width, the KV
+ * heads and every 64 rows.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the same
  * device (-1: sizes that are refused), 16-byte aligned; calls that may overlap need
  * workspaces of their own. */
 typedef struct spline_hip_fp4_attention {
@@ -866,7 +867,8 @@ int launch_paged_fp4_attention_bf16(const spline_hip_fp4_cache* cache, const spl
  *
  * out_table [rows][entries], out_lens [rows] and out_count [1] are not the inputs'
  * memory.  workspace: as the size helpers say (-1: refused), 16-byte aligned, one for
- * each call that may overlap.  At most 2^24 rows and entries, 2^32 cells. */
+ * each call that may overlap.  At most 2^24 rows and entries, and 2^31 entries and pages
+ * for `grow` keys of all rows. */
 typedef struct spline_hip_pages {
     int32_t *out_table, *out_lens, *out_count;
     const int32_t *table, *lens, *parents;

@@ -182,6 +182,15 @@ def test_page_workspaces(lib):
     assert lib.launch_fork_pages(None, None) == 1 and lib.launch_compact_pages(None, None) == 1
 
 
+def test_wishes_are_counted_in_32_bits(lib):
+    size = lib.spline_hip_fork_pages_workspace_bytes
+    rows = dict(rows=2 ** 20, old_rows=2 ** 20, entries=6, page_size=64)
+    assert size(_pages(**rows, grow=64 * 2000)) > 0  # 2^20 rows of 6 + 2 + 2000 pages
+    for grow in (64 * 2040, 2 ** 28):
+        assert size(_pages(**rows, grow=grow)) == -1
+        assert lib.launch_fork_pages(_pages(**rows, grow=grow), None) == 1
+
+
 def test_python_refuses_host_tensors():
     from sfu_repro import fa4_runtime, paged_cache
 
