@@ -1155,6 +1155,11 @@ void check_no_grad(std::initializer_list<const at::Tensor*> operands, const char
     refuse_tangents(operands, what);
 }
 
+// A tensor that a call wrote in place: autograd refuses a backward through what it saved of it.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void paged_fp4_store(at::Tensor cache, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor lens) {
     check_no_grad({&k, &v}, "store_fp4");
     check_heads(k, "k", "[batch, tokens, kv_heads, head_dim]");
@@ -1175,6 +1180,7 @@ void paged_fp4_store(at::Tensor cache, at::Tensor k, at::Tensor v, at::Tensor ta
     check_launch((k.scalar_type() == at::kBFloat16 ? launch_paged_fp4_store_bf16 : launch_paged_fp4_store_fp16)(
                      &c, kr.data_ptr(), vr.data_ptr(), ks, vs, k.size(1), s),
                  s);
+    written(cache);
 }
 
 std::vector<at::Tensor> paged_fp4_load(at::Tensor cache, at::Tensor table, at::Tensor lens, int64_t tokens,
@@ -1234,11 +1240,12 @@ std::vector<at::Tensor> paged_fp4_attn_fwd(at::Tensor q, at::Tensor cache, at::T
 // The caches whose pages move with a table, and the table.
 struct PageCall {
     spline_hip_pages a{};
+    std::vector<at::Tensor> caches;
     std::vector<void*> at;
     std::vector<int64_t> bytes;
     at::Tensor table, out, count, workspace;
 
-    PageCall(const std::vector<at::Tensor>& caches, const at::Tensor& table_) : table(table_) {
+    PageCall(const std::vector<at::Tensor>& caches_, const at::Tensor& table_) : caches(caches_), table(table_) {
         TORCH_CHECK(!caches.empty(), "caches must hold at least one cache");
         TORCH_CHECK(table.is_cuda() && table.scalar_type() == at::kInt && table.dim() == 2,
                     "table must be an int32 CUDA tensor [rows, entries]");
@@ -1275,6 +1282,7 @@ struct PageCall {
         a.workspace = workspace.data_ptr();
         void* s = current_stream(table);
         check_launch(fn(&a, s), s);
+        for (const at::Tensor& t : caches) written(t);
     }
 };
 

@@ -40,6 +40,12 @@ def _ops():
     return spline_ops
 
 
+def _several(caches) -> list:
+    if isinstance(caches, torch.Tensor):  # a list of its pages
+        raise TypeError("caches must be a sequence of caches, one a layer, not one tensor")
+    return list(caches)
+
+
 def fp4_cache(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, *, device=None) -> torch.Tensor:
     """A cache of ``pages`` pages, all zeros.  head_dim 64 or 128, page_size a multiple of 16."""
     if head_dim not in (64, 128):
@@ -92,7 +98,7 @@ def fork_pages(caches, table: torch.Tensor, lens: torch.Tensor, parents: torch.T
     the table's width among them; their entries are -1, and a row whose copy is missing has lost the
     keys of its last page.  The table and lengths given are left as they are.
     """
-    return tuple(_ops().fork_pages(list(caches), table, lens, parents, int(tokens), int(page_size)))
+    return tuple(_ops().fork_pages(_several(caches), table, lens, parents, int(tokens), int(page_size)))
 
 
 def compact_pages(caches, table: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -100,7 +106,7 @@ def compact_pages(caches, table: torch.Tensor) -> tuple[torch.Tensor, torch.Tens
     (as in :func:`fork_pages`, written in place).  Of ``used`` pages (int32 ``[1]``) those with
     numbers from ``used`` on move to the free ones below, both in ascending order; entries
     that named no page are -1.  The table given is left as it is."""
-    return tuple(_ops().compact_pages(list(caches), table))
+    return tuple(_ops().compact_pages(_several(caches), table))
 
 
 __all__ = ["compact_pages", "fork_pages", "fp4_cache", "load_fp4", "store_fp4"]

@@ -412,3 +412,46 @@ def test_refusals(cuda):
                           (lambda: paged_cache.compact_pages([cache], table.float()), "int32")):
         with pytest.raises(RuntimeError, match=message):
             call()
+
+
+def test_a_written_cache_is_not_what_autograd_saved(cuda):
+    from sfu_repro import paged_cache
+
+    cache = paged_cache.fp4_cache(4, 2, 128, 16, device=cuda)
+    wide = torch.randn(4, 2, 16, device=cuda)
+    table, lens = torch.tensor([[0, 3]], dtype=torch.int32, device=cuda), torch.tensor([20], dtype=torch.int32, device=cuda)
+    k = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16, device=cuda)
+    for call, changed in ((lambda: paged_cache.store_fp4(cache, k, k, table, lens), (cache,)),
+                          (lambda: paged_cache.fork_pages((cache, wide), table, lens, page_size=16), (cache, wide)),
+                          (lambda: paged_cache.compact_pages((cache, wide), table), (cache, wide))):
+        before = [t._version for t in changed]
+        call()
+        assert all(t._version > v for t, v in zip(changed, before))
+    version = cache._version
+    paged_cache.load_fp4(cache, table, lens, 1, 128)
+    assert cache._version == version
+    x = torch.ones(4, 2, 16, device=cuda, requires_grad=True)
+    y = (x * wide).sum()
+    paged_cache.fork_pages((wide,), table, lens, page_size=16)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():  # such tensors have no version
+        cache = paged_cache.fp4_cache(4, 2, 128, 16, device=cuda)
+    paged_cache.store_fp4(cache, k, k, table, lens)
+    paged_cache.fork_pages((cache,), table, lens, page_size=16)
+    paged_cache.compact_pages((cache,), table)
+
+
+def test_a_cache_that_is_named_twice(cuda):
+    """Its pages are copied twice, from where they were to where they go."""
+    from sfu_repro import paged_cache
+
+    before = _noise(9, 2, 2, 16 * 68, seed=5).to(cuda)
+    table = torch.tensor([[8, 2], [7, 6]], dtype=torch.int32, device=cuda)
+    lens, parents = torch.tensor([20, 31], dtype=torch.int32, device=cuda), torch.tensor([0, 0, 1, 1], dtype=torch.int32, device=cuda)
+    for call in (lambda caches: paged_cache.fork_pages(caches, table, lens, parents, tokens=17, page_size=16),
+                 lambda caches: paged_cache.compact_pages(caches, table)):
+        one, two = before.clone(), before.clone()
+        for a, b in zip(call([one]), call([two, two])):
+            assert torch.equal(a, b)
+        assert torch.equal(one, two) and not torch.equal(one, before)

@@ -269,3 +269,13 @@ def test_forking_and_compacting():
     assert n.tolist() == [20, 20, 16, 0] and short == 0 and moves == [(7, 0)]
     assert ref.compact(out, 9)[0].tolist() == [[4, 3, -1], [4, 0, -1], [2, 1, -1], [-1, -1, -1]]
     assert ref.compact(out, 9)[1:] == (5, [(7, 3)])
+
+
+def test_one_tensor_is_not_a_list_of_caches():
+    from sfu_repro import paged_cache
+
+    cache, table, lens = paged_cache.fp4_cache(2, 2, 64, 16), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(TypeError, match="sequence of caches"):
+        paged_cache.fork_pages(cache, table, lens, page_size=16)
+    with pytest.raises(TypeError, match="sequence of caches"):
+        paged_cache.compact_pages(cache, table)
