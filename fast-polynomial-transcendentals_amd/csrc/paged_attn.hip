@@ -846,6 +846,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
 // and halving each tile's keys), on v_mfma_f32_32x32x16 (row_state.hpp).  All waves share
 // tiles of 64 keys, which they turn into BF16 rows in LDS, each wave 16 keys, a tile
 // ahead; the codes of the tile behind that are in flight meanwhile.
+//
+// P enters P V in two BF16 terms, as in the kernels of fewer rows: a token's result is as exact,
+// whether it is decoded alone, verified among a few or part of a prompt.  One term, off by
+// 2^-8, is as large an error as the result's own rounding (root mean square 0.0023 instead of 0.0017)
+// and saves its products: 32 x 5 tokens over up to 4100 keys take 38 us with it, 43 with two,
+// 4 x 512 over 17408 keys 588 and 781.
 
 // Rows of K are read 16 rows at a time, 16 bytes of each, rows of V transposed, four rows by
 // 64 bytes: 16 bytes lie between rows of K, 64 between those of V and 16 more between
@@ -971,7 +977,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             const unsigned char* vs = smem + (i & 1) * kSlot + kTileK + tr * kRowV + (tr >> 2) * 16 + (quarter & 1) * 32 + (lane & 3) * 8;
             const int key0 = (step0 + i) * kWideStep;
             const bool masked = key0 + kWideStep - 1 > kfull || holes != 0;
-            constexpr int kTerms = BF ? 1 : 2;  // products a fragment of K or V
+            constexpr int kTerms = BF ? 1 : 2;  // products a fragment of K
             f32x16_t s[NT];
             // fragments of K are read six ahead of their products
             __builtin_amdgcn_sched_barrier(0);
@@ -1016,14 +1022,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             }
             const float mul = score_state<kAttnSoftmaxNative, HD, true, NT, false>(s, st, consts, 0);
             score_exps<HD, NT>(s, st, mul);
-            // fragments of V (two reads each) three ahead
+            // the compiler's order of reads and products: fragments of V three ahead take 788 us where it takes
+            // 781 (4 x 512 tokens over 17408 keys)
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int g = 0; g < 2 * NT; ++g) {
                 const bf16x8_t pf = prob_frag<true>(s[g >> 1], g & 1);
-                bf16x8_t rest;
-                if constexpr (!BF) rest = prob_rest<true>(s[g >> 1], g & 1, pf);
+                const bf16x8_t rest = prob_rest<true>(s[g >> 1], g & 1, pf);
 #pragma unroll
                 for (int dt = 0; dt < kD; ++dt) {
                     const uint16_t* vp = reinterpret_cast<const uint16_t*>(vs + g * (16 * kRowV + 64) + dt * 64);
@@ -1031,16 +1037,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
                     const u32x2_t hi = __builtin_bit_cast(u32x2_t, lds_read_tr16(vp + (8 * kRowV + 32) / 2));
                     const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, (u32x4_t){lo.x, lo.y, hi.x, hi.y});
                     st.o[dt] = mfma32(vf, pf, st.o[dt]);
-                    if constexpr (!BF) st.o[dt] = mfma32(vf, rest, st.o[dt]);
+                    st.o[dt] = mfma32(vf, rest, st.o[dt]);
                 }
             }
-            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-            for (int g = 0; g < 2 * NT * kD - 3; ++g) {
-                __builtin_amdgcn_sched_group_barrier(0x008, kTerms, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, 3 * kTerms, 0);
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(0);
             if (masked && marked[i & 1] != 0)

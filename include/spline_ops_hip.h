@@ -821,10 +821,9 @@ int launch_paged_fp4_load_bf16(const spline_hip_fp4_cache* cache, void* k, void*
  * launch_shared_prefix_attention_bf16, and so are rows without a key (zeros, -inf),
  * the score programs (mode 0, 3, and 4 with BF16 operands) and scale.  Keys and
  * values enter the products exactly, FP16 queries as two BF16 terms;
- * sums are FP32; ahead of P V probabilities are BF16 in two terms, in one with BF16
- * operands and more than 32 rows to a KV head (T Hq / Hkv).  A NaN block in a
- * key that a token sees makes its row NaN, in a value its elements; what nobody sees
- * may hold anything.  Time and workspace go by the keys in use, not by the table's
+ * sums are FP32; ahead of P V probabilities are BF16 in two terms, for any number of
+ * tokens.  A NaN block in a key that a token sees makes its row NaN, in a value its
+ * elements; what nobody sees may hold anything.  Time and workspace go by the keys in use, not by the table's
  * width.  Refused are more than 2^31 steps of 64 keys, over the tables' width, the KV
  * heads and every 64 rows.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the same
  * device (-1: sizes that are refused), 16-byte aligned; calls that may overlap need
