@@ -44,7 +44,12 @@ constexpr int kNarrowStep = 128;  // each wave 32 of them
 constexpr int kWaveKeys = 32;
 constexpr int kDecodeStep = 256;  // each wave 64
 constexpr int kWideStep = 64;
-constexpr int kPieces = 48;       // blocks that a unit is cut into, besides one per 32 of its steps, at most
+// A block's stretch is so long that the longest unit is cut into at most this many pieces, one more for each
+// 32 of its steps, and one where it begins inside a stretch: the blocks that join a unit have not more to do
+// than those that make its pieces.  One KV head, 131072 keys: with 8 heads of 64 21 us, 41 with a piece a
+// block; 4 heads of 128 26 and 57; 8 of 128 beside 15 sequences of 100 keys 29, 66 where the pieces of all
+// units are counted together, so that the short ones leave theirs to the long one.
+constexpr int kPieces = 64;
 // A unit's first keys and its result cost as much as so many steps more: 4 x 512 tokens
 // over up to 8700 keys 262 us counting none, 222 with one, 202 with two, 188 with four, 190 with
 // eight; 64 decoding sequences 136, 131 with one or two, 135 with four.
@@ -132,34 +137,43 @@ struct Stretch {
     // the same keys, are on one XCD, whose L2 holds them.
     template <bool SHARED>
     __device__ __forceinline__ bool find(const PagedParams& p) {
-        __shared__ int sums[4], start[2];
+        __shared__ int sums[4], most[4], start[2];
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         const int per = (p.places + 255) / 256;
         const int64_t first = (int64_t)tid * per;
         const int from = first < p.places ? (int)first : p.places, to = p.places - from < per ? p.places : from + per;
         int mine = 0, plane = 0, ahead = 0;  // steps of the thread's places, of a KV head, ahead
-        for (int i = from; i < to; ++i) mine += At(p, i).length();
+        int top = 0;                         // the thread's longest place
+        for (int i = from; i < to; ++i) {
+            const int n = At(p, i).length();
+            mine += n;
+            top = n > top ? n : top;
+        }
         int inc = mine;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const int y = __shfl_up(inc, d);
             inc += lane >= d ? y : 0;
+            const int z = __shfl_xor(top, d);
+            top = z > top ? z : top;
         }
-        if (lane == 63) sums[wave] = inc;
+        if (lane == 63) {
+            sums[wave] = inc;
+            most[wave] = top;
+        }
         __syncthreads();
+        int longest = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             ahead += w < wave ? sums[w] : 0;
             plane += sums[w];
+            longest = most[w] > longest ? most[w] : longest;
         }
         ahead += inc - mine;
         const int all = plane * p.c.hkv;
-        // With a step each, and so that the block that joins a unit's pieces has not more to do
-        // than those that make them: one sequence and KV head with 8 heads of 64 over 131072 keys
-        // 22 us, 41 with a piece a block; 4 heads of 128 25 and 57.
-        const int64_t most = (int64_t)kPieces * p.places * p.c.hkv + all / 32;
-        int blocks = (int)gridDim.x < all ? (int)gridDim.x : all;
-        blocks = blocks < most ? blocks : (int)most;
+        const int pieces = kPieces + longest / 32, least = (longest + pieces - 1) / pieces;  // steps of a stretch
+        int blocks = all / least;
+        blocks = blocks < (int)gridDim.x ? blocks : (int)gridDim.x;
         const int id = (int)blockIdx.x, share = (blocks + 7) / 8;
         block = SHARED ? id % 8 * share + id / 8 : id;
         if (block >= blocks || (SHARED && id / 8 >= share)) {
