@@ -1140,6 +1140,23 @@ void fill_fp4_cache(spline_hip_fp4_cache& c, const at::Tensor& cache, at::Tensor
     c.table_stride = table.size(0) > 1 ? table.stride(0) : 0;
 }
 
+// The limits of fp4_sizes_ok that shapes can pass, by name.
+void check_fp4_sizes(const spline_hip_fp4_cache& c, int64_t tokens) {
+    TORCH_CHECK(c.page_size <= 65536, "a page holds at most 65536 rows, got ", c.page_size);
+    TORCH_CHECK(c.kv_heads >= 1 && c.kv_heads <= 65536, "a cache has 1 to 65536 kv heads, got ", c.kv_heads);
+    TORCH_CHECK(c.entries <= (int64_t(1) << 30) / c.page_size, "a row of the table holds at most 2^30 keys, got ", c.entries,
+                " entries of ", c.page_size);
+    TORCH_CHECK(tokens <= 16384 || tokens <= c.entries * c.page_size, "more than 16384 tokens have to fit a row of the table (",
+                c.entries, " entries of ", c.page_size, " keys), got ", tokens);
+}
+// A store or load counts vectors of eight elements in 32 bits.
+void check_fp4_elements(const spline_hip_fp4_cache& c, int64_t tokens) {
+    check_fp4_sizes(c, tokens);
+    TORCH_CHECK(tokens == 0 || c.batch <= 0x7fffff00ll / (c.kv_heads * c.head_dim / 8) / tokens,
+                "a call holds fewer than 2^34 elements of keys, got ", c.batch, " x ", tokens, " tokens of ", c.kv_heads,
+                " x ", c.head_dim);
+}
+
 // The operand as rows of a contiguous head dimension, pointer and strides whole
 // multiples of 16 bytes, or a copy of it.
 at::Tensor wide_rows(const at::Tensor& t) {
@@ -1171,6 +1188,7 @@ void paged_fp4_store(at::Tensor cache, at::Tensor k, at::Tensor v, at::Tensor ta
     TORCH_CHECK(k.get_device() == cache.get_device(), "k must be on the same CUDA device as cache");
     TORCH_CHECK(k.size(0) == c.batch, "table must hold k's batch");
     TORCH_CHECK(k.size(2) == c.kv_heads, "k must have the cache's kv heads (", c.kv_heads, "), got ", k.size(2));
+    check_fp4_elements(c, k.size(1));
     c10::OptionalDeviceGuard guard(cache.device());
     const at::Tensor kr = wide_rows(k), vr = wide_rows(v);
     int64_t ks[3], vs[3];
@@ -1189,6 +1207,7 @@ std::vector<at::Tensor> paged_fp4_load(at::Tensor cache, at::Tensor table, at::T
     TORCH_CHECK(tokens >= 0, "tokens must not be negative, got ", tokens);
     spline_hip_fp4_cache c{};
     fill_fp4_cache(c, cache, table, lens, head_dim);
+    check_fp4_elements(c, tokens);
     c10::OptionalDeviceGuard guard(cache.device());
     at::Tensor k = at::empty({c.batch, tokens, c.kv_heads, head_dim}, cache.options().dtype(dtype));
     at::Tensor v = at::empty_like(k);
@@ -1208,6 +1227,7 @@ std::vector<at::Tensor> paged_fp4_attn_fwd(at::Tensor q, at::Tensor cache, at::T
     TORCH_CHECK(q.get_device() == cache.get_device(), "q must be on the same CUDA device as cache");
     TORCH_CHECK(q.size(0) == c.batch, "table must hold q's batch");
     const int64_t b = q.size(0), tokens = q.size(1), hq = q.size(2), d = q.size(3);
+    check_fp4_sizes(c, tokens);
     TORCH_CHECK(c.kv_heads > 0 && hq > 0 && hq % c.kv_heads == 0, "q heads (", hq,
                 ") must be a positive multiple of kv heads (", c.kv_heads, ")");
     TORCH_CHECK(softmax_scale > 0 && softmax_scale <= std::numeric_limits<float>::max(),

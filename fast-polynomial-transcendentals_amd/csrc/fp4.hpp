@@ -69,13 +69,14 @@ struct Fp4Pages {
 // ---- host side -----------------------------------------------------------------
 
 constexpr int64_t kFp4MostKeys = 1 << 30;    // of a sequence's table: positions are 32-bit
-constexpr int64_t kFp4MostTokens = 1 << 14;
+constexpr int64_t kFp4LooseTokens = 1 << 14;   // more have to fit the table
 
 inline bool fp4_sizes_ok(const spline_hip_fp4_cache* c, int64_t tokens) {
-    return c && c->batch >= 0 && c->batch <= 0x7fffffff && tokens >= 0 && tokens <= kFp4MostTokens && c->kv_heads > 0 &&
-           c->kv_heads <= 65536 && (c->head_dim == 64 || c->head_dim == 128) && c->page_size > 0 &&
-           c->page_size % kFp4Group == 0 && c->page_size <= 65536 && c->pages >= 0 && c->pages <= 0x7fffffff &&
-           c->entries >= 0 && c->entries <= kFp4MostKeys / c->page_size;
+    return c && c->batch >= 0 && c->batch <= 0x7fffffff && c->kv_heads > 0 && c->kv_heads <= 65536 &&
+           (c->head_dim == 64 || c->head_dim == 128) && c->page_size > 0 && c->page_size % kFp4Group == 0 &&
+           c->page_size <= 65536 && c->pages >= 0 && c->pages <= 0x7fffffff && c->entries >= 0 &&
+           c->entries <= kFp4MostKeys / c->page_size && tokens >= 0 &&
+           (tokens <= kFp4LooseTokens || tokens <= c->entries * c->page_size);
 }
 
 inline bool fp4_pointers_ok(const spline_hip_fp4_cache* c) {

@@ -1196,6 +1196,7 @@ bool plan(const spline_hip_fp4_cache* c, const spline_hip_fp4_attention* a, bool
     if (!a || !fp4_sizes_ok(c, a->tokens) || a->q_heads <= 0 || a->q_heads > 65536 || a->q_heads % c->kv_heads != 0)
         return false;
     const int64_t rows = a->tokens * (a->q_heads / c->kv_heads);
+    if (rows > 1 << 30) return false;  // of a sequence, in 32 bits
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.classes = 1;
     if (a->tokens == 1 && rows <= 8 && has_classes(a->mode, (int)c->head_dim, bf)) p.classes = rows > 4 ? 2 : 4;

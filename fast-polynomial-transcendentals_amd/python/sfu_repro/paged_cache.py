@@ -61,7 +61,8 @@ def store_fp4(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
     of the last T tokens of each sequence: token t at position ``lens[b] - T + t``.
 
     Tokens whose position is negative (left-padded batches), past the table or on an entry
-    without a page are left out.  A block's power of two 2^e puts its largest
+    without a page are left out; more than 16384 of them have to fit a row of the table, and a call
+    holds fewer than 2^34 elements of keys.  A block's power of two 2^e puts its largest
     magnitude into [3.5, 7) 2^e (-100 <= e <= 125); values are rounded to nearest, ties to even,
     the largest number being 6 2^e.  A block with an infinity or NaN reads as NaN.  A page that
     is written belongs to one sequence (:func:`fork_pages` sees to it): of two tokens of a call
@@ -74,7 +75,7 @@ def load_fp4(cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, token
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values ``[B, tokens, Hkv, head_dim]`` that the cache holds of the last
     ``tokens`` tokens of each sequence: exact in bfloat16, rounded and held to 65504 in float16;
-    zeros where a token has no place."""
+    zeros where a token has no place.  As many tokens as :func:`store_fp4` takes."""
     return tuple(_ops().paged_fp4_load(cache, table, lens, int(tokens), int(head_dim), dtype))
 
 

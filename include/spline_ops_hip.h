@@ -791,8 +791,8 @@ int launch_shared_prefix_attention_bf16(const spline_hip_shared_prefix* args, vo
  * stored there and nobody sees it.  lens: [batch] valid keys (negative: none), the
  * new tokens among them: of T new tokens of a call, token t is at position lens[b] -
  * T + t, and has none where that is negative or past the table (left-padded batches).
- * D 64 or 128, page_size a multiple of 16 up to 65536, at most 2^30 keys a table row,
- * 2^14 tokens. */
+ * D 64 or 128, page_size a multiple of 16 up to 65536, at most 2^30 keys a table row;
+ * more than 2^14 tokens only where a row holds them. */
 typedef struct spline_hip_fp4_cache {
     void* cache;
     const int32_t *table, *lens;
@@ -804,7 +804,8 @@ typedef struct spline_hip_fp4_cache {
  * 2^e is the one that puts its largest magnitude into [3.5, 7) 2^e, -100 <= e <= 125; values
  * are rounded to nearest, ties to the even code, held to 6 2^e.  A block with an
  * infinity or NaN is stored as NaN.  Pages that are written belong to one sequence:
- * two tokens of one call at one place leave either's bytes. */
+ * two tokens of one call at one place leave either's bytes.  B T Hkv D / 8 below
+ * 2^31 - 256. */
 int launch_paged_fp4_store_fp16(const spline_hip_fp4_cache* cache, const void* k, const void* v,
                                 const int64_t* k_strides, const int64_t* v_strides, int64_t tokens, void* stream);
 int launch_paged_fp4_store_bf16(const spline_hip_fp4_cache* cache, const void* k, const void* v,
@@ -823,10 +824,11 @@ int launch_paged_fp4_load_bf16(const spline_hip_fp4_cache* cache, void* k, void*
  * values enter the products exactly, FP16 queries as two BF16 terms;
  * sums are FP32; ahead of P V probabilities are BF16 in two terms, for any number of
  * tokens.  A NaN block in a key that a token sees makes its row NaN, in a value its
- * elements; what nobody sees may hold anything.  Time and workspace go by the keys in use, not by the table's
- * width.  Refused are more than 2^31 steps of 64 keys, over the tables' width, the KV
- * heads and every 64 rows.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the same
- * device (-1: sizes that are refused), 16-byte aligned; calls that may overlap need
+ * elements; what nobody sees may hold anything.  Time and workspace go by the keys in
+ * use, not by the table's width.  Refused are more than 2^31 steps of 64 keys, over the
+ * tables' width, the KV heads and every 64 rows, and more than 2^30 rows (T Hq / Hkv) a
+ * sequence.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the
+ * same device (-1: sizes that are refused), 16-byte aligned; calls that may overlap need
  * workspaces of their own. */
 typedef struct spline_hip_fp4_attention {
     void* out;
