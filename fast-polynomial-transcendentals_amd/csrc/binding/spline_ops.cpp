@@ -1330,6 +1330,14 @@ std::vector<at::Tensor> fork_pages(std::vector<at::Tensor> caches, at::Tensor ta
     call.a.out_lens = out_lens.data_ptr<int32_t>();
     call.a.page_size = page_size;
     call.a.grow = tokens;
+    TORCH_CHECK(spline_hip_fork_pages_workspace_bytes(&call.a) >= 0, "too many rows, entries, pages or tokens");
+    for (const at::Tensor& t : call.caches) {
+        // a cache of store_fp4: pages of rows of 64 / 2 + 64 / 32 bytes or twice that
+        if (t.scalar_type() != at::kByte || t.dim() != 4 || t.size(1) != 2 || t.size(3) == 0 || t.size(3) % (16 * 34) != 0) continue;
+        const int64_t rows = t.size(3) / 34;
+        TORCH_CHECK(page_size == rows || page_size * 2 == rows, "page_size ", page_size, " is not that of a cache whose pages hold ",
+                    rows, " rows of head_dim 64 or ", rows / 2, " of 128");
+    }
     call.launch(spline_hip_fork_pages_workspace_bytes, launch_fork_pages);
     return {call.out, out_lens, call.count};
 }

@@ -75,7 +75,8 @@ def load_fp4(cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, token
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values ``[B, tokens, Hkv, head_dim]`` that the cache holds of the last
     ``tokens`` tokens of each sequence: exact in bfloat16, rounded and held to 65504 in float16;
-    zeros where a token has no place.  As many tokens as :func:`store_fp4` takes."""
+    zeros where a token has no place.  As many tokens as :func:`store_fp4` takes.  ``head_dim`` is the
+    one that was stored: pages of 64 rows of 128 elements read as pages of 128 rows of 64."""
     return tuple(_ops().paged_fp4_load(cache, table, lens, int(tokens), int(head_dim), dtype))
 
 
@@ -94,6 +95,11 @@ def fork_pages(caches, table: torch.Tensor, lens: torch.Tensor, parents: torch.T
     ending a sequence is leaving it out, taking keys back is lowering its ``lens``, and
     rows may hold prefixes that nothing decodes.  New pages are the lowest free ones, in the
     order of rows and entries; other entries are -1.
+
+    ``page_size`` is the keys of a page in every one of ``caches``: a wrong one would share pages that are
+    still written.  Caches of :func:`fp4_cache` whose pages have not the bytes for it are refused (pages
+    of 64 rows of 128 elements have those of 128 rows of 64); what other caches hold is the caller's
+    (one of their shape, uint8 ``[pages, 2, heads, 544 n]``, is passed as ``cache.flatten(1)``).
 
     ``short`` (int32 ``[1]``) counts the pages that were wanted and not to be had, entries past
     the table's width among them; their entries are -1, and a row whose copy is missing has lost the
