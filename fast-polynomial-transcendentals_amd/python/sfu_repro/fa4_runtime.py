@@ -391,15 +391,17 @@ def flash_attn_bwd(q, k, v, out, dout, lse, softmax_scale=None, causal=False, so
                                             scale, cap, bias))
 
 
-def _serving_program(what, q, keys, softmax_scale, softcap, program):
+def _serving_program(what, q, softmax_scale, softcap, program):
     """(mode, cap, scale) of a serving attention, whose score programs are the softmax ones."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
     if not program:
         return (MODE_SOFTCAP_NATIVE, float(softcap), scale) if softcap and softcap > 0 else (MODE_SOFTMAX_NATIVE, 1.0, scale)
-    mode, _, cap, _ = select_forward(seqlen=max(1, keys), softcap=softcap, **program)
+    built = f"{what} is built with the hardware softmax, the hardware softcap and the D4 softcap"
+    if program.get("sigmoid_attention"):
+        raise NotImplementedError(built)
+    mode, _, cap, _ = select_forward(seqlen=1, softcap=softcap, **program)  # the sigmoid programs alone go by it
     if mode not in (MODE_SOFTMAX_NATIVE, MODE_SOFTCAP_NATIVE, MODE_SOFTCAP_D4):
-        raise NotImplementedError(
-            f"{what} is built with the hardware softmax, the hardware softcap and the D4 softcap")
+        raise NotImplementedError(built)
     if mode == MODE_SOFTCAP_D4 and q.dtype != torch.bfloat16:
         raise TypeError(f"the D4 softcap is a bfloat16 program, got {q.dtype}")
     return mode, cap, scale
@@ -427,8 +429,7 @@ def flash_attn_shared_prefix(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_l
     hardware softcap (``softcap``) and, for bfloat16, the D4 softcap (``score_mod``).
     There is no backward: operands that require gradients are refused.
     """
-    mode, cap, scale = _serving_program("the shared-prefix attention", q, prefix_k.shape[0], softmax_scale, softcap,
-                                        program)
+    mode, cap, scale = _serving_program("the shared-prefix attention", q, softmax_scale, softcap, program)
     return tuple(_ops().shared_prefix_attn_fwd(q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, mode, scale, cap))
 
 
@@ -452,7 +453,7 @@ def flash_attn_paged_fp4(q, cache, table, lens, softmax_scale=None, softcap=0.0,
     :func:`flash_attn_shared_prefix`.  There is no backward: queries that require
     gradients are refused.
     """
-    mode, cap, scale = _serving_program("the attention over 4-bit pages", q, 1, softmax_scale, softcap, program)
+    mode, cap, scale = _serving_program("the attention over 4-bit pages", q, softmax_scale, softcap, program)
     return tuple(_ops().paged_fp4_attn_fwd(q, cache, table, lens, mode, scale, cap))
 
 
