@@ -449,7 +449,8 @@ def flash_attn_paged_fp4(q, cache, table, lens, softmax_scale=None, softcap=0.0,
     float16 or bfloat16; head_dim 64 or 128; Hq a multiple of the cache's KV heads; any
     strides (operands that 16-byte loads cannot take are copied).  Keys and values enter
     the products as the cache holds them, without a rounding.  Time and workspace go by
-    the keys in use, not by the table's width.  More than 16384 tokens have to fit a row of the table.  The score program is that of
+    the keys in use, not by the table's width.  More than 16384 tokens have to fit a row of the table.
+    Sums are FP32: values of 2^120 over a row's keys and more may leave an infinity or NaN.  The score program is that of
     :func:`flash_attn_shared_prefix`.  There is no backward: queries that require
     gradients are refused.
     """

@@ -824,12 +824,15 @@ int launch_paged_fp4_load_bf16(const spline_hip_fp4_cache* cache, void* k, void*
  * values enter the products exactly, FP16 queries as two BF16 terms;
  * sums are FP32; ahead of P V probabilities are BF16 in two terms, for any number of
  * tokens.  A NaN block in a key that a token sees makes its row NaN, in a value its
- * elements; what nobody sees may hold anything.  Time and workspace go by the keys in
- * use, not by the table's width.  Refused are more than 2^31 steps of 64 keys, over the
- * tables' width, the KV heads and every 64 rows, and more than 2^30 rows (T Hq / Hkv) a
- * sequence.  workspace: spline_hip_paged_fp4_workspace_bytes of the same sizes on the
- * same device (-1: sizes that are refused), 16-byte aligned; calls that may overlap need
- * workspaces of their own. */
+ * elements; what nobody sees may hold anything.  FP32 ends what is computed: scores
+ * that pass it are infinite, and a row's probabilities are held to 2^8 ahead of the
+ * division by their sum, so that values of 2^120 over the row's keys and more may leave
+ * an infinity or NaN; results that pass FP16 are infinite in it.  Time and workspace go
+ * by the keys in use, not by the table's width.  Refused are more than 2^31 steps of 64
+ * keys, over the tables' width, the KV heads and every 64 rows, and more than 2^30 rows
+ * (T Hq / Hkv) a sequence.  workspace: spline_hip_paged_fp4_workspace_bytes of the same
+ * sizes on the same device (-1: sizes that are refused), 16-byte aligned; calls that may
+ * overlap need workspaces of their own. */
 typedef struct spline_hip_fp4_attention {
     void* out;
     float* lse;
