@@ -85,8 +85,10 @@ def fork_pages(caches, table: torch.Tensor, lens: torch.Tensor, parents: torch.T
     """``(table, lens, short)`` of new rows that continue old ones, with room for
     ``tokens`` more keys each.
 
-    New row i continues row ``parents[i]`` (int32, on the device; an id outside the rows: an
-    empty row; ``None``: row i) with its ``lens`` keys, held to the table.  A row may be
+    New row i continues row ``parents[i]`` (int32, on the device; ``None``: row i) with its ``lens``
+    keys, held to the table.  An id outside the rows is a place in the batch that nothing
+    uses: it gets no pages, whatever ``tokens`` is, and counts nothing in ``short``.  A new sequence
+    continues a row of no keys, which the table keeps for it (``lens`` 0; several may continue the same one).  A row may be
     continued by several, which share the pages that it has filled; the page that
     the next key goes to belongs to one row, the first that continues it, and is copied
     for every other, in each of ``caches`` (tensors of any kind ``[pages, ...]``, one a layer,

@@ -855,7 +855,8 @@ int launch_paged_fp4_attention_bf16(const spline_hip_fp4_cache* cache, const spl
  * page bytes multiples of 16: one a layer, of any kind, all with the same pages.
  *
  * launch_fork_pages: new row i of [rows][entries] continues row parents[i] (null: row
- * i, rows = old_rows or 0; outside 0 .. old_rows - 1: an empty row) with its lens keys, held
+ * i, rows = old_rows or 0; outside 0 .. old_rows - 1: a row without keys that gets no
+ * pages either; a new sequence continues an old row of no keys) with its lens keys, held
  * to 0 .. entries * page_size, which out_lens repeats.  Full pages are shared.  A last
  * page that is not full stays with the first new row that has it as its last, if no
  * row has it as a full one; the others get copies.  Rows get pages for `grow` more
