@@ -26,8 +26,9 @@
 // What bounds it: with few rows the bytes of K and V (17 a block of 32 elements), whose loads
 // alone take 91 us where 64 sequences of up to 16384 keys (571 MB) take 103 to 109, 6.2 TB/s a
 // further key and 15 us a call; from about 64 rows a KV head on the matrix cores and the
-// exponentials and conversions beside them: 4 x 512 tokens over 17408 keys 591 us, 974 TFLOP/s, over up
-// to 8700 keys each 178 us, 820 TFLOP/s, where first keys and results of 512 units count.
+// exponentials and conversions beside them: 4 x 512 tokens over 17408 keys 784 us, 734 TFLOP/s (half as
+// many products again are those of P's second terms), over up to 8700 keys each 222 us, 655 TFLOP/s, where
+// first keys and results of 512 units count.  FP16 queries, of two terms as well, take 1.2 times as long.
 // Two sequences of up to 131072 keys take 37 us, 8 of up to 1200 12 us, most of it latency: lengths,
 // table, codes and the join one behind the other.
 #include <hip/hip_runtime.h>
@@ -51,7 +52,7 @@ constexpr int kWideStep = 64;
 // units are counted together, so that the short ones leave theirs to the long one.
 constexpr int kPieces = 64;
 // A unit's first keys and its result cost as much as so many steps more: 4 x 512 tokens
-// over up to 8700 keys 262 us counting none, 222 with one, 202 with two, 188 with four, 190 with
+// over up to 8700 keys 311 us counting none, 280 with one, 254 with two, 231 with four, 238 with
 // eight; 64 decoding sequences 136, 131 with one or two, 135 with four.
 constexpr int unit_steps(int step) { return step == kWideStep ? 4 : 2; }
 
@@ -867,8 +868,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 
 // P enters P V in two BF16 terms, as in the kernels of fewer rows: a token's result is as exact,
 // whether it is decoded alone, verified among a few or part of a prompt.  One term, off by
 // 2^-8, is as large an error as the result's own rounding (root mean square 0.0023 instead of 0.0017)
-// and saves its products: 32 x 5 tokens over up to 4100 keys take 38 us with it, 43 with two,
-// 4 x 512 over 17408 keys 588 and 781.
+// and saves its products: 32 x 5 tokens over up to 4100 keys take 30 us with it, 33 with two,
+// 4 x 512 over up to 8700 keys 178 and 227, over 17408 588 and 781.
 
 // Rows of K are read 16 rows at a time, 16 bytes of each, rows of V transposed, four rows by
 // 64 bytes: 16 bytes lie between rows of K, 64 between those of V and 16 more between
